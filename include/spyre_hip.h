@@ -287,6 +287,65 @@ int sph_bmm_f16(int64_t batch, int64_t m, int64_t n, int64_t k,
                 const void* a, const void* b, void* d, sph_stream_t stream);
 
 /* ------------------------------------------------------------------ */
+/* 8-bit serving: OCP e4m3 codes with one fp32 scale for each group of  */
+/*   128 columns of a row (activations) or each block of 128 x 128      */
+/*   (weights).  No counterpart in the reference, which has no 8-bit    */
+/*   types; they stand where it runs its RMSNorm composite               */
+/*   (Metadata.yaml:236-253), silu and mul (base.jinja2:16-241) and     */
+/*   spyre__mm_default (spyre_torch_ops.cpp:214-293).                   */
+/*                                                                      */
+/* With amax the largest magnitude of a group, counted as at least      */
+/* 2^-100: scale = amax / 448, code = e4m3(v * (448 / amax)), rounded   */
+/* to nearest even.  A group that holds an infinity or a NaN has it as  */
+/* its scale.  Row r's codes are at q + r*ldq; the scale of its group g */
+/* (block row r / block_rows) at scale + r*scale_row_stride +           */
+/* g*scale_group_stride.  Nothing is written past a row's `cols` codes. */
+/* ------------------------------------------------------------------ */
+
+/* Codes of x [rows, cols] (row stride ldx), dtype in {F16, BF16, F32}, in
+ * groups of block_rows x 128 (block_rows 1 or 128). */
+int sph_quantize_fp8(sph_dtype dtype, const void* x, int64_t ldx, int64_t rows, int64_t cols,
+                     int64_t block_rows, void* q, int64_t ldq, float* scale,
+                     int64_t scale_row_stride, int64_t scale_group_stride, sph_stream_t stream);
+
+/* Codes of RMSNorm: y = h * rsqrt(mean(h^2) + eps) * weight, not rounded to
+ * dtype in between.  residual NULL: h = x (h_out unused); else h =
+ * round_to_dtype(x + residual), also written to h_out (which may be x or
+ * residual itself).  The codes are those of t = h * weight, the scales amax|t|
+ * * rsqrt(..) / 448.  dtype F16 / BF16; weight (may be NULL: 1) of w_dtype F32
+ * or dtype; cols at most 1048576. */
+int sph_rmsnorm_fp8(sph_dtype dtype, sph_dtype w_dtype, const void* x, int64_t ldx,
+                    const void* residual, int64_t ld_residual, const void* weight, void* h_out,
+                    int64_t ld_h, int64_t rows, int64_t cols, float eps, void* q, int64_t ldq,
+                    float* scale, int64_t scale_row_stride, int64_t scale_group_stride,
+                    sph_stream_t stream);
+
+/* Codes of silu(gu[:, :cols]) * gu[:, cols:2*cols] for gu [rows, 2*cols] (row
+ * stride ld), formed in fp32.  dtype F16 / BF16. */
+int sph_silu_mul_fp8(sph_dtype dtype, const void* gu, int64_t ld, int64_t rows, int64_t cols,
+                     void* q, int64_t ldq, float* scale, int64_t scale_row_stride,
+                     int64_t scale_group_stride, sph_stream_t stream);
+
+/* D[i, j] = sum_b xs[i, b] ws[j / 128, b] sum_{p in group b} X[i, p] W[j, p]
+ * + bias[j], rounded once to dtype (F16 or BF16): X [m, k] and W [n, k] are
+ * codes, xs and ws their scales by element strides, bias (may be NULL) has
+ * dtype.  Group sums come from the 8-bit matrix instruction, whose own sum is
+ * off by up to some 1e-5 of the terms' magnitudes (so no fp32 result is
+ * offered), scales and their accumulation are fp32; products of two scales
+ * have to be finite.  Rows of X and W must begin on 16 bytes (else
+ * SPH_ERR_UNSUPPORTED) and are read in whole aligned 16-byte chunks; what lies
+ * past k in the last one does not count.  workspace (may be NULL) of
+ * sph_gemm_fp8_workspace_bytes(m, n, k) bytes (0 for many shapes) lets the K
+ * range be split over workgroups; calls sharing one must be ordered on a
+ * stream. */
+int sph_gemm_fp8(sph_dtype dtype, int64_t m, int64_t n, int64_t k, const void* x, int64_t ldx,
+                 const float* x_scale, int64_t x_scale_row_stride, int64_t x_scale_group_stride,
+                 const void* w, int64_t ldw, const float* w_scale, int64_t w_scale_row_stride,
+                 int64_t w_scale_group_stride, const void* bias, void* d, int64_t ldd,
+                 void* workspace, int64_t workspace_bytes, sph_stream_t stream);
+int64_t sph_gemm_fp8_workspace_bytes(int64_t m, int64_t n, int64_t k);
+
+/* ------------------------------------------------------------------ */
 /* Fused attention forward                                              */
 /* Replaces: the chain the reference runs for attention, spyre__bmm_    */
 /*   default (spyre_torch_ops.cpp:297-377) for the scores, the          */

@@ -72,6 +72,14 @@ _SIGS = {
                           c_int, vp], c_int),
     "sph_gemm_f16": ([c_i64, c_i64, c_i64, vp, vp, vp, vp], c_int),
     "sph_bmm_f16": ([c_i64, c_i64, c_i64, c_i64, vp, vp, vp, vp], c_int),
+    "sph_quantize_fp8": ([c_int, vp, c_i64, c_i64, c_i64, c_i64, vp, c_i64, vp, c_i64, c_i64, vp],
+                         c_int),
+    "sph_rmsnorm_fp8": ([c_int, c_int, vp, c_i64, vp, c_i64, vp, vp, c_i64, c_i64, c_i64, c_f32, vp,
+                         c_i64, vp, c_i64, c_i64, vp], c_int),
+    "sph_silu_mul_fp8": ([c_int, vp, c_i64, c_i64, c_i64, vp, c_i64, vp, c_i64, c_i64, vp], c_int),
+    "sph_gemm_fp8": ([c_int, c_i64, c_i64, c_i64, vp, c_i64, vp, c_i64, c_i64, vp, c_i64, vp, c_i64,
+                      c_i64, vp, vp, c_i64, vp, c_i64, vp], c_int),
+    "sph_gemm_fp8_workspace_bytes": ([c_i64, c_i64, c_i64], c_i64),
     "sph_attention_fwd": ([c_int, c_i64, c_i64, c_i64, c_i64, vp, c_i64, c_i64, vp, c_i64,
                            c_i64, vp, c_i64, c_i64, vp, c_i64, c_i64, c_i64, c_i64, c_f32, vp,
                            c_i64, c_i64, vp, c_i64, vp], c_int),

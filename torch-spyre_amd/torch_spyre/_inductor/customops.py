@@ -419,3 +419,251 @@ def _(qkv, cos, sin, pos, k_cache, v_cache, n_heads, n_kv_heads, scale, v_dim_ma
 @decode_attention.register_fake
 def _(qkv, cos, sin, pos, k_cache, v_cache, n_heads, n_kv_heads, scale, v_dim_major):
     return qkv.new_empty((qkv.shape[0], n_heads * k_cache.shape[-1]))
+
+
+# ---- 8-bit serving: e4m3 codes with a scale for each group of 128 ------------
+#
+# These are defined without the custom_op wrapper, and their spyre kernels are
+# registered in C++ (torch_spyre/_C, ops_fp8.cpp): the wrapper costs 11 us of
+# host time a call, a plain operator 3, and a decode step makes four of these
+# calls per projection and layer.  Elsewhere they run as the formulas below.
+# The reference has no 8-bit types; what a user of it writes for the same layer
+# is its RMSNorm composite (codegen/inputs/Metadata.yaml:236-253), silu and mul
+# (base.jinja2:16-241) and spyre__mm_default (spyre_torch_ops.cpp:214-293).
+
+FP8_GROUP = 128          # columns of one scale; rows of a weight's blocks
+FP8_TOP = 448.0          # e4m3's largest finite value
+FP8_LEAST = 2.0 ** -100  # a group's largest magnitude counts as at least this
+
+_FP8_SCHEMAS = {
+    "quantize_fp8": "(Tensor x, int block_rows=1) -> (Tensor, Tensor)",
+    "rms_norm_fp8": "(Tensor x, Tensor? weight, float eps) -> (Tensor, Tensor)",
+    "add_rms_norm_fp8": "(Tensor x, Tensor residual, Tensor? weight, float eps) "
+                        "-> (Tensor, Tensor, Tensor)",
+    "silu_mul_fp8": "(Tensor gate_up) -> (Tensor, Tensor)",
+    "mm_fp8": "(Tensor x, Tensor x_scale, Tensor w, Tensor w_scale, ScalarType dtype, "
+              "Tensor? bias=None) -> Tensor",
+}
+for _name, _schema in _FP8_SCHEMAS.items():
+    torch.library.define(f"spyre::{_name}", _schema)
+
+
+def _fp8_check(cond: bool, message: str) -> None:
+    if not cond:
+        raise RuntimeError(message)
+
+
+def _fp8_groups(n: int) -> int:
+    return -(-n // FP8_GROUP)
+
+
+def _fp8_empty(x: torch.Tensor, shape) -> tuple[torch.Tensor, torch.Tensor]:
+    """Uninitialised codes of `shape` (rows off 16 bytes padded to the next 16,
+    so that a product can read them in whole chunks) and their scales [...,
+    groups], a group's scales of all rows side by side."""
+    shape = list(shape)
+    q = x.new_empty(shape[:-1] + [-(-shape[-1] // 16) * 16], dtype=torch.float8_e4m3fn)
+    if shape[-1] % 16:
+        q = q.narrow(-1, 0, shape[-1])
+    rows, ng = 1, _fp8_groups(shape[-1])
+    for n in shape[:-1]:
+        rows *= n
+    s = x.new_empty((ng, rows), dtype=torch.float32)
+    return q, s.t().view(shape[:-1] + [ng])
+
+
+def _fp8_blocks_empty(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    q, _ = _fp8_empty(x, x.shape)
+    return q, x.new_empty([_fp8_groups(n) for n in x.shape], dtype=torch.float32)
+
+
+def _fp8_codes(v: torch.Tensor, block_rows: int = 1):
+    """(codes, amax) of fp32 v [R, C] in groups of block_rows x 128."""
+    r, c = v.shape
+    rb, cb = -(-r // block_rows), _fp8_groups(c)
+    p = v.new_zeros(rb * block_rows, cb * FP8_GROUP)
+    p[:r, :c] = v
+    p = p.view(rb, block_rows, cb, FP8_GROUP)
+    amax = p.abs().amax((1, 3), keepdim=True).clamp(min=FP8_LEAST)
+    # (a quotient of tensors: FP8_TOP / amax would multiply by a reciprocal)
+    q = (p * (torch.full_like(amax, FP8_TOP) / amax)).to(torch.float8_e4m3fn)
+    return q.view(rb * block_rows, cb * FP8_GROUP)[:r, :c], amax[:, 0, :, 0]
+
+
+def _fp8_fill(x: torch.Tensor, v: torch.Tensor, shape, row_factor=None):
+    """Codes and scales of fp32 v, the rows of `shape`; row_factor [R, 1]: a
+    positive factor of each row that its scales take on."""
+    q, s = _fp8_empty(x, shape)
+    if v.numel() == 0:
+        return q, s
+    codes, amax = _fp8_codes(v)
+    q.copy_(codes.reshape(shape))
+    s.copy_(((amax if row_factor is None else amax * row_factor) / FP8_TOP).reshape(s.shape))
+    return q, s
+
+
+def _fp8_no_grad(name: str, *tensors) -> None:
+    _fp8_check(not (torch.is_grad_enabled() and
+                    any(t is not None and t.requires_grad for t in tensors)),
+               f"spyre::{name} has no gradient: call it under torch.no_grad()")
+
+
+def _quantize_fp8_check(x, block_rows):
+    _fp8_check(x.dtype in (torch.float16, torch.bfloat16, torch.float32),
+               f"quantize_fp8: x must be fp16, bf16 or fp32, got {x.dtype}")
+    _fp8_check(block_rows in (1, FP8_GROUP),
+               f"quantize_fp8: block_rows must be 1 or 128, got {block_rows}")
+    _fp8_check(block_rows == 1 or x.dim() == 2,
+               "quantize_fp8: blocks of 128 rows need a 2-dimensional x")
+    _fp8_check(x.dim() >= 1, "quantize_fp8: needs at least one dimension")
+
+
+@torch.library.impl("spyre::quantize_fp8", "CompositeExplicitAutograd")
+def quantize_fp8(x: torch.Tensor, block_rows: int = 1):
+    """e4m3 codes and fp32 scales of x [..., K]: with amax the largest
+    magnitude of a group (1 x 128 columns, or with block_rows 128 a block of
+    128 x 128 of a 2-D x; at least 2^-100), scale = amax / 448 and codes =
+    e4m3(x * (448 / amax)).  Returns (codes [..., K], scales [..., ceil(K /
+    128)] or [ceil(N / 128), ceil(K / 128)]).  A group that holds an infinity
+    or a NaN has it as its scale."""
+    _quantize_fp8_check(x, block_rows)
+    _fp8_no_grad("quantize_fp8", x)
+    if block_rows == 1:
+        return _fp8_fill(x, x.reshape(-1, x.shape[-1]).float() if x.numel() else x, x.shape)
+    q, s = _fp8_blocks_empty(x)
+    if x.numel():
+        codes, amax = _fp8_codes(x.float(), block_rows)
+        q.copy_(codes)
+        s.copy_(amax / FP8_TOP)
+    return q, s
+
+
+@torch.library.register_fake("spyre::quantize_fp8")
+def _(x, block_rows=1):
+    _quantize_fp8_check(x, block_rows)
+    return _fp8_empty(x, x.shape) if block_rows == 1 else _fp8_blocks_empty(x)
+
+
+def _rms_norm_fp8_check(name, x, residual, weight):
+    _fp8_check(x.dtype in (torch.float16, torch.bfloat16),
+               f"{name}: x must be fp16 or bf16, got {x.dtype}")
+    _fp8_check(x.dim() >= 1, f"{name}: needs at least one dimension")
+    _fp8_check(residual is None or (residual.shape == x.shape and residual.dtype == x.dtype),
+               f"{name}: residual must have x's shape and type")
+    _fp8_check(weight is None or weight.shape == (x.shape[-1],),
+               f"{name}: weight must be [{x.shape[-1]}]")
+    _fp8_check(weight is None or weight.dtype in (x.dtype, torch.float32),
+               f"{name}: weight must have x's type or fp32")
+
+
+def _rms_norm_fp8(h, weight, eps):
+    f = h.reshape(-1, h.shape[-1]).float() if h.numel() else h.float()
+    rstd = torch.rsqrt((f * f).mean(-1, keepdim=True) + eps)
+    return _fp8_fill(h, f if weight is None else f * weight.float(), h.shape, rstd)
+
+
+@torch.library.impl("spyre::rms_norm_fp8", "CompositeExplicitAutograd")
+def rms_norm_fp8(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float):
+    """(codes, scales) of rms_norm(x, weight, eps) over the last dimension,
+    without rounding it to x's type in between.  The codes are those of x *
+    weight: the row's 1 / rms is a factor of its scales alone."""
+    _rms_norm_fp8_check("rms_norm_fp8", x, None, weight)
+    _fp8_no_grad("rms_norm_fp8", x, weight)
+    return _rms_norm_fp8(x, weight, eps)
+
+
+@torch.library.register_fake("spyre::rms_norm_fp8")
+def _(x, weight, eps):
+    _rms_norm_fp8_check("rms_norm_fp8", x, None, weight)
+    return _fp8_empty(x, x.shape)
+
+
+@torch.library.impl("spyre::add_rms_norm_fp8", "CompositeExplicitAutograd")
+def add_rms_norm_fp8(x: torch.Tensor, residual: torch.Tensor, weight: Optional[torch.Tensor],
+                     eps: float):
+    """(codes, scales, h) with h = x + residual in x's type, normalised as
+    rms_norm_fp8 does."""
+    _rms_norm_fp8_check("add_rms_norm_fp8", x, residual, weight)
+    _fp8_no_grad("add_rms_norm_fp8", x, residual, weight)
+    h = (x + residual).contiguous()
+    return (*_rms_norm_fp8(h, weight, eps), h)
+
+
+@torch.library.register_fake("spyre::add_rms_norm_fp8")
+def _(x, residual, weight, eps):
+    _rms_norm_fp8_check("add_rms_norm_fp8", x, residual, weight)
+    return (*_fp8_empty(x, x.shape), x.new_empty(x.shape))
+
+
+def _silu_mul_fp8_check(gate_up):
+    _fp8_check(gate_up.dtype in (torch.float16, torch.bfloat16),
+               f"silu_mul_fp8: gate_up must be fp16 or bf16, got {gate_up.dtype}")
+    _fp8_check(gate_up.dim() >= 1, "silu_mul_fp8: needs at least one dimension")
+    _fp8_check(gate_up.shape[-1] % 2 == 0,
+               f"silu_mul_fp8: the last dimension must be even, got {gate_up.shape[-1]}")
+
+
+@torch.library.impl("spyre::silu_mul_fp8", "CompositeExplicitAutograd")
+def silu_mul_fp8(gate_up: torch.Tensor):
+    """(codes, scales) of silu(gate_up[..., :n]) * gate_up[..., n:] for
+    gate_up [..., 2n], formed in fp32."""
+    _silu_mul_fp8_check(gate_up)
+    _fp8_no_grad("silu_mul_fp8", gate_up)
+    n = gate_up.shape[-1] // 2
+    shape = list(gate_up.shape[:-1]) + [n]
+    gu = gate_up.reshape(-1, 2 * n).float() if gate_up.numel() else gate_up.float()
+    return _fp8_fill(gate_up, torch.nn.functional.silu(gu[..., :n]) * gu[..., n:], shape)
+
+
+@torch.library.register_fake("spyre::silu_mul_fp8")
+def _(gate_up):
+    _silu_mul_fp8_check(gate_up)
+    return _fp8_empty(gate_up, list(gate_up.shape[:-1]) + [gate_up.shape[-1] // 2])
+
+
+def _mm_fp8_check(x, x_scale, w, w_scale, dtype, bias):
+    _fp8_check(x.dtype == w.dtype == torch.float8_e4m3fn,
+               f"mm_fp8: x and w must be float8_e4m3fn, got {x.dtype} and {w.dtype}")
+    _fp8_check(x_scale.dtype == w_scale.dtype == torch.float32,
+               "mm_fp8: the scales must be fp32")
+    _fp8_check(dtype in (torch.float16, torch.bfloat16),
+               f"mm_fp8: the result must be fp16 or bf16, got {dtype}")
+    _fp8_check(x.dim() >= 1 and w.dim() == 2 and x.shape[-1] == w.shape[1],
+               f"mm_fp8: x must be [..., K] and w [N, K], got {tuple(x.shape)} and "
+               f"{tuple(w.shape)}")
+    kb = _fp8_groups(w.shape[1])
+    want = tuple(x.shape[:-1]) + (kb,)
+    _fp8_check(tuple(x_scale.shape) == want,
+               f"mm_fp8: x_scale must be {list(want)}, got {list(x_scale.shape)}")
+    want = (_fp8_groups(w.shape[0]), kb)
+    _fp8_check(tuple(w_scale.shape) == want,
+               f"mm_fp8: w_scale must be {list(want)}, got {list(w_scale.shape)}")
+    _fp8_check(bias is None or (bias.shape == (w.shape[0],) and bias.dtype == dtype),
+               f"mm_fp8: bias must be [{w.shape[0]}] of the result's type")
+
+
+@torch.library.impl("spyre::mm_fp8", "CompositeExplicitAutograd")
+def mm_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+           dtype: torch.dtype, bias: Optional[torch.Tensor] = None):
+    """y[..., j] = sum_k x[..., k] x_scale[..., k / 128] w[j, k] w_scale[j /
+    128, k / 128] + bias[j] in `dtype` (fp16 or bf16), for codes x [..., K]
+    with their scales (quantize_fp8, rms_norm_fp8, silu_mul_fp8) and a weight
+    w [N, K] quantised in blocks of 128 x 128.  The products of two scales have
+    to be finite."""
+    _mm_fp8_check(x, x_scale, w, w_scale, dtype, bias)
+    _fp8_no_grad("mm_fp8", x_scale, w_scale, bias)
+    k = w.shape[1]
+    if x.numel() == 0 or w.numel() == 0:
+        y = x_scale.new_zeros(list(x.shape[:-1]) + [w.shape[0]])
+    else:
+        xf = x.float() * x_scale.repeat_interleave(FP8_GROUP, -1)[..., :k]
+        wf = w.float() * w_scale.repeat_interleave(FP8_GROUP, 0)[:w.shape[0]].repeat_interleave(
+            FP8_GROUP, 1)[:, :k]
+        y = xf @ wf.t()
+    return (y if bias is None else y + bias.float()).to(dtype)
+
+
+@torch.library.register_fake("spyre::mm_fp8")
+def _(x, x_scale, w, w_scale, dtype, bias=None):
+    _mm_fp8_check(x, x_scale, w, w_scale, dtype, bias)
+    return x.new_empty(list(x.shape[:-1]) + [w.shape[0]], dtype=dtype)

@@ -334,7 +334,8 @@ int sph_silu_mul_fp8(sph_dtype dtype, const void* gu, int64_t ld, int64_t rows, 
  * offered), scales and their accumulation are fp32; products of two scales
  * have to be finite.  Rows of X and W must begin on 16 bytes (else
  * SPH_ERR_UNSUPPORTED) and are read in whole aligned 16-byte chunks; what lies
- * past k in the last one does not count.  workspace (may be NULL) of
+ * past k in the last one does not count.  m is at most 1048560, k, ldx and ldw
+ * at most 4194303, x_scale_row_stride at most 2097152.  workspace (may be NULL) of
  * sph_gemm_fp8_workspace_bytes(m, n, k) bytes (0 for many shapes) lets the K
  * range be split over workgroups; calls sharing one must be ordered on a
  * stream. */
@@ -344,6 +345,16 @@ int sph_gemm_fp8(sph_dtype dtype, int64_t m, int64_t n, int64_t k, const void* x
                  int64_t w_scale_group_stride, const void* bias, void* d, int64_t ldd,
                  void* workspace, int64_t workspace_bytes, sph_stream_t stream);
 int64_t sph_gemm_fp8_workspace_bytes(int64_t m, int64_t n, int64_t k);
+
+/* What a product of these sizes runs on, without launching it (host only):
+ * plan[0] the kernel, [1] and [2] its tile (rows of X, rows of W), [3] the K
+ * slices of its tiles. */
+typedef enum sph_fp8_kernel {
+  SPH_FP8_STREAM = 1, /* few rows, straight from memory */
+  SPH_FP8_RING = 2,   /* ring of LDS stages, small and ragged rows */
+  SPH_FP8_TILES = 3   /* 256 rows of X by 192 or 256 of W, persistent */
+} sph_fp8_kernel;
+int sph_gemm_fp8_plan(int64_t m, int64_t n, int64_t k, int64_t workspace_bytes, int32_t* plan);
 
 /* ------------------------------------------------------------------ */
 /* Fused attention forward                                              */

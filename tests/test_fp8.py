@@ -19,6 +19,7 @@ Expected values come from plain 64-bit arithmetic here.  Tolerances:
     of magnitudes, plus half a step of the result's type.
 """
 
+import ctypes
 import math
 
 import pytest
@@ -256,7 +257,28 @@ MM_SHAPES = [(1, 1, 1), (1, 128, 128), (1, 6144, 4096), (2, 16, 64), (3, 130, 25
              (8, 256, 12800), (9, 300, 384), (16, 129, 130), (17, 640, 2048), (24, 515, 4096),
              (33, 1000, 512), (64, 256, 1024), (65, 96, 48), (100, 384, 4096), (128, 512, 640),
              (130, 257, 1300), (200, 1024, 2048), (256, 256, 128), (257, 513, 384),
-             (333, 640, 4096), (512, 768, 1024), (777, 1100, 272), (300, 2048, 16)]
+             (333, 640, 4096), (512, 768, 1024), (777, 1100, 272), (300, 2048, 16),
+             (24, 4096, 12800), (70, 5000, 1024), (600, 3200, 1920), (1030, 2000, 1310),
+             (777, 6144, 1045), (333, 4096, 6500), (2048, 6144, 512), (1300, 8256, 1024), (1800, 10300, 256), (4096, 9000, 384)]
+
+
+def plan(m, n, k, workspace=None):
+    """(kernel, tile, K slices) that the library runs a product on (host only)."""
+    lib, out = _capi.lib(), (ctypes.c_int32 * 4)()
+    if workspace is None:
+        workspace = lib.sph_gemm_fp8_workspace_bytes(m, n, k)
+    assert lib.sph_gemm_fp8_plan(m, n, k, workspace, ctypes.addressof(out)) == 0
+    return {1: "stream", 2: "ring", 3: "tiles"}[out[0]], (out[1], out[2]), out[3]
+
+
+def test_mm_shapes_cover_every_kernel():
+    seen = {plan(*s)[:2] for s in MM_SHAPES}
+    assert seen == {("stream", (16, 16)), ("ring", (32, 64)), ("ring", (32, 128)),
+                    ("ring", (64, 128)), ("ring", (128, 128)), ("tiles", (256, 192)),
+                    ("tiles", (256, 256))}
+    assert {plan(*s)[2] > 1 for s in MM_SHAPES} == {True, False}
+    # without a workspace nothing is split
+    assert all(plan(*s, 0)[2] == 1 for s in MM_SHAPES)
 
 
 @pytest.mark.gpu

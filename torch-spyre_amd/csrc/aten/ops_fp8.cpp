@@ -224,6 +224,7 @@ at::Tensor mm_fp8(const at::Tensor& x_in, const at::Tensor& x_scale, const at::T
   const Rows x = code_rows(x_in, op), w = code_rows(w_in, op);
   // x_scale as [rows, kb] by two strides
   at::Tensor xs = x_scale.dim() == 2 ? x_scale : x_scale.reshape({x.rows, kb});
+  if (xs.stride(0) > (1 << 21)) xs = contiguous_on_device(xs);  // the entry point's limit
   std::vector<int64_t> shape(x_in.sizes().begin(), x_in.sizes().end());
   shape.back() = n;
   at::Tensor out = empty_spyre(shape, dtype, x_in.device());

@@ -8,127 +8,68 @@
 // accumulator.  W is the MFMA's first operand: a lane then holds 4 consecutive
 // columns j of one row i, all its elements of a 16-row tile share one scale
 // xs[i, b] ws[j / 128, b], and that product is one multiplication per tile.
-#include "fp8_common.h"
-#include "gemm_tile.h"
+#include <algorithm>
+
+#include "gemm_fp8.h"
 
 namespace sph {
 namespace {
 
-using fp8::kGroup;
-
-typedef int i32x8 __attribute__((ext_vector_type(8)));
-
-struct Fp8Args {
-  int64_t m, n, k;
-  const uint8_t* x;
-  int64_t ldx;
-  const float* xs;
-  int64_t xs_row, xs_blk;
-  const uint8_t* w;
-  int64_t ldw;
-  const float* ws;
-  int64_t ws_row, ws_blk;
-  const void* bias;
-  void* d;
-  int64_t ldd;
-  int tiles_m, tiles_n;
-};
-
-__device__ inline i32x8 frag(u32x4 lo, u32x4 hi) {
-  return __builtin_shufflevector(__builtin_bit_cast(i32x4, lo), __builtin_bit_cast(i32x4, hi), 0, 1,
-                                 2, 3, 4, 5, 6, 7);
-}
-
-// (Scale operands of 0 select the unscaled form of the instruction.)
-__device__ inline f32x4 mfma_block(i32x8 a, i32x8 b) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0,
-                                                          0, 0, 0);
-}
-
-// v with zeros from byte `left` on.
-__device__ inline u32x4 keep_bytes(u32x4 v, int left) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int nb = left - 4 * i;
-    v[i] &= nb >= 4 ? ~0u : nb <= 0 ? 0u : (1u << (8 * nb)) - 1u;
-  }
-  return v;
-}
-
-template <typename T>
-__device__ inline uint32_t pack2(float a, float b) {
-  return static_cast<uint32_t>(__builtin_bit_cast(uint16_t, Num<T>::from_f(a))) |
-         (static_cast<uint32_t>(__builtin_bit_cast(uint16_t, Num<T>::from_f(b))) << 16);
-}
-
-// 16 codes at row[p], zeros from K on.  `row` and p are multiples of 16 bytes,
-// so a chunk that begins inside the row is read whole: it cannot leave the page.
-__device__ inline u32x4 load_chunk(const uint8_t* row, int64_t p, int64_t k) {
-  const u32x4 v = *reinterpret_cast<const u32x4*>(row + (p < k ? p : 0));
-  return keep_bytes(v, static_cast<int>(k - p));
-}
-
-// The operand of block b for 16 rows: lane l holds row l % 16, chunks l / 16
-// and l / 16 + 4 of the block (any order of K serves that both operands share).
-__device__ inline i32x8 load_frag(const uint8_t* row, int64_t b, int64_t k, int g4) {
-  const int64_t p = b * kGroup + 16 * g4;
-  return frag(load_chunk(row, p, k), load_chunk(row, p + 64, k));
-}
-
 // ---------------------------------------------------------------------------
-// Large products: tiles of BN of W's rows by 256 of X's, direct global -> LDS
-// loads, the layout of the 16-bit direct-load kernel (a row's block of 128
-// codes is 8 chunks of 16 bytes, chunk c of row r at slot c ^ ((r >> 1) & 7)).
+// Large products: persistent workgroups, one per CU, over tiles of BN of W's
+// rows by 256 of X's, direct global -> LDS loads in the layout of the 16-bit
+// direct-load kernel (a row's block of 128 codes is 8 chunks of 16 bytes, chunk c
+// of row r at slot c ^ ((r >> 1) & 7)).
 //
 //   * 8 waves (2 along W's rows, 4 along X's), each TN x 4 MFMA tiles.  A K step
 //     is one block: TN * 4 MFMAs of 32 cycles, each followed LAG MFMAs later by
 //     its 4 FMAs, so the matrix core runs while the vector ALU scales.
-//   * Registers, not LDS, limit the overlap (TN * 16 accumulators of 256), so
-//     the fragments are not double-buffered as a whole: W's go through a ring
-//     of 4, each slot refilled after its last use; an X fragment is refilled
-//     for the next step right after its use by the last row of tiles.
+//   * Registers limit the overlap (TN * 16 accumulators of 256), so the
+//     fragments are not double-buffered as a whole: W's go through a ring of 4,
+//     each slot refilled after its last use; an X fragment is refilled for the
+//     next step right after its use by the last row of tiles.
 //   * The barrier that hands over the stages comes before MFMA XB, where every
 //     fragment of the present stage has been read; after it come the reads of
 //     the next stage and the loads of the block after it into the stage just
-//     left.
-//   * Scales come by ordinary loads, two steps ahead, and are multiplied
-//     right behind the barrier's wait, so that the wait which the compiler adds
-//     for them finds nothing left in flight.
+//     left.  That stream of blocks runs on into the next tile, so a tile's first
+//     blocks land while the one before is finished and stored.
+//   * A block's scales ride in its stage: waves 0 to 3 fetch X's, 4 and 5 those
+//     of W's first 128 rows (of a 192-row tile: its first block), 6 and 7 the
+//     next.
 // ---------------------------------------------------------------------------
 namespace dl8 {
-constexpr uint32_t kOutside = 0x80000000u;  // past every buffer resource
-constexpr int TM = 4, LAG = 2;
-template <int TN_, int WN_, int WM_>
+constexpr int TM = 4, LAG = 2, WN = 2, WM = 4, NW = 8, NT = 512, BM = 256;
+template <int TN_>
 struct Cfg {
-  static constexpr int TN = TN_, WN = WN_, WM = WM_, NW = WN * WM, NT = NW * 64;
-  static constexpr int WTN = TN * 16, BN = WN * WTN, BM = WM * TM * 16, NMF = TN * TM;
-  static constexpr int W_BYTES = BN * kGroup, X_BYTES = BM * kGroup, STAGE = W_BYTES + X_BYTES;
+  static constexpr int TN = TN_, WTN = TN * 16, BN = WN * WTN, NMF = TN * TM;
+  static constexpr int W_BYTES = BN * kGroup, X_BYTES = BM * kGroup, S_BYTES = NW * 256;
+  static constexpr int STAGE = W_BYTES + X_BYTES + S_BYTES;
   static constexpr int LW = W_BYTES / 1024 / NW, LX = X_BYTES / 1024 / NW, L = LW + LX;
   static_assert(LW * NW * 1024 == W_BYTES && LX * NW * 1024 == X_BYTES, "load lines");
-  static constexpr int XB = (TN - 3) * TM;  // the last W fragment is read 4 MFMAs before
-  static_assert(NMF - XB >= L, "loads fit behind the barrier");
-  static constexpr int SP = WTN + 8;  // epilogue pitch (elements)
-  static_assert(NW * 16 * SP * 2 <= 2 * STAGE, "epilogue slabs fit");
+  // The barrier: behind the present block's last W fragment (read after row of
+  // tiles TN - 5), before the next block's first (read after row TN - 4).
+  static constexpr int XB = (TN - 4) * TM + TM - 1;
+  static_assert(NMF - XB > L, "loads fit behind the barrier");
+  // Tiles of a wave that certainly share W's block: all of 128 rows, pairs of
+  // the 96 that begin on multiples of 32 in a block.
+  static constexpr int NC = TN == 8 ? 1 : TN / 2, CT = TN / NC;
+  static_assert(TN == 8 || TN == 6, "256- or 192-row tiles of W");
 };
 }  // namespace dl8
 
-template <typename T, int TN_, int WN_, int WM_>
-__global__ void __launch_bounds__(WN_ * WM_ * 64) gemm_fp8_dl_kernel(const Fp8Args p) {
+template <typename T, int TN_>
+__global__ void __launch_bounds__(dl8::NT) gemm_fp8_dl_kernel(const Fp8Args p) {
   using namespace dl8;
-  using C = Cfg<TN_, WN_, WM_>;
-  constexpr int TN = C::TN, STAGE = C::STAGE, NMF = C::NMF, WM = C::WM, BM = C::BM, NT = C::NT;
+  using C = Cfg<TN_>;
+  constexpr int TN = C::TN, STAGE = C::STAGE, NMF = C::NMF, BN = C::BN, NC = C::NC;
   __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
-  int tm, tn;
-  tile_of(blockIdx.x, p.tiles_m, p.tiles_n, tm, tn);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int wn = wave / WM, wm = wave % WM, r16 = lane & 15, g4 = lane >> 4;
-  const int64_t m0 = static_cast<int64_t>(tm) * BM, n0 = static_cast<int64_t>(tn) * C::BN;
+  const int lane = threadIdx.x & 63, r16 = lane & 15, g4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int wn = wave / WM, wm = wave % WM;
   const int k = static_cast<int>(p.k), ldx = static_cast<int>(p.ldx), ldw = static_cast<int>(p.ldw);
-  const int ksteps = k / kGroup;  // whole blocks
-  const int xrows = static_cast<int>(min(static_cast<int64_t>(BM), p.m - m0));
-  const int wrows = static_cast<int>(min(static_cast<int64_t>(C::BN), p.n - n0));
-  const i32x4 rx = buffer_rsrc(p.x + m0 * p.ldx, static_cast<uint32_t>((xrows - 1) * ldx + ksteps * kGroup));
-  const i32x4 rw = buffer_rsrc(p.w + n0 * p.ldw, static_cast<uint32_t>((wrows - 1) * ldw + ksteps * kGroup));
+  const int ksteps = k / kGroup;  // K is whole blocks, at least 2
+  const int ntiles = p.tiles_m * p.tiles_n;
+  const uint32_t lds_base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((SPH_LDS char*)(lds)));
   // Lane offsets of this wave's load lines (8 rows of 8 chunks each) 0 and 1;
   // lines two apart differ by 16 rows.  Rows past the last lie outside the
   // resource.
@@ -139,241 +80,215 @@ __global__ void __launch_bounds__(WN_ * WM_ * 64) gemm_fp8_dl_kernel(const Fp8Ar
     vw[i] = static_cast<uint32_t>(rw_ * ldw + (((lane & 7) ^ ((rw_ >> 1) & 7)) << 4));
     vx[i] = static_cast<uint32_t>(rx_ * ldx + (((lane & 7) ^ ((rx_ >> 1) & 7)) << 4));
   }
-  const uint32_t lds_base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((SPH_LDS char*)(lds)));
-  // Load line l (W's first) of block t into stage st & 1.
-  auto dma = [&](int t, int st, int l) __attribute__((always_inline)) {
+  // Where the load stream stands: its tile's resources and block.
+  struct Stream {
+    i32x4 rx, rw, rs;
+    const float* sb;
+    int64_t sblk;
+    uint32_t sbytes, vs;
+    int t, tile;
+  } ld;
+  auto open = [&](int tile) __attribute__((always_inline)) {
+    int tm, tn;
+    tile_of(tile, p.tiles_m, p.tiles_n, tm, tn);
+    const int64_t m0 = static_cast<int64_t>(tm) * BM, n0 = static_cast<int64_t>(tn) * BN;
+    const int xrows = static_cast<int>(min(static_cast<int64_t>(BM), p.m - m0));
+    const int wrows = static_cast<int>(min(static_cast<int64_t>(BN), p.n - n0));
+    ld.rx = buffer_rsrc(p.x + m0 * p.ldx, static_cast<uint32_t>((xrows - 1) * ldx + ksteps * kGroup));
+    ld.rw = buffer_rsrc(p.w + n0 * p.ldw, static_cast<uint32_t>((wrows - 1) * ldw + ksteps * kGroup));
+    if (wave < 4) {
+      ld.sb = p.xs + m0 * p.xs_row;
+      ld.sblk = p.xs_blk;
+      ld.sbytes = (static_cast<uint32_t>(xrows - 1) * static_cast<uint32_t>(p.xs_row) + 1) * 4;
+    } else {
+      const int64_t b = min(n0 / kGroup + (wave >> 1) - 2, (p.n - 1) / kGroup);
+      ld.sb = p.ws + b * p.ws_row;
+      ld.sblk = p.ws_blk;
+      ld.sbytes = 4;
+    }
+    ld.t = 0;
+    ld.tile = tile;
+  };
+  // (rows past the last read zeros: their results are not stored)
+  const uint32_t vs = wave < 4 ? static_cast<uint32_t>(wave * 64 + lane) * static_cast<uint32_t>(p.xs_row) * 4 : 0;
+  // Load line l (W's first; L: the scales) of the stream's block into stage st & 1.
+  auto dma = [&](int st, int l) __attribute__((always_inline)) {
     const uint32_t sb = lds_base + (st & 1) * STAGE;
+    if (l == C::L) {
+      dma4(buffer_rsrc(ld.sb + ld.t * ld.sblk, ld.sbytes),
+           __builtin_amdgcn_readfirstlane(sb + C::W_BYTES + C::X_BYTES + wave * 256), vs);
+      return;
+    }
     const bool is_w = l < C::LW;
     const int h = is_w ? l : l - C::LW, line = wave * (is_w ? C::LW : C::LX) + h;
-    dma16(is_w ? rw : rx,
+    uint32_t v = is_w ? vw[h & 1] : vx[h & 1];
+    asm volatile("" : "+v"(v));  // the sum below is not worth a register across the loop
+    dma16(is_w ? ld.rw : ld.rx,
           __builtin_amdgcn_readfirstlane(sb + (is_w ? 0 : C::W_BYTES) + line * 1024),
-          (is_w ? vw[h & 1] : vx[h & 1]) + (h >> 1) * 16 * (is_w ? ldw : ldx),
-          __builtin_amdgcn_readfirstlane(t * kGroup));
+          v + (h >> 1) * 16 * (is_w ? ldw : ldx), __builtin_amdgcn_readfirstlane(ld.t * kGroup));
   };
+  // On to the next block; past the last tile the last block is loaded again
+  // (nobody uses it), so the loop has no branches around loads.
+  auto next_block = [&]() __attribute__((always_inline)) {
+    if (ld.t + 1 < ksteps)
+      ++ld.t;
+    else if (ld.tile + static_cast<int>(gridDim.x) < ntiles)
+      open(ld.tile + gridDim.x);
+  };
+
   const int sw = (g4 ^ ((r16 >> 1) & 7)) << 4;
   const int woff = (wn * C::WTN + r16) * kGroup, xoff = C::W_BYTES + (wm * 64 + r16) * kGroup;
   auto read = [&](int st, int off, int tile) __attribute__((always_inline)) {
     const char* q = lds + (st & 1) * STAGE + off + tile * 16 * kGroup;
     return frag(*reinterpret_cast<const u32x4*>(q + sw), *reinterpret_cast<const u32x4*>(q + (sw ^ 64)));
   };
-  // Scales: this lane's row of each X tile, and the wave's block of W.
-  const float* xsb = p.xs + m0 * p.xs_row;
-  uint32_t xso[TM];
-#pragma unroll
-  for (int j = 0; j < TM; ++j)
-    xso[j] = static_cast<uint32_t>(min(wm * 64 + 16 * j + r16, xrows - 1)) * static_cast<uint32_t>(p.xs_row);
-  const int64_t wblk = min((n0 + wn * C::WTN) / kGroup, (p.n - 1) / kGroup);
-  const float* wsb = p.ws + wblk * p.ws_row;
-  int zero;  // keeps the load of W's scale off the scalar unit, whose waits would cover LDS reads
-  asm volatile("v_mov_b32 %0, 0" : "=v"(zero));
-  float xr[TM], wr, sc[TM];
-  auto load_scales = [&](int t) __attribute__((always_inline)) {
-    t = min(t, ksteps - 1);
-#pragma unroll
-    for (int j = 0; j < TM; ++j) xr[j] = (xsb + t * p.xs_blk)[xso[j]];
-    wr = (wsb + t * p.ws_blk)[zero];
-  };
 
   f32x4 acc[TN][TM], P[LAG];
+  float sc[NC][TM], xr[TM], wr[NC];
+  int wb[NC];  // where the scale of each class of tiles lies
+  auto read_scales = [&](int st) __attribute__((always_inline)) {
+    const char* q = lds + (st & 1) * STAGE + C::W_BYTES + C::X_BYTES;
 #pragma unroll
-  for (int i = 0; i < TN; ++i)
+    for (int j = 0; j < TM; ++j) xr[j] = *reinterpret_cast<const float*>(q + (wm * 64 + 16 * j + r16) * 4);
 #pragma unroll
-    for (int j = 0; j < TM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < NC; ++c) wr[c] = *reinterpret_cast<const float*>(q + wb[c]);
+  };
+  auto set_scales = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int j = 0; j < TM; ++j) sc[c][j] = xr[j] * wr[c];
+  };
   auto scale_add = [&](int x) __attribute__((always_inline)) {
     f32x4& a = acc[x / TM][x % TM];
     const f32x4 v = P[x % LAG];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) a[e] = fmaf(v[e], sc[x % TM], a[e]);
+    for (int e = 0; e < 4; ++e) a[e] = fmaf(v[e], sc[x / TM / C::CT][x % TM], a[e]);
+  };
+  // Scales of W's rows of this wave's tiles in the tile that begins at row n0.
+  auto place = [&](int64_t n0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int first = static_cast<int>(n0 % kGroup) + wn * C::WTN + c * C::CT * 16;
+      wb[c] = (first < kGroup ? 4 : 6) * 256;
+    }
   };
 
-  load_scales(0);
+  int tile = blockIdx.x;
+  open(tile);
 #pragma unroll
-  for (int l = 0; l < C::L; ++l) dma(0, 0, l);
-  if (ksteps > 1) {
+  for (int l = 0; l <= C::L; ++l) dma(0, l);
+  next_block();
 #pragma unroll
-    for (int l = 0; l < C::L; ++l) dma(1, 1, l);
-    wait_vmcnt<C::L>();
-  } else {
-    wait_vmcnt<0>();
-  }
-#pragma unroll
-  for (int j = 0; j < TM; ++j) sc[j] = xr[j] * wr;
-  load_scales(1);
+  for (int l = 0; l <= C::L; ++l) dma(1, l);
+  wait_vmcnt<C::L + 1>();
   __syncthreads();
   i32x8 wf[4], xf[TM];
 #pragma unroll
   for (int i = 0; i < 4; ++i) wf[i] = read(0, woff, i);
 #pragma unroll
   for (int j = 0; j < TM; ++j) xf[j] = read(0, xoff, j);
-
-  for (int ks = 0; ks < ksteps; ++ks) {
-    const int tnext = min(ks + 2, ksteps - 1);
+  int st = 0, stored = 0;
+  for (;;) {
+    int tm, tn;
+    tile_of(tile, p.tiles_m, p.tiles_n, tm, tn);
+    const int64_t m0 = static_cast<int64_t>(tm) * BM, n0 = static_cast<int64_t>(tn) * BN;
+    place(n0);
+    read_scales(st);
+    set_scales();
 #pragma unroll
-    for (int x = 0; x < NMF; ++x) {
-      const int i = x / TM, j = x % TM;
-      if (x == C::XB) {
-        wait_vmcnt<0>();
-        wait_lgkmcnt0();
+    for (int i = 0; i < TN; ++i)
 #pragma unroll
-        for (int q = 0; q < TM; ++q) {
-          xr[q] *= wr;
-          asm volatile("" : "+v"(xr[q]));
+      for (int j = 0; j < TM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int ks = 0; ks < ksteps; ++ks, ++st) {
+      next_block();
+#pragma unroll
+      for (int x = 0; x < NMF; ++x) {
+        const int i = x / TM, j = x % TM;
+        if (x == C::XB) {
+          // this wave's loads of the next block have landed (behind them a
+          // tile's first step may still have its predecessor's stores under way)
+          asm volatile(
+              "s_cmp_lg_u32 %0, 0\n\ts_cbranch_scc1 .Lstored%=\n\ts_waitcnt vmcnt(0)\n.Lstored%=:\n\t"
+              "s_waitcnt vmcnt(%1) lgkmcnt(0)"
+              :
+              : "s"(__builtin_amdgcn_readfirstlane(stored)), "n"(TN / 2 * TM)
+              : "memory", "scc");
+          __syncthreads();
         }
-        __syncthreads();
-      }
-      if (x >= LAG) scale_add(x - LAG);
-      P[x % LAG] = mfma_block(wf[i & 3], xf[j]);
-      // W's tile i + 4 of this block, else the next block's tile of the slot
-      if (j == TM - 1)
-        wf[i & 3] = i + 4 < TN ? read(ks, woff, i + 4) : read(ks + 1, woff, i & 3);
-      if (i == TN - 1) xf[j] = read(ks + 1, xoff, j);
-      if (x >= C::XB && x - C::XB < C::L) dma(tnext, ks, x - C::XB);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-#pragma unroll
-    for (int x = NMF - LAG; x < NMF; ++x) scale_add(x);
-#pragma unroll
-    for (int q = 0; q < TM; ++q) sc[q] = xr[q];
-    load_scales(ks + 2);
-  }
-
-  // A partial last block: straight from memory.
-  if (k % kGroup != 0) {
-    i32x8 xt[TM];
-#pragma unroll
-    for (int j = 0; j < TM; ++j) {
-      const int64_t row = m0 + min(wm * 64 + 16 * j + r16, xrows - 1);
-      xt[j] = load_frag(p.x + row * p.ldx, ksteps, k, g4);
-      sc[j] = (xsb + ksteps * p.xs_blk)[xso[j]] * (wsb + ksteps * p.ws_blk)[0];
-    }
-#pragma unroll
-    for (int i = 0; i < TN; ++i) {
-      const int64_t row = n0 + min(wn * C::WTN + 16 * i + r16, wrows - 1);
-      const i32x8 wt = load_frag(p.w + row * p.ldw, ksteps, k, g4);
-#pragma unroll
-      for (int j = 0; j < TM; ++j) {
-        P[0] = mfma_block(wt, xt[j]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(P[0][e], sc[j], acc[i][j][e]);
-      }
-    }
-  }
-
-  // Lane: columns 4 g4 .. + 3 of W tile i, row r16 of X tile j.  16 rows at a
-  // time through the wave's own LDS slab, so that stores cover whole lines.
-  wait_vmcnt<0>();
-  wait_lgkmcnt0();
-  __syncthreads();
-  constexpr int SP = C::SP, CPO = C::WTN / 8;
-  T* slab = reinterpret_cast<T*>(lds) + wave * (16 * SP);
-  const T* bias = static_cast<const T*>(p.bias);
-  T* D = static_cast<T*>(p.d);
-  const int64_t col0 = n0 + wn * C::WTN, row0 = m0 + wm * (TM * 16);
-  if (bias != nullptr) {
-#pragma unroll
-    for (int i = 0; i < TN; ++i) {
-      f32x4 b = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int64_t col = col0 + 16 * i + 4 * g4 + e;
-        if (col < p.n) b[e] = Num<T>::to_f(bias[col]);
+        if (x >= LAG) scale_add(x - LAG);
+        P[x % LAG] = mfma_block(wf[i & 3], xf[j]);
+        // W's tile i + 4 of this block, else the next block's tile of the slot
+        if (j == TM - 1)
+          wf[i & 3] = i + 4 < TN ? read(st, woff, i + 4) : read(st + 1, woff, i & 3);
+        if (i == TN - 1) xf[j] = read(st + 1, xoff, j);
+        if (x == NMF - TM - 1) read_scales(st + 1);
+        if (x >= C::XB && x - C::XB <= C::L) dma(st, x - C::XB);
+        __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
-      for (int j = 0; j < TM; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][e] += b[e];
+      for (int x = NMF - LAG; x < NMF; ++x) scale_add(x);
+      set_scales();
+      stored = 0;
     }
+    // (the lane number anew: addresses of the stores kept over the K loop would
+    // cost registers there)
+    int l = lane;
+    asm volatile("" : "+v"(l));
+    store_tiles<T, TN, TM>(p, acc, m0 + wm * (TM * 16), n0 + wn * C::WTN, l & 15, l >> 4);
+    tile += gridDim.x;
+    if (tile >= ntiles) break;
+    // a whole tile's stores are TN / 2 * TM instructions
+    stored = m0 + BM <= p.m && n0 + BN <= p.n;
   }
-#pragma unroll
-  for (int j = 0; j < TM; ++j) {
-#pragma unroll
-    for (int i = 0; i < TN; ++i) {
-      u32x2 v;
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        v[e] = pack2<T>(acc[i][j][2 * e], acc[i][j][2 * e + 1]);
-      *reinterpret_cast<u32x2*>(slab + r16 * SP + 16 * i + 4 * g4) = v;
-    }
-    wait_lgkmcnt0();
-#pragma unroll
-    for (int q = lane; q < 16 * CPO; q += 64) {
-      const int rr = q / CPO, cc = (q % CPO) * 8;
-      const int64_t row = row0 + 16 * j + rr, col = col0 + cc;
-      if (row >= p.m || col >= p.n) continue;
-      const u32x4 v = *reinterpret_cast<const u32x4*>(slab + rr * SP + cc);
-      T* dp = D + row * p.ldd + col;
-      if (col + 8 <= p.n) {
-        __builtin_nontemporal_store(v, reinterpret_cast<u32x4_any*>(dp));
-      } else {
-        const T* e = reinterpret_cast<const T*>(&v);
-#pragma unroll
-        for (int c = 0; c < 8; ++c)
-          if (col + c < p.n) dp[c] = e[c];
-      }
-    }
-    wait_lgkmcnt0();
-  }
+  wait_vmcnt<0>();  // the last loads land before the LDS is given back
 }
 
-// A wave computes 16 columns of W's rows by 64 rows of X, straight from memory.
-template <typename T>
-__global__ void __launch_bounds__(256) gemm_fp8_kernel(const Fp8Args p) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, g4 = lane >> 4;
-  const int64_t n0 = (static_cast<int64_t>(blockIdx.x) * 4 + wave) * 16;
-  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * 64;
-  if (n0 >= p.n) return;
-  const uint8_t* wr = p.w + min(n0 + r16, p.n - 1) * p.ldw;
-  const uint8_t* xr[4];
-  const float* xs[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int64_t row = min(m0 + 16 * j + r16, p.m - 1);
-    xr[j] = p.x + row * p.ldx;
-    xs[j] = p.xs + row * p.xs_row;
-  }
-  const float* ws = p.ws + n0 / kGroup * p.ws_row;
-  const int64_t nb = (p.k + kGroup - 1) / kGroup;
-  f32x4 acc[4] = {};
-  for (int64_t b = 0; b < nb; ++b) {
-    const i32x8 wf = load_frag(wr, b, p.k, g4);
-    const float wscale = ws[b * p.ws_blk];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const f32x4 s = mfma_block(wf, load_frag(xr[j], b, p.k, g4));
-      const float sc = xs[j][b * p.xs_blk] * wscale;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[j][e] = fmaf(s[e], sc, acc[j][e]);
-    }
-  }
-  const T* bias = static_cast<const T*>(p.bias);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int64_t row = m0 + 16 * j + r16;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int64_t col = n0 + 4 * g4 + e;
-      if (row < p.m && col < p.n)
-        static_cast<T*>(p.d)[row * p.ldd + col] =
-            Num<T>::from_f(acc[j][e] + (bias ? Num<T>::to_f(bias[col]) : 0.f));
-    }
-  }
-}
-
-template <typename T, int TN, int WN, int WM>
+template <typename T, int TN>
 int launch_dl(Fp8Args p, hipStream_t stream) {
-  using C = dl8::Cfg<TN, WN, WM>;
-  p.tiles_m = static_cast<int>(ceil_div(p.m, C::BM));
+  using C = dl8::Cfg<TN>;
+  p.tiles_m = static_cast<int>(ceil_div(p.m, dl8::BM));
   p.tiles_n = static_cast<int>(ceil_div(p.n, C::BN));
-  gemm_fp8_dl_kernel<T, TN, WN, WM><<<p.tiles_m * p.tiles_n, C::NT, 0, stream>>>(p);
+  const int grid = std::min(p.tiles_m * p.tiles_n, 256);
+  gemm_fp8_dl_kernel<T, TN><<<grid, dl8::NT, 0, stream>>>(p);
   return check_launch("sph_gemm_fp8");
 }
 
-template <typename T>
-int launch(const Fp8Args& p, hipStream_t stream) {
-  if (p.k >= kGroup && p.m > 128) return launch_dl<T, 8, 2, 4>(p, stream);
-  const dim3 grid(static_cast<uint32_t>(ceil_div(p.n, 64)), static_cast<uint32_t>(ceil_div(p.m, 64)));
-  gemm_fp8_kernel<T><<<grid, 256, 0, stream>>>(p);
-  return check_launch("sph_gemm_fp8");
+// The kernel of a product (one MI355X, operands of three products in turn, us).
+//   Streamed rows, where one pass of workgroups over 16 rows each of X and W and
+// 4 blocks a wave is the whole product: 512 workgroups and K of 4096 at most,
+// above 16 rows (W read more than once, from the caches) half of their product.
+//     1 x 6144 x 4096 8.0 (ring 8.8), 16 x 4096 x 4096 6.6 (8.2), 16 x 8192 x 4096
+//     10.3 (10.3), 16 x 12288 x 4096 14.8 (12.1), 1 x 4096 x 12800 12.8 (12.4),
+//     64 x 2048 x 2048 5.8 (6.9), 512 x 256 x 4096 10.2 (8.2)
+//   Others the kernel whose fitted time is the least:
+//     16 x 25600 x 4096 ring 21.7 (streamed 30), 333 x 4096 x 12800 ring 37.5 (256-
+//     row tiles 117), 2048 x 6144 x 4096 192-row tiles 47.3 (256-row 50.5, ring
+//     73.8), 2048 x 25600 x 4096 256-row tiles 239 (ring 285)
+Fp8Plan fp8_plan(int64_t m, int64_t n, int64_t k, int64_t max_bytes) {
+  Fp8Plan best;
+  const int64_t wgs = ceil_div(n, 16) * ceil_div(m, 16);
+  if (k < kGroup || (wgs <= 512 && k <= 32 * kGroup && wgs * k <= (m <= 16 ? 1 << 21 : 1 << 20)))
+    return best;
+  const double nb = static_cast<double>(k / kGroup);
+  best = fp8_ring_plan(m, n, k, max_bytes);
+  if (k >= 2 * kGroup && k % kGroup == 0) {
+    constexpr double kLaunch = 1.0, kRound[2] = {5.7, 4.5}, kBlock[2] = {1.29, 1.10};
+    for (int c = 0; c < 2; ++c) {
+      const int64_t tiles = ceil_div(m, dl8::BM) * ceil_div(n, c == 0 ? 256 : 192);
+      const double us = kLaunch + static_cast<double>(ceil_div(tiles, 256)) * (kRound[c] + nb * kBlock[c]);
+      if (us < best.us) best = Fp8Plan{Fp8Plan::kTiles, c, 1, 0, 0, us};
+    }
+  }
+  return best;
+}
+
+int launch(bool bf16, Fp8Args p, const Fp8Plan& plan, hipStream_t st) {
+  if (plan.kernel == Fp8Plan::kStream) return launch_fp8_stream(bf16, p, st);
+  if (plan.kernel == Fp8Plan::kRing) return launch_fp8_ring(bf16, p, plan, st);
+  if (plan.cfg == 1) return bf16 ? launch_dl<bf16_t, 6>(p, st) : launch_dl<half_t, 6>(p, st);
+  return bf16 ? launch_dl<bf16_t, 8>(p, st) : launch_dl<half_t, 8>(p, st);
 }
 
 }  // namespace
@@ -382,8 +297,23 @@ int launch(const Fp8Args& p, hipStream_t stream) {
 using namespace sph;
 
 extern "C" int64_t sph_gemm_fp8_workspace_bytes(int64_t m, int64_t n, int64_t k) {
-  (void)m, (void)n, (void)k;
-  return 0;
+  if (m <= 0 || n <= 0 || k <= 0) return 0;
+  return fp8_plan(m, n, k, INT64_MAX).bytes;
+}
+
+extern "C" int sph_gemm_fp8_plan(int64_t m, int64_t n, int64_t k, int64_t workspace_bytes,
+                                 int32_t* plan) {
+  SPH_REQUIRE(m > 0 && n > 0 && k > 0 && plan != nullptr, SPH_ERR_INVALID_ARG,
+              "sph_gemm_fp8_plan: sizes must be positive");
+  const Fp8Plan p = fp8_plan(m, n, k, workspace_bytes);
+  const Fp8Tile t = p.kernel == Fp8Plan::kStream  ? Fp8Tile{16, 16}
+                    : p.kernel == Fp8Plan::kRing ? fp8_ring_tile(p.cfg)
+                                                 : Fp8Tile{dl8::BM, p.cfg == 0 ? 256 : 192};
+  plan[0] = p.kernel;
+  plan[1] = t.m;
+  plan[2] = t.n;
+  plan[3] = p.splits;
+  return SPH_OK;
 }
 
 extern "C" int sph_gemm_fp8(sph_dtype dtype, int64_t m, int64_t n, int64_t k, const void* x,
@@ -392,7 +322,6 @@ extern "C" int sph_gemm_fp8(sph_dtype dtype, int64_t m, int64_t n, int64_t k, co
                             const float* w_scale, int64_t w_scale_row_stride,
                             int64_t w_scale_group_stride, const void* bias, void* d, int64_t ldd,
                             void* workspace, int64_t workspace_bytes, sph_stream_t stream) {
-  (void)workspace, (void)workspace_bytes;
   SPH_REQUIRE(m >= 0 && n >= 0 && k >= 0, SPH_ERR_INVALID_ARG, "sph_gemm_fp8: negative size");
   SPH_REQUIRE(dtype == SPH_F16 || dtype == SPH_BF16, SPH_ERR_UNSUPPORTED,
               "sph_gemm_fp8: dtype must be F16 or BF16");
@@ -415,7 +344,10 @@ extern "C" int sph_gemm_fp8(sph_dtype dtype, int64_t m, int64_t n, int64_t k, co
               SPH_ERR_TOO_LARGE, "sph_gemm_fp8: k, ldx or ldw above 4194303");
   SPH_REQUIRE(m <= INT32_MAX && n <= INT32_MAX, SPH_ERR_TOO_LARGE,
               "sph_gemm_fp8: m or n above 2^31 - 1");
-  SPH_REQUIRE(ceil_div(m, 64) <= 65535, SPH_ERR_TOO_LARGE, "sph_gemm_fp8: too many rows");
+  SPH_REQUIRE(m <= 16 * 65535 && m * n <= (int64_t{1} << 40), SPH_ERR_TOO_LARGE,
+              "sph_gemm_fp8: more than 1048560 rows or 2^40 results");
+  SPH_REQUIRE(m == 1 || k == 0 || x_scale_row_stride <= (1 << 21), SPH_ERR_TOO_LARGE,
+              "sph_gemm_fp8: x_scale_row_stride above 2097152");
   Fp8Args p{m,
                   n,
                   k,
@@ -433,7 +365,10 @@ extern "C" int sph_gemm_fp8(sph_dtype dtype, int64_t m, int64_t n, int64_t k, co
                   d,
                   ldd,
                   0,
-                  0};
-  const hipStream_t st = as_stream(stream);
-  return dtype == SPH_F16 ? launch<half_t>(p, st) : launch<bf16_t>(p, st);
+                  0,
+                  1,
+                  0,
+                  static_cast<float*>(workspace)};
+  const Fp8Plan plan = fp8_plan(m, n, k, workspace != nullptr ? workspace_bytes : 0);
+  return launch(dtype == SPH_BF16, p, plan, as_stream(stream));
 }

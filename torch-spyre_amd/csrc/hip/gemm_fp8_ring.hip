@@ -1,0 +1,285 @@
+// 8-bit products whose rows do not fill the CUs with 256-row tiles: decode
+// batches, short and ragged prompts.
+//
+//   * Tiles of BM of X's rows by BN of W's on 4 waves (2 x 2), two or three
+//     workgroups per CU; ST - 1 blocks of K in flight through a ring of ST LDS
+//     stages (direct loads, 128 codes a row, chunk c of row r at slot c ^
+//     ((r >> 1) & 7)).
+//   * The block's scales ride in the same stage by one 4-byte load per lane: the
+//     first waves fetch X's, the others W's (one value), so they are covered by
+//     the same wait and barrier and need no registers in flight.
+//   * K is split over workgroups until the chip is full: fp32 sums in a caller's
+//     workspace, added in a fixed order by a second kernel.
+#include <algorithm>
+
+#include "gemm_fp8.h"
+
+namespace sph {
+namespace {
+
+namespace ring8 {
+constexpr uint32_t kOutside = 0x80000000u;  // past every buffer resource
+
+template <int BM_, int BN_, int ST_>
+struct Cfg {
+  static constexpr int BM = BM_, BN = BN_, ST = ST_, NW = 4, WTM = BM / 2, WTN = BN / 2;
+  static constexpr int TM = WTM / 16, TN = WTN / 16;
+  static constexpr int X_BYTES = BM * kGroup, W_BYTES = BN * kGroup, S_BYTES = NW * 256;
+  static constexpr int STAGE = X_BYTES + W_BYTES + S_BYTES;
+  static constexpr int LX = X_BYTES / 1024 / NW, LW = W_BYTES / 1024 / NW, L = LX + LW + 1;
+  static constexpr int XSW = (BM + 63) / 64;  // waves that fetch X's scales
+  static_assert(LX * NW * 1024 == X_BYTES && LW * NW * 1024 == W_BYTES, "load lines");
+  static_assert(XSW < NW && BN <= kGroup && TN % 2 == 0, "scales, one block of W, tile pairs");
+  static_assert((ST - 2) * L < 64, "vmcnt range");
+};
+}  // namespace ring8
+
+template <int ST, int L>
+__device__ inline void wait_blocks(int blocks) {
+  static_assert(ST <= 4, "at most two blocks in flight behind the one awaited");
+  if constexpr (ST >= 4) {
+    if (blocks >= 2) return wait_vmcnt<2 * L>();
+  }
+  if constexpr (ST >= 3) {
+    if (blocks >= 1) return wait_vmcnt<L>();
+  }
+  wait_vmcnt<0>();
+}
+
+template <typename T, int BM_, int BN_, int ST_>
+__global__ void __launch_bounds__(256) gemm_fp8_ring_kernel(const Fp8Args p) {
+  using C = ring8::Cfg<BM_, BN_, ST_>;
+  constexpr int BM = C::BM, BN = C::BN, ST = C::ST, TM = C::TM, TN = C::TN;
+  __shared__ __attribute__((aligned(1024))) char lds[ST * C::STAGE];
+  // Workgroup -> (tile, K slice): a contiguous run per XCD, row tiles of one
+  // panel of W next to each other.
+  int id = blockIdx.x;
+  {
+    const int total = gridDim.x, q = total >> 3, r = total & 7, x = id & 7;
+    id = x * q + min(x, r) + (id >> 3);
+  }
+  const int tm = id % p.tiles_m;
+  id /= p.tiles_m;
+  const int split = id % p.splits, tn = id / p.splits;
+  const int64_t m0 = static_cast<int64_t>(tm) * BM, n0 = static_cast<int64_t>(tn) * BN;
+  const int k = static_cast<int>(p.k), nbf = k / kGroup;
+  const int kb0 = split * p.kslice, ksteps = min(p.kslice, nbf - kb0);
+  const int ldx = static_cast<int>(p.ldx), ldw = static_cast<int>(p.ldw);
+  const int xrows = static_cast<int>(min(static_cast<int64_t>(BM), p.m - m0));
+  const int wrows = static_cast<int>(min(static_cast<int64_t>(BN), p.n - n0));
+  const int lane = threadIdx.x & 63, r16 = lane & 15, g4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int wm = wave >> 1, wn = wave & 1;
+  const i32x4 rx = buffer_rsrc(p.x + m0 * p.ldx, static_cast<uint32_t>((xrows - 1) * ldx + nbf * kGroup));
+  const i32x4 rw = buffer_rsrc(p.w + n0 * p.ldw, static_cast<uint32_t>((wrows - 1) * ldw + nbf * kGroup));
+  uint32_t vx[C::LX], vw[C::LW];
+#pragma unroll
+  for (int i = 0; i < C::LX; ++i) {
+    const int r = (wave * C::LX + i) * 8 + (lane >> 3);
+    vx[i] = r < xrows ? static_cast<uint32_t>(r * ldx + (((lane & 7) ^ ((r >> 1) & 7)) << 4)) : ring8::kOutside;
+  }
+#pragma unroll
+  for (int i = 0; i < C::LW; ++i) {
+    const int r = (wave * C::LW + i) * 8 + (lane >> 3);
+    vw[i] = r < wrows ? static_cast<uint32_t>(r * ldw + (((lane & 7) ^ ((r >> 1) & 7)) << 4)) : ring8::kOutside;
+  }
+  // Scales: this wave's source, step per block, and lane offset.
+  const bool sx = wave < C::XSW;
+  const float* sbase = sx ? p.xs + m0 * p.xs_row : p.ws + n0 / kGroup * p.ws_row;
+  const int64_t sblk = sx ? p.xs_blk : p.ws_blk;
+  const uint32_t sbytes = sx ? (static_cast<uint32_t>(xrows - 1) * static_cast<uint32_t>(p.xs_row) + 1) * 4 : 4;
+  const uint32_t vs = sx ? static_cast<uint32_t>(min(wave * 64 + lane, xrows - 1)) * static_cast<uint32_t>(p.xs_row) * 4 : 0;
+  const uint32_t lds_base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((SPH_LDS char*)(lds)));
+
+  auto issue = [&](int t, int slot) __attribute__((always_inline)) {
+    const uint32_t sb = lds_base + slot * C::STAGE;
+    const int kb = kb0 + t;
+#pragma unroll
+    for (int i = 0; i < C::LX; ++i)
+      dma16(rx, __builtin_amdgcn_readfirstlane(sb + (wave * C::LX + i) * 1024), vx[i],
+            __builtin_amdgcn_readfirstlane(kb * kGroup));
+#pragma unroll
+    for (int i = 0; i < C::LW; ++i)
+      dma16(rw, __builtin_amdgcn_readfirstlane(sb + C::X_BYTES + (wave * C::LW + i) * 1024), vw[i],
+            __builtin_amdgcn_readfirstlane(kb * kGroup));
+    dma4(buffer_rsrc(sbase + kb * sblk, sbytes),
+         __builtin_amdgcn_readfirstlane(sb + C::X_BYTES + C::W_BYTES + wave * 256), vs);
+  };
+
+  const int sw = (g4 ^ ((r16 >> 1) & 7)) << 4;
+  const int xoff = (wm * C::WTM + r16) * kGroup, woff = C::X_BYTES + (wn * C::WTN + r16) * kGroup;
+  const int soff = C::X_BYTES + C::W_BYTES;
+  f32x4 acc[TN][TM];
+#pragma unroll
+  for (int i = 0; i < TN; ++i)
+#pragma unroll
+    for (int j = 0; j < TM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  for (int t = 0; t < ST - 1 && t < ksteps; ++t) issue(t, t);
+  int slot = 0;
+  for (int ks = 0; ks < ksteps; ++ks) {
+    // block ks has landed once only later blocks' loads are outstanding; the
+    // barrier also means that every wave is done with the slot of block ks - 1
+    wait_blocks<ST, C::L>(min(ST - 2, ksteps - 1 - ks));
+    wait_lgkmcnt0();
+    __syncthreads();
+    if (ks + ST - 1 < ksteps) issue(ks + ST - 1, slot == 0 ? ST - 1 : slot - 1);
+    const char* sp = lds + slot * C::STAGE;
+    const float wsc = *reinterpret_cast<const float*>(sp + soff + (C::NW - 1) * 256);
+    float sc[TM];
+    i32x8 xf[TM], wf[TN];
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+      sc[j] = *reinterpret_cast<const float*>(sp + soff + (wm * C::WTM + 16 * j + r16) * 4) * wsc;
+      const char* q = sp + xoff + j * 16 * kGroup;
+      xf[j] = frag(*reinterpret_cast<const u32x4*>(q + sw), *reinterpret_cast<const u32x4*>(q + (sw ^ 64)));
+    }
+#pragma unroll
+    for (int i = 0; i < TN; ++i) {
+      const char* q = sp + woff + i * 16 * kGroup;
+      wf[i] = frag(*reinterpret_cast<const u32x4*>(q + sw), *reinterpret_cast<const u32x4*>(q + (sw ^ 64)));
+    }
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+      for (int j = 0; j < TM; ++j) {
+        const f32x4 s = mfma_block(wf[i], xf[j]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(s[e], sc[j], acc[i][j][e]);
+      }
+    slot = slot + 1 == ST ? 0 : slot + 1;
+  }
+
+  const int64_t row0 = m0 + wm * C::WTM, col0 = n0 + wn * C::WTN;
+  if (k % kGroup != 0 && split == p.splits - 1) {  // the partial last block
+    const int64_t xbase = m0 + xrows - 1, wbase = n0 + wrows - 1;
+    i32x8 xf[TM];
+    float sc[TM];
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+      const int64_t row = min(row0 + 16 * j + r16, xbase);
+      xf[j] = load_frag(p.x + row * p.ldx, nbf, k, g4);
+      sc[j] = p.xs[row * p.xs_row + nbf * p.xs_blk] * p.ws[n0 / kGroup * p.ws_row + nbf * p.ws_blk];
+    }
+#pragma unroll
+    for (int i = 0; i < TN; ++i) {
+      const i32x8 wf = load_frag(p.w + min(col0 + 16 * i + r16, wbase) * p.ldw, nbf, k, g4);
+#pragma unroll
+      for (int j = 0; j < TM; ++j) {
+        const f32x4 s = mfma_block(wf, xf[j]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(s[e], sc[j], acc[i][j][e]);
+      }
+    }
+  }
+  if (p.splits == 1) return store_tiles<T, TN, TM>(p, acc, row0, col0, r16, g4);
+  const int64_t pitch = (p.n + 3) & ~static_cast<int64_t>(3);
+  float* W = p.part + static_cast<int64_t>(split) * p.m * pitch;
+#pragma unroll
+  for (int i = 0; i < TN; ++i) {
+    const int64_t col = col0 + 16 * i + 4 * g4;
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+      const int64_t row = row0 + 16 * j + r16;
+      if (row < p.m && col < pitch) *reinterpret_cast<f32x4*>(W + row * pitch + col) = acc[i][j];
+    }
+  }
+}
+
+// Adds the K slices' sums in slice order, then bias: 4 columns a thread.
+template <typename T>
+__global__ void __launch_bounds__(256) gemm_fp8_reduce(const Fp8Args p) {
+  const int64_t nq = (p.n + 3) >> 2, idx = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (idx >= p.m * nq) return;
+  const int64_t row = idx / nq, col = (idx - row * nq) * 4, step = p.m * nq * 4;
+  const float* W = p.part + row * nq * 4 + col;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = 0; s < p.splits; ++s) v += *reinterpret_cast<const f32x4*>(W + s * step);
+  store_row4<T>(p, row, col, v);
+}
+
+template <typename T, int BM, int BN, int ST>
+int launch_ring8(Fp8Args& p, hipStream_t st) {
+  p.tiles_m = static_cast<int>(ceil_div(p.m, BM));
+  p.tiles_n = static_cast<int>(ceil_div(p.n, BN));
+  const unsigned grid = static_cast<unsigned>(p.tiles_m) * p.tiles_n * p.splits;
+  gemm_fp8_ring_kernel<T, BM, BN, ST><<<grid, 256, 0, st>>>(p);
+  if (p.splits > 1)
+    gemm_fp8_reduce<T><<<static_cast<unsigned>(ceil_div(p.m * ceil_div(p.n, 4), 256)), 256, 0, st>>>(p);
+  return check_launch("sph_gemm_fp8");
+}
+
+// Tile configurations: per_cu workgroups share a CU (LDS); us of a round of
+// workgroups beside its blocks of K, of the launch, and per block of K with
+// 1, 2 or 3 workgroups on the CU; us of the reduce's launch and TB/s of its
+// sums.  Fitted to 5200 timings of 1 to 2600 rows by 512 to 49155 columns, K
+// 1024 to 12800, 1 to 16 slices (rms error 6 %; the plan that the fitted times
+// choose is 2 % slower than the fastest of a product on average, 16 % at most:
+// 256 x 25600 x 4096).
+struct RingCfg {
+  int bm, bn, per_cu;
+  double round, launch, blk[3], reduce, sums;
+};
+constexpr RingCfg kRing[] = {{32, 64, 3, 0.2, 2.3, {0.297, 0.369, 0.492}, 2.5, 4.7},
+                             {32, 128, 2, 0.2, 2.4, {0.442, 0.552, 0}, 2.6, 5.3},
+                             {64, 128, 2, 0.1, 2.9, {0.631, 0.772, 0}, 2.5, 5.4},
+                             {128, 128, 2, 1.6, 2.1, {0.993, 1.186, 0}, 2.6, 5.9}};
+constexpr int kRingCfgs = sizeof(kRing) / sizeof(kRing[0]);
+
+template <typename T>
+int launch_cfg(Fp8Args& p, int cfg, hipStream_t st) {
+  switch (cfg) {
+    case 0: return launch_ring8<T, 32, 64, 4>(p, st);
+    case 1: return launch_ring8<T, 32, 128, 3>(p, st);
+    case 2: return launch_ring8<T, 64, 128, 3>(p, st);
+    default: return launch_ring8<T, 128, 128, 2>(p, st);
+  }
+}
+
+}  // namespace
+
+Fp8Plan fp8_ring_plan(int64_t m, int64_t n, int64_t k, int64_t max_bytes) {
+  Fp8Plan best;
+  best.us = 1e30;
+  constexpr int64_t kCUs = 256;
+  const int64_t nbf = k / kGroup, pitch = (n + 3) / 4 * 4;
+  const double mem_us = static_cast<double>(m * k + n * k + 2 * m * n) / 5.6e6;
+  for (int c = 0; c < kRingCfgs; ++c) {
+    const RingCfg& f = kRing[c];
+    const int64_t tiles = ceil_div(m, f.bm) * ceil_div(n, f.bn), slots = kCUs * f.per_cu;
+    for (int s = 1; s <= 16; ++s) {
+      // at least 2 blocks a slice, no more slices than two rounds hold
+      if (s > 1 && (tiles * s > 2 * slots || nbf < 2 * s)) break;
+      const int64_t slice = ceil_div(nbf, s);
+      if (ceil_div(nbf, slice) != s) continue;  // every slice has blocks
+      const int64_t bytes = s > 1 ? s * m * pitch * 4 : 0;
+      if (bytes > max_bytes) continue;
+      const int64_t full = tiles * s / slots, rest = tiles * s % slots;
+      const double blocks = static_cast<double>(slice);
+      double us = static_cast<double>(full) * (f.round + blocks * f.blk[f.per_cu - 1]);
+      if (rest > 0) us += 0.7 * f.round + blocks * f.blk[(rest - 1) / kCUs];
+      us = f.launch + std::max(us, mem_us);
+      if (s > 1) us += f.reduce + 2.0 * static_cast<double>(bytes) / (f.sums * 1e6);
+      if (us < best.us) {
+        best.kernel = Fp8Plan::kRing;
+        best.cfg = c;
+        best.splits = s;
+        best.kslice = static_cast<int>(slice);
+        best.bytes = bytes;
+        best.us = us;
+      }
+    }
+  }
+  return best;
+}
+
+Fp8Tile fp8_ring_tile(int cfg) { return {kRing[cfg].bm, kRing[cfg].bn}; }
+
+int launch_fp8_ring(bool bf16, Fp8Args p, const Fp8Plan& plan, hipStream_t st) {
+  p.splits = plan.splits;
+  p.kslice = plan.kslice;
+  return bf16 ? launch_cfg<bf16_t>(p, plan.cfg, st) : launch_cfg<half_t>(p, plan.cfg, st);
+}
+
+}  // namespace sph

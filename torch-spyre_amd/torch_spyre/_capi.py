@@ -80,6 +80,7 @@ _SIGS = {
     "sph_gemm_fp8": ([c_int, c_i64, c_i64, c_i64, vp, c_i64, vp, c_i64, c_i64, vp, c_i64, vp, c_i64,
                       c_i64, vp, vp, c_i64, vp, c_i64, vp], c_int),
     "sph_gemm_fp8_workspace_bytes": ([c_i64, c_i64, c_i64], c_i64),
+    "sph_gemm_fp8_plan": ([c_i64, c_i64, c_i64, c_i64, vp], c_int),
     "sph_attention_fwd": ([c_int, c_i64, c_i64, c_i64, c_i64, vp, c_i64, c_i64, vp, c_i64,
                            c_i64, vp, c_i64, c_i64, vp, c_i64, c_i64, c_i64, c_i64, c_f32, vp,
                            c_i64, c_i64, vp, c_i64, vp], c_int),

@@ -78,10 +78,12 @@ at::Tensor empty_codes(at::IntArrayRef sizes, c10::Device device) {
 
 // One scale per row and group, a group's scales of all rows side by side.
 at::Tensor empty_scales(at::IntArrayRef sizes, int64_t rows, c10::Device device) {
-  const int64_t ng = groups(sizes.back());
-  std::vector<int64_t> shape(sizes.begin(), sizes.end());
-  shape.back() = ng;
-  return empty_spyre({ng, rows}, at::kFloat, device).t().view(shape);
+  c10::SmallVector<int64_t, 5> shape(sizes.begin(), sizes.end()), strides(sizes.size());
+  shape.back() = groups(sizes.back());
+  strides.back() = rows;
+  int64_t s = 1;
+  for (size_t d = sizes.size() - 1; d-- > 0; s *= sizes[d]) strides[d] = s;
+  return at::empty_strided(shape, strides, at::TensorOptions().dtype(at::kFloat).device(device));
 }
 
 int64_t row_stride(const at::Tensor& q) { return (q.size(-1) + 15) / 16 * 16; }

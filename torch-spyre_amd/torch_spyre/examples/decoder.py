@@ -17,6 +17,14 @@ operand along its contiguous dimension (scores: K rows; output: V^T rows),
 which is the small-M streaming GEMM's layout.  The buffers are separate
 tensors, so a compiled decode step scatters the new token's K/V into them
 in place instead of copying an aliased cache.
+
+With the weights of quantize_params the projections run in 8 bits: every
+norm, the attention output and the SwiGLU activation leave as e4m3 codes with
+a scale for each 128 columns (torch.ops.spyre.{rms_norm_fp8,
+add_rms_norm_fp8, quantize_fp8, silu_mul_fp8}) and meet the weights' codes in
+torch.ops.spyre.mm_fp8; the residual stream, RoPE, attention and the cache stay
+in the model's type.  prefill, decode_step, decode_step_static and generate
+take such weights as they are.
 """
 
 from __future__ import annotations
@@ -106,6 +114,24 @@ def init_params(cfg: DecoderConfig, device, dtype=torch.float16, seed: int = 0xA
     return params
 
 
+def quantize_params(params: dict) -> dict:
+    """`params` with every projection (Q/K/V, O, gate / up, down, LM head) as
+    e4m3 codes and scales of 128 x 128 blocks, half the bytes of the 16-bit
+    weights; embedding and norm weights as they are."""
+    def q(w):
+        return torch.ops.spyre.quantize_fp8(w.detach(), 128)
+
+    def fused(w, whole, parts):
+        return w[whole] if whole in w else torch.cat([w[p] for p in parts])
+
+    layers = [{"attn_norm": w["attn_norm"], "mlp_norm": w["mlp_norm"],
+               "wqkv_fp8": q(fused(w, "wqkv", ("wq", "wk", "wv"))), "wo_fp8": q(w["wo"]),
+               "wgu_fp8": q(fused(w, "wgu", ("wg", "wu"))), "wd_fp8": q(w["wd"])}
+              for w in params["layers"]]
+    return {"embed": params["embed"], "layers": layers, "final_norm": params["final_norm"],
+            "lm_head_fp8": q(params["lm_head"])}
+
+
 def rope_tables(cfg: DecoderConfig, max_pos: int, device, dtype=torch.float16):
     """cos / sin [max_pos, head_dim] (both halves equal), angles in fp32."""
     d = cfg.head_dim
@@ -148,11 +174,37 @@ def _attention(q, k, v, cfg: DecoderConfig, mask):
     return o.view(B, kv, g, Sq, D).permute(0, 3, 1, 2, 4).reshape(B * Sq, kv * g * D)
 
 
+def _first_norm(h, w: dict, cfg: DecoderConfig):
+    """h normalised for a layer's Q/K/V projection: a tensor, or for 8-bit
+    weights its (codes, scales)."""
+    if "wqkv_fp8" in w:
+        return torch.ops.spyre.rms_norm_fp8(h, w["attn_norm"], cfg.eps)
+    return F.rms_norm(h, (cfg.hidden,), w["attn_norm"], cfg.eps)
+
+
+def _rest_of_layer_fp8(a, h, w: dict, cfg: DecoderConfig, next_norm):
+    """Output projection, residual and MLP of an 8-bit layer for its attention
+    output a [rows, n_heads * head_dim] and residual stream h: (new h, its
+    (codes, scales) under next_norm, or None)."""
+    ops, dt = torch.ops.spyre, h.dtype
+    o = ops.mm_fp8(*ops.quantize_fp8(a), *w["wo_fp8"], dt).view(h.shape)
+    xq, xs, h = ops.add_rms_norm_fp8(o, h, w["mlp_norm"], cfg.eps)
+    gu = ops.mm_fp8(xq, xs, *w["wgu_fp8"], dt)
+    d = ops.mm_fp8(*ops.silu_mul_fp8(gu), *w["wd_fp8"], dt)
+    if next_norm is None:
+        return h + d, None
+    xq, xs, h = ops.add_rms_norm_fp8(d, h, next_norm, cfg.eps)
+    return h, (xq, xs)
+
+
 def _qkv(x, w: dict, cfg: DecoderConfig):
-    """Q, K, V projections of x [..., hidden]: one GEMM over the fused
-    weight when the layer has one."""
+    """Q, K, V projections of x [..., hidden] (of its (codes, scales) for
+    8-bit weights): one GEMM over the fused weight when the layer has one."""
+    nq, nkv = cfg.n_heads * cfg.head_dim, cfg.n_kv_heads * cfg.head_dim
+    if "wqkv_fp8" in w:
+        qkv = torch.ops.spyre.mm_fp8(*x, *w["wqkv_fp8"], w["attn_norm"].dtype)
+        return qkv[..., :nq], qkv[..., nq:nq + nkv], qkv[..., nq + nkv:]
     if "wqkv" in w:
-        nq, nkv = cfg.n_heads * cfg.head_dim, cfg.n_kv_heads * cfg.head_dim
         qkv = F.linear(x, w["wqkv"])
         return qkv[..., :nq], qkv[..., nq:nq + nkv], qkv[..., nq + nkv:]
     return F.linear(x, w["wq"]), F.linear(x, w["wk"]), F.linear(x, w["wv"])
@@ -180,7 +232,7 @@ def layer_forward(h, w: dict, cos, sin, mask, cfg: DecoderConfig, cache_kv=None,
     are one kernel of this layer's compiled graph."""
     B, S, _ = h.shape
     if x is None:
-        x = F.rms_norm(h, (cfg.hidden,), w["attn_norm"], cfg.eps)
+        x = _first_norm(h, w, cfg)
     q, k, v = _qkv(x, w, cfg)
     q = q.reshape(B, S, cfg.n_heads, cfg.head_dim)
     k = k.reshape(B, S, cfg.n_kv_heads, cfg.head_dim)
@@ -191,6 +243,9 @@ def layer_forward(h, w: dict, cos, sin, mask, cfg: DecoderConfig, cache_kv=None,
     if cache_kv is not None:
         cache_kv[0][:, :, :S].copy_(k)
         cache_kv[1][:, :, :, :S].copy_(v.transpose(2, 3))
+    if "wo_fp8" in w:
+        h, x = _rest_of_layer_fp8(_attention(q, k, v, cfg, mask), h, w, cfg, next_norm)
+        return h if next_norm is None else (h, x)
     h = h + F.linear(_attention(q, k, v, cfg, mask), w["wo"]).view(B, S, cfg.hidden)
     x = F.rms_norm(h, (cfg.hidden,), w["mlp_norm"], cfg.eps)
     h = h + _mlp(x, w, cfg)
@@ -218,6 +273,9 @@ def new_cache(cfg: DecoderConfig, batch: int, max_len: int, device, dtype=torch.
 
 def lm_logits(h_last, params: dict, cfg: DecoderConfig):
     """Final RMSNorm + LM head on h_last [B, hidden] -> logits [B, vocab]."""
+    if "lm_head_fp8" in params:
+        x = torch.ops.spyre.rms_norm_fp8(h_last, params["final_norm"], cfg.eps)
+        return torch.ops.spyre.mm_fp8(*x, *params["lm_head_fp8"], h_last.dtype)
     x = F.rms_norm(h_last, (cfg.hidden,), params["final_norm"], cfg.eps)
     return F.linear(x, params["lm_head"])
 
@@ -231,10 +289,13 @@ def prefill(tokens, params: dict, cos, sin, mask, cache, cfg: DecoderConfig, lay
     # Each layer also normalises its output for the next one (the last for
     # the LM head), so every call has the same arguments: one compiled
     # graph serves all layers.
-    x = F.rms_norm(h, (cfg.hidden,), layers[0]["attn_norm"], cfg.eps)
+    x = _first_norm(h, layers[0], cfg)
     for i, w in enumerate(layers):
         nxt = layers[i + 1]["attn_norm"] if i + 1 < len(layers) else params["final_norm"]
         h, x = layer_fn(h, w, cos, sin, mask, cfg, cache[i], x, nxt)
+    if "lm_head_fp8" in params:
+        xq, xs = x
+        return torch.ops.spyre.mm_fp8(xq[:, -1], xs[:, -1], *params["lm_head_fp8"], h.dtype)
     return F.linear(x[:, -1], params["lm_head"])
 
 
@@ -245,7 +306,7 @@ def decode_step(tokens, pos: int, params: dict, cos, sin, cache, cfg: DecoderCon
     h = F.embedding(tokens, params["embed"]).view(B, 1, cfg.hidden)
     c, s = cos[pos:pos + 1], sin[pos:pos + 1]
     for i, w in enumerate(params["layers"]):
-        x = F.rms_norm(h, (cfg.hidden,), w["attn_norm"], cfg.eps)
+        x = _first_norm(h, w, cfg)
         q, k, v = _qkv(x, w, cfg)
         q = apply_rope(q.reshape(B, 1, cfg.n_heads, cfg.head_dim), c, s)
         k = apply_rope(k.reshape(B, 1, cfg.n_kv_heads, cfg.head_dim), c, s)
@@ -254,6 +315,9 @@ def decode_step(tokens, pos: int, params: dict, cos, sin, cache, cfg: DecoderCon
         kc[:, :, pos:pos + 1].copy_(k.transpose(1, 2))
         vc[:, :, :, pos:pos + 1].copy_(v.permute(0, 2, 3, 1))
         kc, vc = kc[:, :, :pos + 1], vc[:, :, :, :pos + 1].transpose(2, 3)
+        if "wo_fp8" in w:
+            h, _ = _rest_of_layer_fp8(_attention(q, kc, vc, cfg, None), h, w, cfg, None)
+            continue
         h = h + F.linear(_attention(q, kc, vc, cfg, None), w["wo"]).view(B, 1, cfg.hidden)
         x = F.rms_norm(h, (cfg.hidden,), w["mlp_norm"], cfg.eps)
         h = h + _mlp(x, w, cfg)
@@ -280,13 +344,20 @@ def decode_step_static(tokens, pos, params: dict, cos, sin, cache, cfg: DecoderC
     keys = torch.arange(L, device=tokens.device)
     mask = torch.where(keys <= pos, 0.0, float("-inf")).to(h.dtype)
     for i, w in enumerate(params["layers"]):
-        x = F.rms_norm(h, (cfg.hidden,), w["attn_norm"], cfg.eps)
-        if fused_attention and "wqkv" in w and cfg.head_dim == 128:
+        x = _first_norm(h, w, cfg)
+        fp8 = "wqkv_fp8" in w
+        if fused_attention and (fp8 or "wqkv" in w) and cfg.head_dim == 128:
             kc, vc = cache[i]
-            qkv = F.linear(x, w["wqkv"]).view(B, -1)
+            if fp8:
+                qkv = torch.ops.spyre.mm_fp8(*x, *w["wqkv_fp8"], h.dtype).view(B, -1)
+            else:
+                qkv = F.linear(x, w["wqkv"]).view(B, -1)
             a = torch.ops.spyre.decode_attention(qkv, cos, sin, pos, kc, vc, cfg.n_heads,
                                                  cfg.n_kv_heads, 1.0 / math.sqrt(cfg.head_dim),
                                                  True)
+            if fp8:
+                h, _ = _rest_of_layer_fp8(a, h, w, cfg, None)
+                continue
             h = h + F.linear(a, w["wo"]).view(B, 1, cfg.hidden)
             x = F.rms_norm(h, (cfg.hidden,), w["mlp_norm"], cfg.eps)
             h = h + _mlp(x, w, cfg)
@@ -298,6 +369,10 @@ def decode_step_static(tokens, pos, params: dict, cos, sin, cache, cfg: DecoderC
         kc, vc = cache[i]
         kc.index_copy_(2, pos, k.transpose(1, 2))
         vc.index_copy_(3, pos, v.permute(0, 2, 3, 1))
+        if fp8:
+            h, _ = _rest_of_layer_fp8(_attention(q, kc, vc.transpose(2, 3), cfg, mask), h, w, cfg,
+                                      None)
+            continue
         h = h + F.linear(_attention(q, kc, vc.transpose(2, 3), cfg, mask),
                          w["wo"]).view(B, 1, cfg.hidden)
         x = F.rms_norm(h, (cfg.hidden,), w["mlp_norm"], cfg.eps)

@@ -247,10 +247,11 @@ def whole_operands(m, n, k, seed=0):
     return x, xs, w, ws
 
 
-def mm64(x, xs, w, ws):
+def mm64(x, xs, w, ws, mags=False):
+    """The product in 64 bits; with mags, that of the magnitudes."""
     a = codes64(x) * spread(xs.double(), x.shape)
     b = codes64(w) * spread(ws.double(), w.shape, 128)
-    return a @ b.t(), a.abs() @ b.abs().t()
+    return a.abs() @ b.abs().t() if mags else a @ b.t()
 
 
 MM_SHAPES = [(1, 1, 1), (1, 128, 128), (1, 6144, 4096), (2, 16, 64), (3, 130, 257), (4, 4100, 1040),
@@ -259,33 +260,35 @@ MM_SHAPES = [(1, 1, 1), (1, 128, 128), (1, 6144, 4096), (2, 16, 64), (3, 130, 25
              (130, 257, 1300), (200, 1024, 2048), (256, 256, 128), (257, 513, 384),
              (333, 640, 4096), (512, 768, 1024), (777, 1100, 272), (300, 2048, 16),
              (24, 4096, 12800), (70, 5000, 1024), (600, 3200, 1920), (1030, 2000, 1310),
-             (777, 6144, 1045), (333, 4096, 6500), (2048, 6144, 512), (1300, 8256, 1024), (1800, 10300, 256), (4096, 9000, 384)]
+             (777, 6144, 1045), (651, 1033, 5539), (333, 4096, 6500), (116, 6117, 5199), (1800, 10300, 256),
+             (2040, 6100, 2048), (3000, 5000, 1536), (4000, 6200, 2048)]
 
 
 def plan(m, n, k, workspace=None):
-    """(kernel, tile, K slices) that the library runs a product on (host only)."""
-    lib, out = _capi.lib(), (ctypes.c_int32 * 4)()
+    """((kernel, rows of X, rows of W, workgroups per CU), K slices) that the
+    library runs a product on (host only)."""
+    lib, out = _capi.lib(), (ctypes.c_int32 * 5)()
     if workspace is None:
         workspace = lib.sph_gemm_fp8_workspace_bytes(m, n, k)
     assert lib.sph_gemm_fp8_plan(m, n, k, workspace, ctypes.addressof(out)) == 0
-    return {1: "stream", 2: "ring", 3: "tiles"}[out[0]], (out[1], out[2]), out[3]
+    return ({1: "stream", 2: "ring", 3: "tiles"}[out[0]], out[1], out[2], out[4]), out[3]
 
 
 def test_mm_shapes_cover_every_kernel():
-    seen = {plan(*s)[:2] for s in MM_SHAPES}
-    assert seen == {("stream", (16, 16)), ("ring", (32, 64)), ("ring", (32, 128)),
-                    ("ring", (64, 128)), ("ring", (128, 128)), ("tiles", (256, 192)),
-                    ("tiles", (256, 256))}
-    assert {plan(*s)[2] > 1 for s in MM_SHAPES} == {True, False}
+    assert {plan(*s)[0] for s in MM_SHAPES} == {
+        ("stream", 16, 16, 4), ("ring", 32, 64, 3), ("ring", 64, 128, 2), ("ring", 64, 128, 3),
+        ("ring", 128, 128, 1), ("ring", 128, 128, 2), ("tiles", 256, 192, 1),
+        ("tiles", 256, 256, 1)}
+    assert {plan(*s)[1] > 1 for s in MM_SHAPES} == {True, False}
     # without a workspace nothing is split
-    assert all(plan(*s, 0)[2] == 1 for s in MM_SHAPES)
+    assert all(plan(*s, 0)[1] == 1 for s in MM_SHAPES)
 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("m,n,k", MM_SHAPES)
 def test_mm_whole_numbers(m, n, k):
     x, xs, w, ws = whole_operands(m, n, k, m + n + k)
-    want, _ = mm64(x, xs, w, ws)
+    want = mm64(x, xs, w, ws)
     # |sums| <= 9 * 12800 in quarters: exact in fp32; rounded once to the type
     dev = [t.to("spyre") for t in (x, xs.t().contiguous().t(), w, ws)]
     for dtype in (torch.bfloat16, torch.float16):
@@ -306,8 +309,8 @@ def test_mm_random(m, n, k, dtype, device):
     wq, ws = ops.quantize_fp8(rand((n, k), 12, 0.05).to(device), 128)
     bias = rand((n,), 13, 0.5, dtype)
     y = ops.mm_fp8(xq, xs, wq, ws, dtype, bias.to(device)).cpu().double()
-    want, mags = mm64(xq.cpu(), xs.cpu(), wq.cpu(), ws.cpu())
-    want = want + bias.double()
+    parts = [t.cpu() for t in (xq, xs, wq, ws)]
+    want, mags = mm64(*parts) + bias.double(), mm64(*parts, mags=True)
     half = torch.finfo(dtype).eps / 2
     bound = mags * 2.0 ** -12 + want.abs() * half * (1 + 2.0 ** -8) + 2.0 ** -24
     assert bool(((y - want).abs() <= bound).all()), ((y - want).abs() / bound).max()
@@ -320,7 +323,7 @@ def test_mm_layouts(m):
     not, scales in every order, inputs of more dimensions."""
     n, k = 260, 200
     x, xs, w, ws = whole_operands(m, n, k, m)
-    want = mm64(x, xs, w, ws)[0].float().half()
+    want = mm64(x, xs, w, ws).float().half()
 
     def inside(t, left, right):
         base = torch.full((t.shape[0] + 2, left + t.shape[1] + right), 0x7F, dtype=torch.uint8)
@@ -342,7 +345,7 @@ def test_mm_layouts(m):
 @pytest.mark.parametrize("m,n,k", [(2, 300, 512), (70, 300, 512), (300, 300, 512)])
 def test_mm_nan_stays_in_its_row_and_column(m, n, k):
     x, xs, w, ws = whole_operands(m, n, k)
-    want = mm64(x, xs, w, ws)[0].float().half()
+    want = mm64(x, xs, w, ws).float().half()
     x.view(torch.uint8)[1, 300] = 0x7F
     w.view(torch.uint8)[131, 17] = 0xFF
     y = ops.mm_fp8(x.to("spyre"), xs.to("spyre"), w.to("spyre"), ws.to("spyre"),

@@ -35,7 +35,7 @@ struct Fp8Plan {
   double us = 0;
 };
 struct Fp8Tile {
-  int m, n;
+  int m, n, per_cu;
 };
 int launch_fp8_stream(bool bf16, const Fp8Args& p, hipStream_t st);
 Fp8Plan fp8_ring_plan(int64_t m, int64_t n, int64_t k, int64_t max_bytes);

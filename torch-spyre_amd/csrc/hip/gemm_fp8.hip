@@ -263,9 +263,9 @@ int launch_dl(Fp8Args p, hipStream_t stream) {
 //     10.3 (10.3), 16 x 12288 x 4096 14.8 (12.1), 1 x 4096 x 12800 12.8 (12.4),
 //     64 x 2048 x 2048 5.8 (6.9), 512 x 256 x 4096 10.2 (8.2)
 //   Others the kernel whose fitted time is the least:
-//     16 x 25600 x 4096 ring 21.7 (streamed 30), 333 x 4096 x 12800 ring 37.5 (256-
+//     16 x 25600 x 4096 ring 21.7 (streamed 30), 333 x 4096 x 12800 ring 34.5 (256-
 //     row tiles 117), 2048 x 6144 x 4096 192-row tiles 47.3 (256-row 50.5, ring
-//     73.8), 2048 x 25600 x 4096 256-row tiles 239 (ring 285)
+//     63), 2048 x 25600 x 4096 256-row tiles 239 (ring 262)
 Fp8Plan fp8_plan(int64_t m, int64_t n, int64_t k, int64_t max_bytes) {
   Fp8Plan best;
   const int64_t wgs = ceil_div(n, 16) * ceil_div(m, 16);
@@ -274,10 +274,16 @@ Fp8Plan fp8_plan(int64_t m, int64_t n, int64_t k, int64_t max_bytes) {
   const double nb = static_cast<double>(k / kGroup);
   best = fp8_ring_plan(m, n, k, max_bytes);
   if (k >= 2 * kGroup && k % kGroup == 0) {
-    constexpr double kLaunch = 1.0, kRound[2] = {5.7, 4.5}, kBlock[2] = {1.29, 1.10};
+    // us of the launch, of a round beside its blocks, and per block with few and
+    // with all CUs at work (they share the chip's power)
+    constexpr double kLaunch = 1.0, kRound[2] = {5.7, 4.7}, kFew[2] = {1.0, 0.95},
+                     kAll[2] = {1.6, 1.33};
     for (int c = 0; c < 2; ++c) {
       const int64_t tiles = ceil_div(m, dl8::BM) * ceil_div(n, c == 0 ? 256 : 192);
-      const double us = kLaunch + static_cast<double>(ceil_div(tiles, 256)) * (kRound[c] + nb * kBlock[c]);
+      const int64_t full = tiles / 256, rest = tiles % 256;
+      double us = kLaunch + static_cast<double>(full) * (kRound[c] + nb * kAll[c]);
+      if (rest > 0)
+        us += kRound[c] + nb * (kFew[c] + (kAll[c] - kFew[c]) * static_cast<double>(rest) / 256);
       if (us < best.us) best = Fp8Plan{Fp8Plan::kTiles, c, 1, 0, 0, us};
     }
   }
@@ -306,13 +312,14 @@ extern "C" int sph_gemm_fp8_plan(int64_t m, int64_t n, int64_t k, int64_t worksp
   SPH_REQUIRE(m > 0 && n > 0 && k > 0 && plan != nullptr, SPH_ERR_INVALID_ARG,
               "sph_gemm_fp8_plan: sizes must be positive");
   const Fp8Plan p = fp8_plan(m, n, k, workspace_bytes);
-  const Fp8Tile t = p.kernel == Fp8Plan::kStream  ? Fp8Tile{16, 16}
+  const Fp8Tile t = p.kernel == Fp8Plan::kStream  ? Fp8Tile{16, 16, 4}
                     : p.kernel == Fp8Plan::kRing ? fp8_ring_tile(p.cfg)
-                                                 : Fp8Tile{dl8::BM, p.cfg == 0 ? 256 : 192};
+                                                 : Fp8Tile{dl8::BM, p.cfg == 0 ? 256 : 192, 1};
   plan[0] = p.kernel;
   plan[1] = t.m;
   plan[2] = t.n;
   plan[3] = p.splits;
+  plan[4] = t.per_cu;
   return SPH_OK;
 }
 

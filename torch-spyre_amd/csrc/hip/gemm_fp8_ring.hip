@@ -1,15 +1,20 @@
 // 8-bit products whose rows do not fill the CUs with 256-row tiles: decode
 // batches, short and ragged prompts.
 //
-//   * Tiles of BM of X's rows by BN of W's on 4 waves (2 x 2), two or three
-//     workgroups per CU; ST - 1 blocks of K in flight through a ring of ST LDS
-//     stages (direct loads, 128 codes a row, chunk c of row r at slot c ^
-//     ((r >> 1) & 7)).
-//   * The block's scales ride in the same stage by one 4-byte load per lane: the
+//   * Tiles of BM of X's rows by BN of W's on 4 or 8 waves (2 along X's rows), one
+//     to three workgroups per CU; a ring of ST LDS stages of KB blocks of K each,
+//     ST - 1 of them in flight (direct loads, 128 codes a row, chunk c of row r
+//     at slot c ^ ((r >> 1) & 7)).
+//   * The blocks' scales ride in the same stage by one 4-byte load per lane: the
 //     first waves fetch X's, the others W's (one value), so they are covered by
 //     the same wait and barrier and need no registers in flight.
 //   * K is split over workgroups until the chip is full: fp32 sums in a caller's
 //     workspace, added in a fixed order by a second kernel.
+//
+// A step of one block costs a small tile some 600 cycles of latency (wait,
+// barrier, LDS, MFMA, FMA) whatever its size, so the small tiles take two blocks
+// a step (256 x 4096 x 4096 in 32 x 64 tiles 12.1 us, 15.1 with one) and the
+// larger ones 8 waves (777 x 6144 x 4096 in 128 x 128 tiles 32.0 us, 39.8 on 4).
 #include <algorithm>
 
 #include "gemm_fp8.h"
@@ -20,13 +25,13 @@ namespace {
 namespace ring8 {
 constexpr uint32_t kOutside = 0x80000000u;  // past every buffer resource
 
-template <int BM_, int BN_, int ST_>
+template <int BM_, int BN_, int NW_, int KB_, int ST_>
 struct Cfg {
-  static constexpr int BM = BM_, BN = BN_, ST = ST_, NW = 4, WTM = BM / 2, WTN = BN / 2;
+  static constexpr int BM = BM_, BN = BN_, KB = KB_, ST = ST_, NW = NW_, WN = NW / 2, WTM = BM / 2, WTN = BN / WN;
   static constexpr int TM = WTM / 16, TN = WTN / 16;
   static constexpr int X_BYTES = BM * kGroup, W_BYTES = BN * kGroup, S_BYTES = NW * 256;
-  static constexpr int STAGE = X_BYTES + W_BYTES + S_BYTES;
-  static constexpr int LX = X_BYTES / 1024 / NW, LW = W_BYTES / 1024 / NW, L = LX + LW + 1;
+  static constexpr int BLK = X_BYTES + W_BYTES + S_BYTES, STAGE = KB * BLK;
+  static constexpr int LX = X_BYTES / 1024 / NW, LW = W_BYTES / 1024 / NW, LB = LX + LW + 1, L = KB * LB;
   static constexpr int XSW = (BM + 63) / 64;  // waves that fetch X's scales
   static_assert(LX * NW * 1024 == X_BYTES && LW * NW * 1024 == W_BYTES, "load lines");
   static_assert(XSW < NW && BN <= kGroup && TN % 2 == 0, "scales, one block of W, tile pairs");
@@ -46,10 +51,10 @@ __device__ inline void wait_blocks(int blocks) {
   wait_vmcnt<0>();
 }
 
-template <typename T, int BM_, int BN_, int ST_>
-__global__ void __launch_bounds__(256) gemm_fp8_ring_kernel(const Fp8Args p) {
-  using C = ring8::Cfg<BM_, BN_, ST_>;
-  constexpr int BM = C::BM, BN = C::BN, ST = C::ST, TM = C::TM, TN = C::TN;
+template <typename T, int BM_, int BN_, int NW_, int KB_, int ST_>
+__global__ void __launch_bounds__(NW_ * 64) gemm_fp8_ring_kernel(const Fp8Args p) {
+  using C = ring8::Cfg<BM_, BN_, NW_, KB_, ST_>;
+  constexpr int BM = C::BM, BN = C::BN, KB = C::KB, ST = C::ST, TM = C::TM, TN = C::TN;
   __shared__ __attribute__((aligned(1024))) char lds[ST * C::STAGE];
   // Workgroup -> (tile, K slice): a contiguous run per XCD, row tiles of one
   // panel of W next to each other.
@@ -63,13 +68,13 @@ __global__ void __launch_bounds__(256) gemm_fp8_ring_kernel(const Fp8Args p) {
   const int split = id % p.splits, tn = id / p.splits;
   const int64_t m0 = static_cast<int64_t>(tm) * BM, n0 = static_cast<int64_t>(tn) * BN;
   const int k = static_cast<int>(p.k), nbf = k / kGroup;
-  const int kb0 = split * p.kslice, ksteps = min(p.kslice, nbf - kb0);
+  const int kb0 = split * p.kslice, nblk = min(p.kslice, nbf - kb0), ksteps = (nblk + KB - 1) / KB;
   const int ldx = static_cast<int>(p.ldx), ldw = static_cast<int>(p.ldw);
   const int xrows = static_cast<int>(min(static_cast<int64_t>(BM), p.m - m0));
   const int wrows = static_cast<int>(min(static_cast<int64_t>(BN), p.n - n0));
   const int lane = threadIdx.x & 63, r16 = lane & 15, g4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
-  const int wm = wave >> 1, wn = wave & 1;
+  const int wm = wave / C::WN, wn = wave % C::WN;
   const i32x4 rx = buffer_rsrc(p.x + m0 * p.ldx, static_cast<uint32_t>((xrows - 1) * ldx + nbf * kGroup));
   const i32x4 rw = buffer_rsrc(p.w + n0 * p.ldw, static_cast<uint32_t>((wrows - 1) * ldw + nbf * kGroup));
   uint32_t vx[C::LX], vw[C::LW];
@@ -92,18 +97,21 @@ __global__ void __launch_bounds__(256) gemm_fp8_ring_kernel(const Fp8Args p) {
   const uint32_t lds_base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((SPH_LDS char*)(lds)));
 
   auto issue = [&](int t, int slot) __attribute__((always_inline)) {
-    const uint32_t sb = lds_base + slot * C::STAGE;
-    const int kb = kb0 + t;
 #pragma unroll
-    for (int i = 0; i < C::LX; ++i)
-      dma16(rx, __builtin_amdgcn_readfirstlane(sb + (wave * C::LX + i) * 1024), vx[i],
-            __builtin_amdgcn_readfirstlane(kb * kGroup));
+    for (int b = 0; b < KB; ++b) {
+      const uint32_t sb = lds_base + slot * C::STAGE + b * C::BLK;
+      const int kb = min(kb0 + t * KB + b, nbf - 1);  // (a block past the slice is not used)
 #pragma unroll
-    for (int i = 0; i < C::LW; ++i)
-      dma16(rw, __builtin_amdgcn_readfirstlane(sb + C::X_BYTES + (wave * C::LW + i) * 1024), vw[i],
-            __builtin_amdgcn_readfirstlane(kb * kGroup));
-    dma4(buffer_rsrc(sbase + kb * sblk, sbytes),
-         __builtin_amdgcn_readfirstlane(sb + C::X_BYTES + C::W_BYTES + wave * 256), vs);
+      for (int i = 0; i < C::LX; ++i)
+        dma16(rx, __builtin_amdgcn_readfirstlane(sb + (wave * C::LX + i) * 1024), vx[i],
+              __builtin_amdgcn_readfirstlane(kb * kGroup));
+#pragma unroll
+      for (int i = 0; i < C::LW; ++i)
+        dma16(rw, __builtin_amdgcn_readfirstlane(sb + C::X_BYTES + (wave * C::LW + i) * 1024), vw[i],
+              __builtin_amdgcn_readfirstlane(kb * kGroup));
+      dma4(buffer_rsrc(sbase + kb * sblk, sbytes),
+           __builtin_amdgcn_readfirstlane(sb + C::X_BYTES + C::W_BYTES + wave * 256), vs);
+    }
   };
 
   const int sw = (g4 ^ ((r16 >> 1) & 7)) << 4;
@@ -124,29 +132,33 @@ __global__ void __launch_bounds__(256) gemm_fp8_ring_kernel(const Fp8Args p) {
     wait_lgkmcnt0();
     __syncthreads();
     if (ks + ST - 1 < ksteps) issue(ks + ST - 1, slot == 0 ? ST - 1 : slot - 1);
-    const char* sp = lds + slot * C::STAGE;
-    const float wsc = *reinterpret_cast<const float*>(sp + soff + (C::NW - 1) * 256);
-    float sc[TM];
-    i32x8 xf[TM], wf[TN];
 #pragma unroll
-    for (int j = 0; j < TM; ++j) {
-      sc[j] = *reinterpret_cast<const float*>(sp + soff + (wm * C::WTM + 16 * j + r16) * 4) * wsc;
-      const char* q = sp + xoff + j * 16 * kGroup;
-      xf[j] = frag(*reinterpret_cast<const u32x4*>(q + sw), *reinterpret_cast<const u32x4*>(q + (sw ^ 64)));
-    }
-#pragma unroll
-    for (int i = 0; i < TN; ++i) {
-      const char* q = sp + woff + i * 16 * kGroup;
-      wf[i] = frag(*reinterpret_cast<const u32x4*>(q + sw), *reinterpret_cast<const u32x4*>(q + (sw ^ 64)));
-    }
-#pragma unroll
-    for (int i = 0; i < TN; ++i)
+    for (int b = 0; b < KB; ++b) {
+      if (b > 0 && ks * KB + b >= nblk) break;
+      const char* sp = lds + slot * C::STAGE + b * C::BLK;
+      const float wsc = *reinterpret_cast<const float*>(sp + soff + (C::NW - 1) * 256);
+      float sc[TM];
+      i32x8 xf[TM], wf[TN];
 #pragma unroll
       for (int j = 0; j < TM; ++j) {
-        const f32x4 s = mfma_block(wf[i], xf[j]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(s[e], sc[j], acc[i][j][e]);
+        sc[j] = *reinterpret_cast<const float*>(sp + soff + (wm * C::WTM + 16 * j + r16) * 4) * wsc;
+        const char* q = sp + xoff + j * 16 * kGroup;
+        xf[j] = frag(*reinterpret_cast<const u32x4*>(q + sw), *reinterpret_cast<const u32x4*>(q + (sw ^ 64)));
       }
+#pragma unroll
+      for (int i = 0; i < TN; ++i) {
+        const char* q = sp + woff + i * 16 * kGroup;
+        wf[i] = frag(*reinterpret_cast<const u32x4*>(q + sw), *reinterpret_cast<const u32x4*>(q + (sw ^ 64)));
+      }
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int j = 0; j < TM; ++j) {
+          const f32x4 s = mfma_block(wf[i], xf[j]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(s[e], sc[j], acc[i][j][e]);
+        }
+    }
     slot = slot + 1 == ST ? 0 : slot + 1;
   }
 
@@ -199,41 +211,45 @@ __global__ void __launch_bounds__(256) gemm_fp8_reduce(const Fp8Args p) {
   store_row4<T>(p, row, col, v);
 }
 
-template <typename T, int BM, int BN, int ST>
+template <typename T, int BM, int BN, int NW, int KB, int ST>
 int launch_ring8(Fp8Args& p, hipStream_t st) {
   p.tiles_m = static_cast<int>(ceil_div(p.m, BM));
   p.tiles_n = static_cast<int>(ceil_div(p.n, BN));
   const unsigned grid = static_cast<unsigned>(p.tiles_m) * p.tiles_n * p.splits;
-  gemm_fp8_ring_kernel<T, BM, BN, ST><<<grid, 256, 0, st>>>(p);
+  gemm_fp8_ring_kernel<T, BM, BN, NW, KB, ST><<<grid, NW * 64, 0, st>>>(p);
   if (p.splits > 1)
     gemm_fp8_reduce<T><<<static_cast<unsigned>(ceil_div(p.m * ceil_div(p.n, 4), 256)), 256, 0, st>>>(p);
   return check_launch("sph_gemm_fp8");
 }
 
-// Tile configurations: per_cu workgroups share a CU (LDS); us of a round of
-// workgroups beside its blocks of K, of the launch, and per block of K with
-// 1, 2 or 3 workgroups on the CU; us of the reduce's launch and TB/s of its
-// sums.  Fitted to 5200 timings of 1 to 2600 rows by 512 to 49155 columns, K
-// 1024 to 12800, 1 to 16 slices (rms error 6 %; the plan that the fitted times
-// choose is 2 % slower than the fastest of a product on average, 16 % at most:
-// 256 x 25600 x 4096).
+// Tile configurations: per_cu workgroups share a CU (LDS), each with `fly` blocks
+// in flight; us of a round of workgroups beside its blocks of K, of the launch,
+// and per block of K with 1, 2 or 3 workgroups on the CU (64 x 128 with 3 is bound
+// by its traffic); us of the reduce's launch and TB/s of its sums; TB/s of the
+// tiles' traffic from the caches.  Fitted to 9000 timings of 1 to 2600 rows by
+// 256 to 49155 columns, K 256 to 12800, 1 to 16 slices (rms error 7 to 18 %; the
+// plan that the fitted times choose is 2 % slower than the fastest of a product
+// on average, 21 % at most: 64 x 25600 x 4096).
 struct RingCfg {
-  int bm, bn, per_cu;
-  double round, launch, blk[3], reduce, sums;
+  int bm, bn, kb, per_cu, fly;
+  double round, launch, blk[3], reduce, sums, traffic;
 };
-constexpr RingCfg kRing[] = {{32, 64, 3, 0.2, 2.3, {0.297, 0.369, 0.492}, 2.5, 4.7},
-                             {32, 128, 2, 0.2, 2.4, {0.442, 0.552, 0}, 2.6, 5.3},
-                             {64, 128, 2, 0.1, 2.9, {0.631, 0.772, 0}, 2.5, 5.4},
-                             {128, 128, 2, 1.6, 2.1, {0.993, 1.186, 0}, 2.6, 5.9}};
+constexpr RingCfg kRing[] = {
+    {32, 64, 2, 3, 2, 2.08, 1.0, {0.263, 0.343, 0.444}, 2.57, 5.51, 18.9},
+    {64, 128, 1, 2, 2, 1.06, 2.05, {0.425, 0.670, 0}, 2.69, 5.20, 16.6},
+    {64, 128, 1, 3, 1, 3.77, 1.0, {0.525, 0.718, 0.02}, 1.30, 4.10, 16.8},
+    {128, 128, 1, 2, 1, 1.54, 1.78, {0.608, 0.945, 0}, 2.59, 4.75, 14.1},
+    {128, 128, 1, 1, 2, 1.54, 2.02, {0.594, 0, 0}, 2.55, 4.92, 11.4}};
 constexpr int kRingCfgs = sizeof(kRing) / sizeof(kRing[0]);
 
 template <typename T>
 int launch_cfg(Fp8Args& p, int cfg, hipStream_t st) {
   switch (cfg) {
-    case 0: return launch_ring8<T, 32, 64, 4>(p, st);
-    case 1: return launch_ring8<T, 32, 128, 3>(p, st);
-    case 2: return launch_ring8<T, 64, 128, 3>(p, st);
-    default: return launch_ring8<T, 128, 128, 2>(p, st);
+    case 0: return launch_ring8<T, 32, 64, 4, 2, 2>(p, st);
+    case 1: return launch_ring8<T, 64, 128, 8, 1, 3>(p, st);
+    case 2: return launch_ring8<T, 64, 128, 8, 1, 2>(p, st);
+    case 3: return launch_ring8<T, 128, 128, 8, 1, 2>(p, st);
+    default: return launch_ring8<T, 128, 128, 8, 1, 3>(p, st);
   }
 }
 
@@ -255,11 +271,17 @@ Fp8Plan fp8_ring_plan(int64_t m, int64_t n, int64_t k, int64_t max_bytes) {
       if (ceil_div(nbf, slice) != s) continue;  // every slice has blocks
       const int64_t bytes = s > 1 ? s * m * pitch * 4 : 0;
       if (bytes > max_bytes) continue;
-      const int64_t full = tiles * s / slots, rest = tiles * s % slots;
-      const double blocks = static_cast<double>(slice);
+      const int64_t wgs = tiles * s, full = wgs / slots, rest = wgs % slots;
+      const double blocks = static_cast<double>(ceil_div(slice, f.kb) * f.kb);
       double us = static_cast<double>(full) * (f.round + blocks * f.blk[f.per_cu - 1]);
       if (rest > 0) us += 0.7 * f.round + blocks * f.blk[(rest - 1) / kCUs];
-      us = f.launch + std::max(us, mem_us);
+      // no faster than what is in flight arrives (1.3 us), the tiles' traffic, or
+      // the operands from memory
+      const double block_bytes = static_cast<double>((f.bm + f.bn) * kGroup);
+      const double fly = static_cast<double>(std::min(wgs, slots) * f.fly) * block_bytes;
+      us = std::max({us, static_cast<double>((m + n) * k) / fly * 1.3, mem_us,
+                     static_cast<double>(wgs * slice) * block_bytes / (f.traffic * 1e6)});
+      us += f.launch;
       if (s > 1) us += f.reduce + 2.0 * static_cast<double>(bytes) / (f.sums * 1e6);
       if (us < best.us) {
         best.kernel = Fp8Plan::kRing;
@@ -274,7 +296,7 @@ Fp8Plan fp8_ring_plan(int64_t m, int64_t n, int64_t k, int64_t max_bytes) {
   return best;
 }
 
-Fp8Tile fp8_ring_tile(int cfg) { return {kRing[cfg].bm, kRing[cfg].bn}; }
+Fp8Tile fp8_ring_tile(int cfg) { return {kRing[cfg].bm, kRing[cfg].bn, kRing[cfg].per_cu}; }
 
 int launch_fp8_ring(bool bf16, Fp8Args p, const Fp8Plan& plan, hipStream_t st) {
   p.splits = plan.splits;

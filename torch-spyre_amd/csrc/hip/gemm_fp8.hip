@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(dl8::NT) gemm_fp8_dl_kernel(const Fp8Args p) {
     // cost registers there)
     int l = lane;
     asm volatile("" : "+v"(l));
-    store_tiles<T, TN, TM>(p, acc, m0 + wm * (TM * 16), n0 + wn * C::WTN, l & 15, l >> 4);
+    store_tiles<T, TN, TM, true>(p, acc, m0 + wm * (TM * 16), n0 + wn * C::WTN, l & 15, l >> 4);
     tile += gridDim.x;
     if (tile >= ntiles) break;
     // a whole tile's stores are TN / 2 * TM instructions
@@ -276,8 +276,8 @@ Fp8Plan fp8_plan(int64_t m, int64_t n, int64_t k, int64_t max_bytes) {
   if (k >= 2 * kGroup && k % kGroup == 0) {
     // us of the launch, of a round beside its blocks, and per block with few and
     // with all CUs at work (they share the chip's power)
-    constexpr double kLaunch = 1.0, kRound[2] = {5.7, 4.7}, kFew[2] = {1.0, 0.95},
-                     kAll[2] = {1.6, 1.33};
+    constexpr double kLaunch = 0.5, kRound[2] = {5.8, 5.0}, kFew[2] = {1.21, 1.01},
+                     kAll[2] = {1.70, 1.38};
     for (int c = 0; c < 2; ++c) {
       const int64_t tiles = ceil_div(m, dl8::BM) * ceil_div(n, c == 0 ? 256 : 192);
       const int64_t full = tiles / 256, rest = tiles % 256;

@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(NW_ * 64) gemm_fp8_ring_kernel(const Fp8Args p
       }
     }
   }
-  if (p.splits == 1) return store_tiles<T, TN, TM>(p, acc, row0, col0, r16, g4);
+  if (p.splits == 1) return store_tiles<T, TN, TM, false>(p, acc, row0, col0, r16, g4);
   const int64_t pitch = (p.n + 3) & ~static_cast<int64_t>(3);
   float* W = p.part + static_cast<int64_t>(split) * p.m * pitch;
 #pragma unroll
@@ -224,22 +224,21 @@ int launch_ring8(Fp8Args& p, hipStream_t st) {
 
 // Tile configurations: per_cu workgroups share a CU (LDS), each with `fly` blocks
 // in flight; us of a round of workgroups beside its blocks of K, of the launch,
-// and per block of K with 1, 2 or 3 workgroups on the CU (64 x 128 with 3 is bound
-// by its traffic); us of the reduce's launch and TB/s of its sums; TB/s of the
-// tiles' traffic from the caches.  Fitted to 9000 timings of 1 to 2600 rows by
-// 256 to 49155 columns, K 256 to 12800, 1 to 16 slices (rms error 7 to 18 %; the
-// plan that the fitted times choose is 2 % slower than the fastest of a product
-// on average, 21 % at most: 64 x 25600 x 4096).
+// and per block of K with 1, 2 or 3 workgroups on the CU; us of the reduce's
+// launch and TB/s of its sums; TB/s of the tiles' traffic from the caches and of
+// the operands from memory.  Fitted to 7300 timings of 1 to 2600 rows by 256 to
+// 49155 columns, K 256 to 12800, 1 to 16 slices (rms error 7 to 13 %; the plan
+// that the fitted times choose is 2 % slower than the fastest of a product on
+// average, 16 % at most: 333 x 25600 x 4096).
 struct RingCfg {
   int bm, bn, kb, per_cu, fly;
-  double round, launch, blk[3], reduce, sums, traffic;
+  double round, launch, blk[3], reduce, sums, traffic, mem;
 };
 constexpr RingCfg kRing[] = {
-    {32, 64, 2, 3, 2, 2.08, 1.0, {0.263, 0.343, 0.444}, 2.57, 5.51, 18.9},
-    {64, 128, 1, 2, 2, 1.06, 2.05, {0.425, 0.670, 0}, 2.69, 5.20, 16.6},
-    {64, 128, 1, 3, 1, 3.77, 1.0, {0.525, 0.718, 0.02}, 1.30, 4.10, 16.8},
-    {128, 128, 1, 2, 1, 1.54, 1.78, {0.608, 0.945, 0}, 2.59, 4.75, 14.1},
-    {128, 128, 1, 1, 2, 1.54, 2.02, {0.594, 0, 0}, 2.55, 4.92, 11.4}};
+    {32, 64, 2, 3, 2, 2.15, 1.0, {0.264, 0.344, 0.439}, 2.44, 5.60, 19.1, 5.24},
+    {64, 128, 1, 2, 2, 0.51, 2.4, {0.428, 0.687, 0}, 2.64, 5.10, 16.7, 5.86},
+    {128, 128, 1, 2, 1, 2.07, 1.42, {0.604, 0.835, 0}, 2.59, 5.12, 13.7, 4.97},
+    {128, 128, 1, 1, 2, 1.54, 2.02, {0.592, 0, 0}, 2.54, 4.96, 12.4, 5.55}};
 constexpr int kRingCfgs = sizeof(kRing) / sizeof(kRing[0]);
 
 template <typename T>
@@ -247,8 +246,7 @@ int launch_cfg(Fp8Args& p, int cfg, hipStream_t st) {
   switch (cfg) {
     case 0: return launch_ring8<T, 32, 64, 4, 2, 2>(p, st);
     case 1: return launch_ring8<T, 64, 128, 8, 1, 3>(p, st);
-    case 2: return launch_ring8<T, 64, 128, 8, 1, 2>(p, st);
-    case 3: return launch_ring8<T, 128, 128, 8, 1, 2>(p, st);
+    case 2: return launch_ring8<T, 128, 128, 8, 1, 2>(p, st);
     default: return launch_ring8<T, 128, 128, 8, 1, 3>(p, st);
   }
 }
@@ -260,7 +258,7 @@ Fp8Plan fp8_ring_plan(int64_t m, int64_t n, int64_t k, int64_t max_bytes) {
   best.us = 1e30;
   constexpr int64_t kCUs = 256;
   const int64_t nbf = k / kGroup, pitch = (n + 3) / 4 * 4;
-  const double mem_us = static_cast<double>(m * k + n * k + 2 * m * n) / 5.6e6;
+  const double mem_mb = static_cast<double>(m * k + n * k + 2 * m * n) * 1e-6;
   for (int c = 0; c < kRingCfgs; ++c) {
     const RingCfg& f = kRing[c];
     const int64_t tiles = ceil_div(m, f.bm) * ceil_div(n, f.bn), slots = kCUs * f.per_cu;
@@ -279,7 +277,7 @@ Fp8Plan fp8_ring_plan(int64_t m, int64_t n, int64_t k, int64_t max_bytes) {
       // the operands from memory
       const double block_bytes = static_cast<double>((f.bm + f.bn) * kGroup);
       const double fly = static_cast<double>(std::min(wgs, slots) * f.fly) * block_bytes;
-      us = std::max({us, static_cast<double>((m + n) * k) / fly * 1.3, mem_us,
+      us = std::max({us, static_cast<double>((m + n) * k) / fly * 1.3, mem_mb / f.mem,
                      static_cast<double>(wgs * slice) * block_bytes / (f.traffic * 1e6)});
       us += f.launch;
       if (s > 1) us += f.reduce + 2.0 * static_cast<double>(bytes) / (f.sums * 1e6);

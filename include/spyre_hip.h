@@ -348,7 +348,9 @@ int64_t sph_gemm_fp8_workspace_bytes(int64_t m, int64_t n, int64_t k);
 
 /* What a product of these sizes runs on, without launching it (host only):
  * plan[0] the kernel, [1] and [2] its tile (rows of X, rows of W), [3] the K
- * slices of its tiles, [4] how many workgroups share a CU. */
+ * slices of its tiles, [4] how many workgroups share a CU; where not 0, [5] how
+ * many columns ([6] = 1) or rows ([6] = 2) it takes, the others being a product
+ * of their own. */
 typedef enum sph_fp8_kernel {
   SPH_FP8_STREAM = 1, /* few rows, straight from memory */
   SPH_FP8_RING = 2,   /* ring of LDS stages, small and ragged rows */

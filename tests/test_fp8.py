@@ -261,17 +261,20 @@ MM_SHAPES = [(1, 1, 1), (1, 128, 128), (1, 6144, 4096), (2, 16, 64), (3, 130, 25
              (333, 640, 4096), (512, 768, 1024), (777, 1100, 272), (300, 2048, 16),
              (24, 4096, 12800), (70, 5000, 1024), (600, 3200, 1920), (1030, 2000, 1310),
              (777, 6144, 1045), (651, 1033, 5539), (73, 7747, 5376), (333, 4096, 6500), (116, 6117, 5199), (1800, 10300, 256),
-             (2040, 6100, 2048), (3000, 5000, 1536), (4000, 6200, 2048)]
+             (2040, 6100, 2048), (3000, 5000, 1536), (4000, 6200, 2048),
+             (2313, 5123, 1152), (3459, 4616, 896), (2591, 6357, 1152)]
 
 
 def plan(m, n, k, workspace=None):
-    """((kernel, rows of X, rows of W, workgroups per CU), K slices) that the
-    library runs a product on (host only)."""
-    lib, out = _capi.lib(), (ctypes.c_int32 * 5)()
+    """((kernel, rows of X, rows of W, workgroups per CU), K slices, "", "columns"
+    or "rows": what is split off for a second product) that the library runs a
+    product on (host only)."""
+    lib, out = _capi.lib(), (ctypes.c_int32 * 7)()
     if workspace is None:
         workspace = lib.sph_gemm_fp8_workspace_bytes(m, n, k)
     assert lib.sph_gemm_fp8_plan(m, n, k, workspace, ctypes.addressof(out)) == 0
-    return ({1: "stream", 2: "ring", 3: "tiles"}[out[0]], out[1], out[2], out[4]), out[3]
+    return ({1: "stream", 2: "ring", 3: "tiles"}[out[0]], out[1], out[2], out[4]), out[3], ("", "columns",
+            "rows")[out[6]]
 
 
 def test_mm_shapes_cover_every_kernel():
@@ -280,6 +283,7 @@ def test_mm_shapes_cover_every_kernel():
         ("ring", 128, 128, 1), ("ring", 128, 128, 2), ("tiles", 256, 192, 1),
         ("tiles", 256, 256, 1)}
     assert {plan(*s)[1] > 1 for s in MM_SHAPES} == {True, False}
+    assert {plan(*s)[2] for s in MM_SHAPES} == {"", "columns", "rows"}
     # without a workspace nothing is split
     assert all(plan(*s, 0)[1] == 1 for s in MM_SHAPES)
 

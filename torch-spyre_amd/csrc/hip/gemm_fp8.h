@@ -20,6 +20,7 @@ struct Fp8Args {
   const void* bias;
   void* d;
   int64_t ldd;
+  int whole_lines;  // every row of d begins on 128 bytes
   int tiles_m, tiles_n;
   // K split: `splits` workgroups of kslice blocks each per tile, fp32 sums of
   // split s at part + s * m * pitch (pitch: n rounded up to 4).
@@ -33,6 +34,8 @@ struct Fp8Plan {
   int cfg = 0, splits = 1, kslice = 0;
   int64_t bytes = 0;  // of workspace
   double us = 0;
+  // where not 0: this plan's columns (rows); the others are a product of their own
+  int64_t n1 = 0, m1 = 0;
 };
 struct Fp8Tile {
   int m, n, per_cu;
@@ -99,12 +102,12 @@ __device__ inline i32x8 load_frag(const uint8_t* row, int64_t b, int64_t k, int 
 }
 
 // 8 consecutive results of one row, the last row piece element by element.
-template <typename T, bool NT>
+template <typename T>
 __device__ inline void store_row8(const Fp8Args& p, int64_t row, int64_t col, u32x4 v) {
   if (row >= p.m || col >= p.n) return;
   T* dp = static_cast<T*>(p.d) + row * p.ldd + col;
   if (col + 8 <= p.n) {
-    if constexpr (NT)
+    if (p.whole_lines)
       __builtin_nontemporal_store(v, reinterpret_cast<u32x4_any*>(dp));
     else
       *reinterpret_cast<u32x4_any*>(dp) = v;
@@ -142,11 +145,11 @@ __device__ inline void store_row4(const Fp8Args& p, int64_t row, int64_t col, f3
 // .. + 3 of row row0 + 16 j + r16 in lane 16 g4 + r16.  v_permlane16_swap
 // exchanges the odd 16-lane rows of one tile with the even ones of the next, so
 // that a lane holds 8 consecutive columns and a store covers 64 bytes of a row,
-// without LDS or a barrier.  NT: streaming stores, for outputs that leave in
-// bursts of whole lines (4096 x 16384 x 4096 in 256-row tiles 247 us without, 227
-// with); rows of odd length need the cache to join their pieces (24 x 49155 x
-// 4096 50 us with, 43 without).
-template <typename T, int TN, int TM, bool NT>
+// without LDS or a barrier.  Rows that begin on cache lines (128 bytes) leave by
+// streaming stores (4096 x 16384 x 4096 in 256-row tiles 267 us without, 249 with);
+// other rows need the cache to join their pieces (4000 x 6200 x 2048 86 us with,
+// 61 without; 24 x 49155 x 4096 50 and 43).
+template <typename T, int TN, int TM>
 __device__ inline void store_tiles(const Fp8Args& p, f32x4 (&acc)[TN][TM], int64_t row0,
                                    int64_t col0, int r16, int g4) {
   static_assert(TN % 2 == 0, "tiles go out in pairs");
@@ -168,7 +171,7 @@ __device__ inline void store_tiles(const Fp8Args& p, f32x4 (&acc)[TN][TM], int64
       const f32x4 u = acc[i][j] + b[0], w = acc[i + 1][j] + b[1];
       const auto lo = __builtin_amdgcn_permlane16_swap(pack2<T>(u[0], u[1]), pack2<T>(w[0], w[1]), false, false);
       const auto hi = __builtin_amdgcn_permlane16_swap(pack2<T>(u[2], u[3]), pack2<T>(w[2], w[3]), false, false);
-      store_row8<T, NT>(p, row0 + 16 * j + r16, col0 + 16 * (i + (g4 & 1)) + 8 * (g4 >> 1),
+      store_row8<T>(p, row0 + 16 * j + r16, col0 + 16 * (i + (g4 & 1)) + 8 * (g4 >> 1),
                     u32x4{lo[0], hi[0], lo[1], hi[1]});
     }
   }

@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(dl8::NT) gemm_fp8_dl_kernel(const Fp8Args p) {
     // cost registers there)
     int l = lane;
     asm volatile("" : "+v"(l));
-    store_tiles<T, TN, TM, true>(p, acc, m0 + wm * (TM * 16), n0 + wn * C::WTN, l & 15, l >> 4);
+    store_tiles<T, TN, TM>(p, acc, m0 + wm * (TM * 16), n0 + wn * C::WTN, l & 15, l >> 4);
     tile += gridDim.x;
     if (tile >= ntiles) break;
     // a whole tile's stores are TN / 2 * TM instructions
@@ -245,14 +245,30 @@ __global__ void __launch_bounds__(dl8::NT) gemm_fp8_dl_kernel(const Fp8Args p) {
   wait_vmcnt<0>();  // the last loads land before the LDS is given back
 }
 
+constexpr int64_t kTileCUs = 256;
+
 template <typename T, int TN>
 int launch_dl(Fp8Args p, hipStream_t stream) {
   using C = dl8::Cfg<TN>;
   p.tiles_m = static_cast<int>(ceil_div(p.m, dl8::BM));
   p.tiles_n = static_cast<int>(ceil_div(p.n, C::BN));
-  const int grid = std::min(p.tiles_m * p.tiles_n, 256);
+  const int grid = std::min<int>(p.tiles_m * p.tiles_n, kTileCUs);
   gemm_fp8_dl_kernel<T, TN><<<grid, dl8::NT, 0, stream>>>(p);
   return check_launch("sph_gemm_fp8");
+}
+
+// us of `tiles` 256- (c = 0) or 192-row tiles: the launch, and per round what it
+// takes beside its blocks and per block, with few and with all CUs at work (they
+// share the chip's power).
+double tiles_us(int c, int64_t tiles, int64_t k) {
+  constexpr double kLaunch = 0.5, kRound[2] = {5.8, 5.0}, kFew[2] = {1.21, 1.01},
+                   kAll[2] = {1.62, 1.36};
+  const double nb = static_cast<double>(k / kGroup);
+  const int64_t full = tiles / kTileCUs, rest = tiles % kTileCUs;
+  double us = kLaunch + static_cast<double>(full) * (kRound[c] + nb * kAll[c]);
+  if (rest > 0)
+    us += kRound[c] + nb * (kFew[c] + (kAll[c] - kFew[c]) * static_cast<double>(rest) / kTileCUs);
+  return us;
 }
 
 // The kernel of a product (one MI355X, operands of three products in turn, us).
@@ -266,35 +282,70 @@ int launch_dl(Fp8Args p, hipStream_t stream) {
 //     16 x 25600 x 4096 ring 21.7 (streamed 30), 333 x 4096 x 12800 ring 34.5 (256-
 //     row tiles 117), 2048 x 6144 x 4096 192-row tiles 47.3 (256-row 50.5, ring
 //     63), 2048 x 25600 x 4096 256-row tiles 239 (ring 262)
-Fp8Plan fp8_plan(int64_t m, int64_t n, int64_t k, int64_t max_bytes) {
+//   Large tiles that would leave most of a last round of workgroups idle take whole
+// rounds alone and leave the other rows (or columns) to a second product, where
+// the fitted times gain 13 %: 2600 x 6144 x 4096 71, whole 82 (192-row tiles) and
+// 78 (ring); 22 such products of random sizes took 0.84 to 1.09 (on average 0.96)
+// of the fastest single kernel.  With less to gain it pays little or nothing: 4096 x
+// 25600 x 4096 417 and 427, 1500 x 25600 x 4096 169 and 171, 4000 x 6200 x 2048 77
+// and 63.
+Fp8Plan fp8_plan(int64_t m, int64_t n, int64_t k, int64_t max_bytes, bool whole = false) {
   Fp8Plan best;
   const int64_t wgs = ceil_div(n, 16) * ceil_div(m, 16);
   if (k < kGroup || (wgs <= 512 && k <= 32 * kGroup && wgs * k <= (m <= 16 ? 1 << 21 : 1 << 20)))
     return best;
-  const double nb = static_cast<double>(k / kGroup);
   best = fp8_ring_plan(m, n, k, max_bytes);
-  if (k >= 2 * kGroup && k % kGroup == 0) {
-    // us of the launch, of a round beside its blocks, and per block with few and
-    // with all CUs at work (they share the chip's power)
-    constexpr double kLaunch = 0.5, kRound[2] = {5.8, 5.0}, kFew[2] = {1.21, 1.01},
-                     kAll[2] = {1.70, 1.38};
-    for (int c = 0; c < 2; ++c) {
-      const int64_t tiles = ceil_div(m, dl8::BM) * ceil_div(n, c == 0 ? 256 : 192);
-      const int64_t full = tiles / 256, rest = tiles % 256;
-      double us = kLaunch + static_cast<double>(full) * (kRound[c] + nb * kAll[c]);
-      if (rest > 0)
-        us += kRound[c] + nb * (kFew[c] + (kAll[c] - kFew[c]) * static_cast<double>(rest) / 256);
-      if (us < best.us) best = Fp8Plan{Fp8Plan::kTiles, c, 1, 0, 0, us};
+  if (k < 2 * kGroup || k % kGroup != 0) return best;
+  for (int c = 0; c < 2; ++c) {
+    const int64_t bn = c == 0 ? 256 : 192, tm = ceil_div(m, dl8::BM), tn = ceil_div(n, bn);
+    const double us = tiles_us(c, tm * tn, k);
+    if (us < best.us) best = Fp8Plan{Fp8Plan::kTiles, c, 1, 0, 0, us};
+    const int64_t full = tm * tn / kTileCUs * kTileCUs;
+    if (whole || full == 0 || full == tm * tn) continue;
+    const int64_t unit = c == 0 ? 256 : 384;  // whole tiles and whole blocks of W
+    const int64_t n1 = full / tm * bn / unit * unit, m1 = full / tn * dl8::BM;
+    for (const bool cols : {true, false}) {
+      const int64_t done = cols ? n1 : m1;
+      if (done == 0 || done >= (cols ? n : m)) continue;
+      const Fp8Plan rest = cols ? fp8_plan(m, n - done, k, max_bytes, true)
+                                : fp8_plan(m - done, n, k, max_bytes, true);
+      const double both = tiles_us(c, cols ? tm * (done / bn) : done / dl8::BM * tn, k) + rest.us;
+      if (both < 0.87 * best.us) {
+        best = Fp8Plan{Fp8Plan::kTiles, c, 1, 0, rest.bytes, both};
+        (cols ? best.n1 : best.m1) = done;
+      }
     }
   }
   return best;
 }
 
-int launch(bool bf16, Fp8Args p, const Fp8Plan& plan, hipStream_t st) {
+int launch(bool bf16, const Fp8Args& p, const Fp8Plan& plan, hipStream_t st) {
   if (plan.kernel == Fp8Plan::kStream) return launch_fp8_stream(bf16, p, st);
   if (plan.kernel == Fp8Plan::kRing) return launch_fp8_ring(bf16, p, plan, st);
   if (plan.cfg == 1) return bf16 ? launch_dl<bf16_t, 6>(p, st) : launch_dl<half_t, 6>(p, st);
   return bf16 ? launch_dl<bf16_t, 8>(p, st) : launch_dl<half_t, 8>(p, st);
+}
+
+int run(bool bf16, const Fp8Args& p, int64_t max_bytes, hipStream_t st) {
+  const Fp8Plan plan = fp8_plan(p.m, p.n, p.k, max_bytes);
+  if (plan.m1 == 0 && plan.n1 == 0) return launch(bf16, p, plan, st);
+  Fp8Args first = p, rest = p;
+  if (plan.n1 > 0) {
+    first.n = plan.n1;
+    rest.n -= plan.n1;
+    rest.w += plan.n1 * p.ldw;
+    rest.ws += plan.n1 / kGroup * p.ws_row;
+    if (p.bias != nullptr) rest.bias = static_cast<const uint16_t*>(p.bias) + plan.n1;
+    rest.d = static_cast<uint16_t*>(p.d) + plan.n1;
+  } else {
+    first.m = plan.m1;
+    rest.m -= plan.m1;
+    rest.x += plan.m1 * p.ldx;
+    rest.xs += plan.m1 * p.xs_row;
+    rest.d = static_cast<uint16_t*>(p.d) + plan.m1 * p.ldd;
+  }
+  if (const int rc = launch(bf16, first, plan, st)) return rc;
+  return launch(bf16, rest, fp8_plan(rest.m, rest.n, rest.k, max_bytes, true), st);
 }
 
 }  // namespace
@@ -320,6 +371,8 @@ extern "C" int sph_gemm_fp8_plan(int64_t m, int64_t n, int64_t k, int64_t worksp
   plan[2] = t.n;
   plan[3] = p.splits;
   plan[4] = t.per_cu;
+  plan[5] = static_cast<int32_t>(p.n1 > 0 ? p.n1 : p.m1);
+  plan[6] = p.n1 > 0 ? 1 : p.m1 > 0 ? 2 : 0;
   return SPH_OK;
 }
 
@@ -371,11 +424,11 @@ extern "C" int sph_gemm_fp8(sph_dtype dtype, int64_t m, int64_t n, int64_t k, co
                   bias,
                   d,
                   ldd,
+                  (reinterpret_cast<uintptr_t>(d) % 128 == 0 && ldd % 64 == 0) ? 1 : 0,
                   0,
                   0,
                   1,
                   0,
                   static_cast<float*>(workspace)};
-  const Fp8Plan plan = fp8_plan(m, n, k, workspace != nullptr ? workspace_bytes : 0);
-  return launch(dtype == SPH_BF16, p, plan, as_stream(stream));
+  return run(dtype == SPH_BF16, p, workspace != nullptr ? workspace_bytes : 0, as_stream(stream));
 }

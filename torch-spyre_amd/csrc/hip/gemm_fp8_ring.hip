@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(NW_ * 64) gemm_fp8_ring_kernel(const Fp8Args p
       }
     }
   }
-  if (p.splits == 1) return store_tiles<T, TN, TM, false>(p, acc, row0, col0, r16, g4);
+  if (p.splits == 1) return store_tiles<T, TN, TM>(p, acc, row0, col0, r16, g4);
   const int64_t pitch = (p.n + 3) & ~static_cast<int64_t>(3);
   float* W = p.part + static_cast<int64_t>(split) * p.m * pitch;
 #pragma unroll
@@ -229,7 +229,8 @@ int launch_ring8(Fp8Args& p, hipStream_t st) {
 // the operands from memory.  Fitted to 7300 timings of 1 to 2600 rows by 256 to
 // 49155 columns, K 256 to 12800, 1 to 16 slices (rms error 7 to 13 %; the plan
 // that the fitted times choose is 2 % slower than the fastest of a product on
-// average, 16 % at most: 333 x 25600 x 4096).
+// average, 16 % at most: 333 x 25600 x 4096), the 128-row tiles' traffic then set to
+// that of products of several rounds (777 x 6144 to 4000 x 6144).
 struct RingCfg {
   int bm, bn, kb, per_cu, fly;
   double round, launch, blk[3], reduce, sums, traffic, mem;
@@ -237,8 +238,8 @@ struct RingCfg {
 constexpr RingCfg kRing[] = {
     {32, 64, 2, 3, 2, 2.15, 1.0, {0.264, 0.344, 0.439}, 2.44, 5.60, 19.1, 5.24},
     {64, 128, 1, 2, 2, 0.51, 2.4, {0.428, 0.687, 0}, 2.64, 5.10, 16.7, 5.86},
-    {128, 128, 1, 2, 1, 2.07, 1.42, {0.604, 0.835, 0}, 2.59, 5.12, 13.7, 4.97},
-    {128, 128, 1, 1, 2, 1.54, 2.02, {0.592, 0, 0}, 2.54, 4.96, 12.4, 5.55}};
+    {128, 128, 1, 2, 1, 2.07, 1.42, {0.604, 0.835, 0}, 2.59, 5.12, 11.8, 4.97},
+    {128, 128, 1, 1, 2, 1.54, 2.02, {0.592, 0, 0}, 2.54, 4.96, 11.4, 5.55}};
 constexpr int kRingCfgs = sizeof(kRing) / sizeof(kRing[0]);
 
 template <typename T>

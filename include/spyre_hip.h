@@ -335,10 +335,11 @@ int sph_silu_mul_fp8(sph_dtype dtype, const void* gu, int64_t ld, int64_t rows, 
  * have to be finite.  Rows of X and W must begin on 16 bytes (else
  * SPH_ERR_UNSUPPORTED) and are read in whole aligned 16-byte chunks; what lies
  * past k in the last one does not count.  m is at most 1048560, k, ldx and ldw
- * at most 4194303, x_scale_row_stride at most 2097152.  workspace (may be NULL) of
- * sph_gemm_fp8_workspace_bytes(m, n, k) bytes (0 for many shapes) lets the K
- * range be split over workgroups; calls sharing one must be ordered on a
- * stream. */
+ * at most 4194303, x_scale_row_stride at most 2097152 (m of 1: any), n what the
+ * grid holds (134217712 with k below 128): else SPH_ERR_TOO_LARGE.  workspace (may
+ * be NULL, 16-byte aligned) of sph_gemm_fp8_workspace_bytes(m, n, k) bytes (0 for
+ * many shapes) lets the K range be split over workgroups; calls sharing one must
+ * be ordered on a stream. */
 int sph_gemm_fp8(sph_dtype dtype, int64_t m, int64_t n, int64_t k, const void* x, int64_t ldx,
                  const float* x_scale, int64_t x_scale_row_stride, int64_t x_scale_group_stride,
                  const void* w, int64_t ldw, const float* w_scale, int64_t w_scale_row_stride,

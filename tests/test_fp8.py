@@ -346,7 +346,7 @@ def test_mm_layouts(m):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("m,n,k", [(2, 300, 512), (70, 300, 512), (300, 300, 512)])
+@pytest.mark.parametrize("m,n,k", [(2, 300, 512), (70, 300, 512), (300, 300, 512), (2040, 6100, 1024)])
 def test_mm_nan_stays_in_its_row_and_column(m, n, k):
     x, xs, w, ws = whole_operands(m, n, k)
     want = mm64(x, xs, w, ws).float().half()
@@ -357,6 +357,75 @@ def test_mm_nan_stays_in_its_row_and_column(m, n, k):
     nan = torch.zeros(m, n, dtype=torch.bool)
     nan[1], nan[:, 131] = True, True
     assert torch.equal(y.isnan(), nan) and torch.equal(y[~nan], want[~nan])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(2, 1100, 512), (40, 1100, 600), (300, 1100, 640), (2040, 6100, 1024)])
+def test_mm_rows_far_apart(m, n, k):
+    """Rows of W (and, from 1030 rows on, X) that reach past 2^32 bytes."""
+    x, xs, w, ws = whole_operands(m, n, k, m)
+
+    def apart(t):
+        ld = 4194288  # the largest stride of whole chunks
+        base = torch.empty(t.shape[0] * ld, dtype=torch.uint8, device="spyre").view(E4M3)
+        view = base.as_strided(t.shape, (ld, 1))
+        view.copy_(t.to("spyre"))
+        return view
+
+    y = ops.mm_fp8(apart(x), xs.to("spyre"), apart(w), ws.to("spyre"), torch.float16)
+    assert torch.equal(y.cpu(), mm64(x, xs, w, ws).float().half())
+
+
+@pytest.mark.gpu
+def test_mm_result_past_32_bits():
+    """50000 x 49152 results are 4.9 GB; the last rows against a product of their own."""
+    m, n, k = 50000, 49152, 128
+    x, xs, w, ws = (t.to("spyre") for t in whole_operands(m, n, k))
+    y = ops.mm_fp8(x, xs, w, ws, torch.bfloat16)
+    for rows in (slice(0, 70), slice(43690, 43760), slice(m - 70, m)):
+        want = mm64(*(t.cpu() for t in (x[rows], xs[rows], w, ws)))
+        assert torch.equal(y[rows].cpu(), want.float().to(torch.bfloat16))
+
+
+@pytest.mark.gpu
+def test_rows_past_32_bits():
+    """Row kernels on 70000 x 32768 values (4.6 GB): the last rows as on their own."""
+    x = torch.empty(70000, 32768, dtype=torch.bfloat16, device="spyre")
+    tail = rand((40, 32768), 21).to("spyre")
+    x[-40:] = tail
+    x[:40] = tail
+    runs = [lambda t: ops.quantize_fp8(t), lambda t: ops.quantize_fp8(t[:, :4160]),
+            lambda t: ops.silu_mul_fp8(t), lambda t: ops.rms_norm_fp8(t, None, 1e-5),
+            lambda t: ops.rms_norm_fp8(t[:, :4096], None, 1e-5),
+            lambda t: ops.add_rms_norm_fp8(t[:, :1024], t[:, 1024:2048], None, 1e-5)]
+    for run in runs:
+        for big, alone in zip(run(x), run(tail)):
+            for part in (big[-40:], big[:40]):
+                assert torch.equal(part.cpu().float(), alone.cpu().float())
+
+
+@pytest.mark.gpu
+def test_mm_on_two_streams_at_once():
+    """Two products with K slices, each with a workspace of its own, through the C
+    entry on two streams."""
+    lib = _capi.lib()
+    jobs = []
+    for m, n, k in ((16, 300, 6400), (70, 900, 4096)):
+        host = whole_operands(m, n, k, m)
+        dev = [t.cuda() for t in host]
+        nws = lib.sph_gemm_fp8_workspace_bytes(m, n, k)
+        assert nws > 0
+        jobs.append((m, n, k, host, dev, torch.empty(nws, dtype=torch.uint8, device="cuda"),
+                     torch.zeros(m, n, dtype=torch.float16, device="cuda"), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for m, n, k, _, (x, xs, w, ws), wsp, y, st in jobs:
+            _capi.call("sph_gemm_fp8", _capi.F16, m, n, k, x.data_ptr(), k, xs.data_ptr(),
+                       *xs.stride(), w.data_ptr(), k, ws.data_ptr(), *ws.stride(), None,
+                       y.data_ptr(), n, wsp.data_ptr(), wsp.numel(), st.cuda_stream)
+    torch.cuda.synchronize()
+    for *_, host, _, _, y, _ in jobs:
+        assert torch.equal(y.cpu(), mm64(*host).float().half())
 
 
 @pytest.mark.parametrize("device", DEVICES)
@@ -449,6 +518,33 @@ def test_c_entry_refusals():
     assert gemm(x=P + 8) == 1002 and gemm(w=P + 1) == 1002 and gemm(ldx=264) == 1002
     assert gemm(k=1 << 30, ldx=1 << 30, ldw=1 << 30) == 1003
     assert gemm(m=0, x=None, d=None) == 0
+
+
+def test_c_entry_limits():
+    """More workgroups than a launch holds, sizes past the limits and a workspace
+    off 16 bytes: refused on the host."""
+    lib, F16 = _capi.lib(), _capi.F16
+    P = 0x10000  # never read
+
+    def gemm(m, n, k, ld=4096, wsp=None, nws=0):
+        return lib.sph_gemm_fp8(F16, m, n, k, P, ld, P, 1, 1, P, ld, P, 1, 1, None, P, n, wsp, nws,
+                                None)
+
+    assert gemm(1, 134217713, 16) == 1003 and gemm(1, 1 << 31, 16) == 1003
+    assert gemm(20, 1 << 30, 256) == 1003 and gemm(1048561, 8, 16) == 1003
+    assert gemm(1 << 20, 1 << 21, 16) == 1003 and gemm(4, 8, 256, wsp=P + 4, nws=64) == 1002
+    out = (ctypes.c_int32 * 7)()
+    for m, n, k in ((1 << 40, 1 << 40, 1 << 40), (1, 1 << 31, 16), (8, 8, 1 << 22)):
+        assert lib.sph_gemm_fp8_workspace_bytes(m, n, k) == 0
+        assert lib.sph_gemm_fp8_plan(m, n, k, 0, ctypes.addressof(out)) == 1003
+    big = 1 << 29  # rows of one column (or two)
+    assert lib.sph_silu_mul_fp8(F16, P, 2, big, 1, P, 1, P, 1, big, None) == 1003
+    assert lib.sph_rmsnorm_fp8(F16, F16, P, 1, None, 0, None, None, 0, big, 1, 1e-5, P, 1, P, 1, big,
+                               None) == 1003
+    assert lib.sph_rmsnorm_fp8(F16, F16, P, 16384, None, 0, None, None, 0, 1 << 22, 16384, 1e-5, P,
+                               16384, P, 1, 1 << 22, None) == 1003
+    for rows in (1 << 60, (1 << 63) - 1):
+        assert lib.sph_quantize_fp8(F16, P, 8, rows, 8, 1, P, 8, P, 1, 1, None) == 1003
 
 
 def test_fakes_match_the_formulas():

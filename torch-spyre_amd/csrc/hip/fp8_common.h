@@ -17,5 +17,12 @@ constexpr uint32_t kLeastBits = 0x0d800000u;
 
 inline int64_t groups(int64_t cols) { return ceil_div(cols, kGroup); }
 
+// A grid dimension holds fewer than 2^32 threads.
+inline int check_grid(const char* what, int64_t workgroups, int64_t threads) {
+  SPH_REQUIRE(workgroups <= UINT32_MAX / threads, SPH_ERR_TOO_LARGE,
+              std::string(what) + ": more workgroups than a launch holds");
+  return SPH_OK;
+}
+
 }  // namespace fp8
 }  // namespace sph

@@ -310,8 +310,6 @@ __global__ void __launch_bounds__(1024) fp8_rmsnorm_long_kernel(const NormArgs p
   for (int g = t; g < ng; g += NT) p.o.scale[row * p.o.sr + g * p.o.sg] = amax[g] * rstd / kTop;
 }
 
-constexpr int64_t kMaxGrid = 0x7fffffff;
-
 // Rows, columns and strides common to the entry points below.
 int check_out(const char* what, int64_t rows, int64_t cols, const Out& o) {
   SPH_REQUIRE(rows >= 0 && cols >= 0, SPH_ERR_INVALID_ARG, std::string(what) + ": negative size");
@@ -321,7 +319,7 @@ int check_out(const char* what, int64_t rows, int64_t cols, const Out& o) {
               std::string(what) + ": ldq is less than the columns");
   SPH_REQUIRE(o.sr >= 0 && o.sg >= 0, SPH_ERR_INVALID_ARG,
               std::string(what) + ": negative scale stride");
-  SPH_REQUIRE(ceil_div(rows, 16) <= kMaxGrid && cols <= kMaxGrid, SPH_ERR_TOO_LARGE,
+  SPH_REQUIRE(rows <= int64_t{1} << 48 && cols <= INT32_MAX, SPH_ERR_TOO_LARGE,
               std::string(what) + ": too many rows or columns");
   return SPH_OK;
 }
@@ -331,6 +329,7 @@ int launch_groups(const char* what, const S& src, const Out& o, int64_t rows, in
                   hipStream_t stream) {
   const int64_t ng = fp8::groups(cols), nr = ceil_div(rows, 16);
   const int64_t gx = S::kRowsFirst ? nr : ng, gy = S::kRowsFirst ? ng : nr;
+  if (const int rc = fp8::check_grid(what, gx, 256)) return rc;
   const dim3 grid(static_cast<uint32_t>(gx), static_cast<uint32_t>(gy < 65535 ? gy : 65535));
   fp8_groups_kernel<S><<<grid, 256, 0, stream>>>(src, o, rows, cols);
   return check_launch(what);
@@ -343,6 +342,7 @@ int quantize(const void* x, int64_t ldx, int64_t rows, int64_t cols, int64_t blo
   if (block_rows == 1) return launch_groups("sph_quantize_fp8", src, o, rows, cols, stream);
   SPH_REQUIRE(ceil_div(rows, kGroup) <= 65535, SPH_ERR_TOO_LARGE,
               "sph_quantize_fp8: more than 65535 blocks of 128 rows");
+  if (const int rc = fp8::check_grid("sph_quantize_fp8", fp8::groups(cols), 256)) return rc;
   const dim3 grid(static_cast<uint32_t>(fp8::groups(cols)),
                   static_cast<uint32_t>(ceil_div(rows, kGroup)));
   fp8_blocks_kernel<T><<<grid, 256, 0, stream>>>(src, o, rows, cols);
@@ -350,10 +350,12 @@ int quantize(const void* x, int64_t ldx, int64_t rows, int64_t cols, int64_t blo
 }
 
 template <typename T, typename W, int TPR, int VPT>
-void launch_rmsnorm(const NormArgs& p, hipStream_t stream) {
+int launch_rmsnorm(const NormArgs& p, hipStream_t stream) {
   constexpr int NT = TPR > 256 ? TPR : 256;
-  fp8_rmsnorm_kernel<T, W, TPR, VPT>
-      <<<static_cast<uint32_t>(ceil_div(p.rows, NT / TPR)), NT, 0, stream>>>(p);
+  const int64_t wgs = ceil_div(p.rows, NT / TPR);
+  if (const int rc = fp8::check_grid("sph_rmsnorm_fp8", wgs, NT)) return rc;
+  fp8_rmsnorm_kernel<T, W, TPR, VPT><<<static_cast<uint32_t>(wgs), NT, 0, stream>>>(p);
+  return check_launch("sph_rmsnorm_fp8");
 }
 
 template <typename T, typename W>
@@ -361,19 +363,14 @@ int rmsnorm(const NormArgs& p, hipStream_t stream) {
   // One chunk of 8 columns a thread wherever a workgroup holds the row: 8192 x
   // 4096 (with residual) 52.1 us on 512 threads, 54.0 on 256 of two chunks, 68.6
   // on 64 of eight; 1000 x 16384 25.5 by passes, 27.4 on 1024 threads of two.
-  if (p.cols <= 512)
-    launch_rmsnorm<T, W, 64, 1>(p, stream);
-  else if (p.cols <= 1024)
-    launch_rmsnorm<T, W, 64, 2>(p, stream);
-  else if (p.cols <= 2048)
-    launch_rmsnorm<T, W, 256, 1>(p, stream);
-  else if (p.cols <= 4096)
-    launch_rmsnorm<T, W, 512, 1>(p, stream);
-  else if (p.cols <= 8192)
-    launch_rmsnorm<T, W, 1024, 1>(p, stream);
-  else
-    fp8_rmsnorm_long_kernel<T, W><<<static_cast<uint32_t>(p.rows), 1024,
-                                    static_cast<size_t>(fp8::groups(p.cols)) * 4, stream>>>(p);
+  if (p.cols <= 512) return launch_rmsnorm<T, W, 64, 1>(p, stream);
+  if (p.cols <= 1024) return launch_rmsnorm<T, W, 64, 2>(p, stream);
+  if (p.cols <= 2048) return launch_rmsnorm<T, W, 256, 1>(p, stream);
+  if (p.cols <= 4096) return launch_rmsnorm<T, W, 512, 1>(p, stream);
+  if (p.cols <= 8192) return launch_rmsnorm<T, W, 1024, 1>(p, stream);
+  if (const int rc = fp8::check_grid("sph_rmsnorm_fp8", p.rows, 1024)) return rc;
+  fp8_rmsnorm_long_kernel<T, W><<<static_cast<uint32_t>(p.rows), 1024,
+                                  static_cast<size_t>(fp8::groups(p.cols)) * 4, stream>>>(p);
   return check_launch("sph_rmsnorm_fp8");
 }
 
@@ -429,7 +426,6 @@ extern "C" int sph_rmsnorm_fp8(sph_dtype dtype, sph_dtype w_dtype, const void* x
                                int64_t scale_group_stride, sph_stream_t stream) {
   const Out o{static_cast<uint8_t*>(q), ldq, scale, scale_row_stride, scale_group_stride};
   if (const int rc = check_out("sph_rmsnorm_fp8", rows, cols, o)) return rc;
-  SPH_REQUIRE(rows <= kMaxGrid, SPH_ERR_TOO_LARGE, "sph_rmsnorm_fp8: more than 2^31 - 1 rows");
   SPH_REQUIRE(fp8::groups(cols) <= 8192, SPH_ERR_TOO_LARGE,
               "sph_rmsnorm_fp8: rows of more than 1048576 columns");
   SPH_REQUIRE(rows <= 1 || ldx >= cols, SPH_ERR_INVALID_ARG,

@@ -326,6 +326,13 @@ int launch(bool bf16, const Fp8Args& p, const Fp8Plan& plan, hipStream_t st) {
   return bf16 ? launch_dl<bf16_t, 8>(p, st) : launch_dl<half_t, 8>(p, st);
 }
 
+int check_sizes(const char* what, int64_t m, int64_t n, int64_t k) {
+  SPH_REQUIRE(k <= INT32_MAX / 512, SPH_ERR_TOO_LARGE, std::string(what) + ": k above 4194303");
+  SPH_REQUIRE(m <= 16 * 65535 && n <= INT32_MAX && m * n <= (int64_t{1} << 40), SPH_ERR_TOO_LARGE,
+              std::string(what) + ": more than 1048560 rows, 2^31 - 1 columns or 2^40 results");
+  return SPH_OK;
+}
+
 int run(bool bf16, const Fp8Args& p, int64_t max_bytes, hipStream_t st) {
   const Fp8Plan plan = fp8_plan(p.m, p.n, p.k, max_bytes);
   if (plan.m1 == 0 && plan.n1 == 0) return launch(bf16, p, plan, st);
@@ -354,7 +361,7 @@ int run(bool bf16, const Fp8Args& p, int64_t max_bytes, hipStream_t st) {
 using namespace sph;
 
 extern "C" int64_t sph_gemm_fp8_workspace_bytes(int64_t m, int64_t n, int64_t k) {
-  if (m <= 0 || n <= 0 || k <= 0) return 0;
+  if (m <= 0 || n <= 0 || k <= 0 || check_sizes("sph_gemm_fp8", m, n, k) != SPH_OK) return 0;
   return fp8_plan(m, n, k, INT64_MAX).bytes;
 }
 
@@ -362,6 +369,7 @@ extern "C" int sph_gemm_fp8_plan(int64_t m, int64_t n, int64_t k, int64_t worksp
                                  int32_t* plan) {
   SPH_REQUIRE(m > 0 && n > 0 && k > 0 && plan != nullptr, SPH_ERR_INVALID_ARG,
               "sph_gemm_fp8_plan: sizes must be positive");
+  if (const int rc = check_sizes("sph_gemm_fp8_plan", m, n, k)) return rc;
   const Fp8Plan p = fp8_plan(m, n, k, workspace_bytes);
   const Fp8Tile t = p.kernel == Fp8Plan::kStream  ? Fp8Tile{16, 16, 4}
                     : p.kernel == Fp8Plan::kRing ? fp8_ring_tile(p.cfg)
@@ -400,35 +408,32 @@ extern "C" int sph_gemm_fp8(sph_dtype dtype, int64_t m, int64_t n, int64_t k, co
                     (m == 1 || ldx % 16 == 0) && (n == 1 || ldw % 16 == 0),
                 SPH_ERR_UNSUPPORTED, "sph_gemm_fp8: rows of x and w must be 16-byte aligned");
   }
-  SPH_REQUIRE(k <= INT32_MAX / 512 && ldx <= INT32_MAX / 512 && ldw <= INT32_MAX / 512,
-              SPH_ERR_TOO_LARGE, "sph_gemm_fp8: k, ldx or ldw above 4194303");
-  SPH_REQUIRE(m <= INT32_MAX && n <= INT32_MAX, SPH_ERR_TOO_LARGE,
-              "sph_gemm_fp8: m or n above 2^31 - 1");
-  SPH_REQUIRE(m <= 16 * 65535 && m * n <= (int64_t{1} << 40), SPH_ERR_TOO_LARGE,
-              "sph_gemm_fp8: more than 1048560 rows or 2^40 results");
+  if (const int rc = check_sizes("sph_gemm_fp8", m, n, k)) return rc;
+  SPH_REQUIRE(ldx <= INT32_MAX / 512 && ldw <= INT32_MAX / 512, SPH_ERR_TOO_LARGE,
+              "sph_gemm_fp8: ldx or ldw above 4194303");
+  SPH_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, SPH_ERR_UNSUPPORTED,
+              "sph_gemm_fp8: workspace must be 16-byte aligned");
   SPH_REQUIRE(m == 1 || k == 0 || x_scale_row_stride <= (1 << 21), SPH_ERR_TOO_LARGE,
               "sph_gemm_fp8: x_scale_row_stride above 2097152");
-  Fp8Args p{m,
-                  n,
-                  k,
-                  static_cast<const uint8_t*>(x),
-                  ldx,
-                  x_scale,
-                  x_scale_row_stride,
-                  x_scale_group_stride,
-                  static_cast<const uint8_t*>(w),
-                  ldw,
-                  w_scale,
-                  w_scale_row_stride,
-                  w_scale_group_stride,
-                  bias,
-                  d,
-                  ldd,
-                  (reinterpret_cast<uintptr_t>(d) % 128 == 0 && ldd % 64 == 0) ? 1 : 0,
-                  0,
-                  0,
-                  1,
-                  0,
-                  static_cast<float*>(workspace)};
+  Fp8Args p{};
+  p.m = m;
+  p.n = n;
+  p.k = k;
+  p.x = static_cast<const uint8_t*>(x);
+  p.ldx = ldx;
+  p.xs = x_scale;
+  p.xs_row = x_scale_row_stride;
+  p.xs_blk = x_scale_group_stride;
+  p.w = static_cast<const uint8_t*>(w);
+  p.ldw = ldw;
+  p.ws = w_scale;
+  p.ws_row = w_scale_row_stride;
+  p.ws_blk = w_scale_group_stride;
+  p.bias = bias;
+  p.d = d;
+  p.ldd = ldd;
+  p.whole_lines = reinterpret_cast<uintptr_t>(d) % 128 == 0 && ldd % 64 == 0;
+  p.splits = 1;
+  p.part = static_cast<float*>(workspace);
   return run(dtype == SPH_BF16, p, workspace != nullptr ? workspace_bytes : 0, as_stream(stream));
 }

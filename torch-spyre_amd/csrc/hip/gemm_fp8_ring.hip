@@ -215,8 +215,9 @@ template <typename T, int BM, int BN, int NW, int KB, int ST>
 int launch_ring8(Fp8Args& p, hipStream_t st) {
   p.tiles_m = static_cast<int>(ceil_div(p.m, BM));
   p.tiles_n = static_cast<int>(ceil_div(p.n, BN));
-  const unsigned grid = static_cast<unsigned>(p.tiles_m) * p.tiles_n * p.splits;
-  gemm_fp8_ring_kernel<T, BM, BN, NW, KB, ST><<<grid, NW * 64, 0, st>>>(p);
+  const int64_t grid = static_cast<int64_t>(p.tiles_m) * p.tiles_n * p.splits;
+  if (const int rc = fp8::check_grid("sph_gemm_fp8", grid, NW * 64)) return rc;
+  gemm_fp8_ring_kernel<T, BM, BN, NW, KB, ST><<<static_cast<unsigned>(grid), NW * 64, 0, st>>>(p);
   if (p.splits > 1)
     gemm_fp8_reduce<T><<<static_cast<unsigned>(ceil_div(p.m * ceil_div(p.n, 4), 256)), 256, 0, st>>>(p);
   return check_launch("sph_gemm_fp8");

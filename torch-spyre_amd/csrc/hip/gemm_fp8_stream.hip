@@ -81,6 +81,7 @@ __global__ void __launch_bounds__(st8::NW * 64) gemm_fp8_stream_kernel(const Fp8
 }  // namespace
 
 int launch_fp8_stream(bool bf16, const Fp8Args& p, hipStream_t st) {
+  if (const int rc = fp8::check_grid("sph_gemm_fp8", ceil_div(p.n, 16), st8::NW * 64)) return rc;
   const dim3 grid(static_cast<unsigned>(ceil_div(p.n, 16)), static_cast<unsigned>(ceil_div(p.m, 16)));
   if (bf16)
     gemm_fp8_stream_kernel<bf16_t><<<grid, st8::NW * 64, 0, st>>>(p);

@@ -377,6 +377,22 @@ def test_mm_rows_far_apart(m, n, k):
 
 
 @pytest.mark.gpu
+def test_mm_rows_further_apart_than_the_entry_takes():
+    """The last position of 1024 x 4096 codes a sequence (4194304 bytes apart), one
+    row of such a tensor, and W laid out that way."""
+    x, xs, w, ws = whole_operands(4, 300, 4096, 9)
+    base = torch.zeros(4, 1024, 4096, dtype=torch.uint8, device="spyre").view(E4M3)
+    base[:, -1] = x.to("spyre")
+    xs, w, ws = xs.to("spyre"), w.to("spyre"), ws.to("spyre")
+    want = mm64(x, *(t.cpu() for t in (xs, w, ws))).float().half()
+    assert torch.equal(ops.mm_fp8(base[:, -1], xs, w, ws, torch.float16).cpu(), want)
+    assert torch.equal(ops.mm_fp8(base[2:3, -1], xs[2:3], w, ws, torch.float16).cpu(), want[2:3])
+    assert torch.equal(ops.mm_fp8(base[2, -1], xs[2], w, ws, torch.float16).cpu(), want[2])
+    wide = ops.mm_fp8(x.to("spyre"), xs, base[:, -1], xs[:1], torch.float16).cpu()
+    assert torch.equal(wide, mm64(x, xs.cpu(), x, xs[:1].cpu()).float().half())
+
+
+@pytest.mark.gpu
 def test_mm_result_past_32_bits():
     """50000 x 49152 results are 4.9 GB; the last rows against a product of their own."""
     m, n, k = 50000, 49152, 128

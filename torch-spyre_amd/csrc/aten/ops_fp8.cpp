@@ -181,10 +181,14 @@ std::tuple<at::Tensor, at::Tensor> silu_mul_fp8(const at::Tensor& gu) {
 }
 
 // Codes whose rows the product can read in whole chunks: as they lie where the
-// rows begin on 16 bytes, else copied into padded rows.
+// rows begin on 16 bytes and are at most kMaxLd apart (the entry point's limit),
+// else copied into padded rows.
+constexpr int64_t kMaxLd = 4194303;
 Rows code_rows(const at::Tensor& in, const char* op) {
   Rows r = as_rows(in, op);
-  if (r.t.numel() == 0 || (aligned16(r.t) && (r.rows <= 1 || r.ld % 16 == 0))) return r;
+  if (r.rows <= 1) r.ld = r.cols;
+  if (r.t.numel() == 0 || (aligned16(r.t) && (r.rows <= 1 || (r.ld % 16 == 0 && r.ld <= kMaxLd))))
+    return r;
   const int64_t ld = (r.cols + 15) / 16 * 16;
   at::Tensor padded = empty_spyre({r.rows, ld}, kCode, in.device());
   at::Tensor view = padded.narrow(1, 0, r.cols);

@@ -197,6 +197,12 @@ def _rest_of_layer_fp8(a, h, w: dict, cfg: DecoderConfig, next_norm):
     return h, (xq, xs)
 
 
+def _norm_after(i: int, params: dict):
+    """The norm weight that follows layer i: the next layer's or the final one."""
+    layers = params["layers"]
+    return layers[i + 1]["attn_norm"] if i + 1 < len(layers) else params["final_norm"]
+
+
 def _qkv(x, w: dict, cfg: DecoderConfig):
     """Q, K, V projections of x [..., hidden] (of its (codes, scales) for
     8-bit weights): one GEMM over the fused weight when the layer has one."""
@@ -271,10 +277,12 @@ def new_cache(cfg: DecoderConfig, batch: int, max_len: int, device, dtype=torch.
              torch.zeros(vshape, dtype=dtype, device=device)) for _ in range(cfg.n_layers)]
 
 
-def lm_logits(h_last, params: dict, cfg: DecoderConfig):
-    """Final RMSNorm + LM head on h_last [B, hidden] -> logits [B, vocab]."""
+def lm_logits(h_last, params: dict, cfg: DecoderConfig, x=None):
+    """Final RMSNorm + LM head on h_last [B, hidden] -> logits [B, vocab].  x: with
+    8-bit weights, the (codes, scales) of that norm if the last layer formed them."""
     if "lm_head_fp8" in params:
-        x = torch.ops.spyre.rms_norm_fp8(h_last, params["final_norm"], cfg.eps)
+        if x is None:
+            x = torch.ops.spyre.rms_norm_fp8(h_last, params["final_norm"], cfg.eps)
         return torch.ops.spyre.mm_fp8(*x, *params["lm_head_fp8"], h_last.dtype)
     x = F.rms_norm(h_last, (cfg.hidden,), params["final_norm"], cfg.eps)
     return F.linear(x, params["lm_head"])
@@ -291,8 +299,7 @@ def prefill(tokens, params: dict, cos, sin, mask, cache, cfg: DecoderConfig, lay
     # graph serves all layers.
     x = _first_norm(h, layers[0], cfg)
     for i, w in enumerate(layers):
-        nxt = layers[i + 1]["attn_norm"] if i + 1 < len(layers) else params["final_norm"]
-        h, x = layer_fn(h, w, cos, sin, mask, cfg, cache[i], x, nxt)
+        h, x = layer_fn(h, w, cos, sin, mask, cfg, cache[i], x, _norm_after(i, params))
     if "lm_head_fp8" in params:
         xq, xs = x
         return torch.ops.spyre.mm_fp8(xq[:, -1], xs[:, -1], *params["lm_head_fp8"], h.dtype)
@@ -305,8 +312,9 @@ def decode_step(tokens, pos: int, params: dict, cos, sin, cache, cfg: DecoderCon
     B = tokens.shape[0]
     h = F.embedding(tokens, params["embed"]).view(B, 1, cfg.hidden)
     c, s = cos[pos:pos + 1], sin[pos:pos + 1]
+    xn = None  # 8-bit layers: the next norm's (codes, scales), from the same kernel as the sum
     for i, w in enumerate(params["layers"]):
-        x = _first_norm(h, w, cfg)
+        x = xn or _first_norm(h, w, cfg)
         q, k, v = _qkv(x, w, cfg)
         q = apply_rope(q.reshape(B, 1, cfg.n_heads, cfg.head_dim), c, s)
         k = apply_rope(k.reshape(B, 1, cfg.n_kv_heads, cfg.head_dim), c, s)
@@ -316,12 +324,13 @@ def decode_step(tokens, pos: int, params: dict, cos, sin, cache, cfg: DecoderCon
         vc[:, :, :, pos:pos + 1].copy_(v.permute(0, 2, 3, 1))
         kc, vc = kc[:, :, :pos + 1], vc[:, :, :, :pos + 1].transpose(2, 3)
         if "wo_fp8" in w:
-            h, _ = _rest_of_layer_fp8(_attention(q, kc, vc, cfg, None), h, w, cfg, None)
+            h, xn = _rest_of_layer_fp8(_attention(q, kc, vc, cfg, None), h, w, cfg,
+                                       _norm_after(i, params))
             continue
         h = h + F.linear(_attention(q, kc, vc, cfg, None), w["wo"]).view(B, 1, cfg.hidden)
         x = F.rms_norm(h, (cfg.hidden,), w["mlp_norm"], cfg.eps)
         h = h + _mlp(x, w, cfg)
-    return lm_logits(h[:, 0], params, cfg)
+    return lm_logits(h[:, 0], params, cfg, xn and [t[:, 0] for t in xn])
 
 
 def decode_step_static(tokens, pos, params: dict, cos, sin, cache, cfg: DecoderConfig,
@@ -343,8 +352,9 @@ def decode_step_static(tokens, pos, params: dict, cos, sin, cache, cfg: DecoderC
     c, s = cos.index_select(0, pos), sin.index_select(0, pos)
     keys = torch.arange(L, device=tokens.device)
     mask = torch.where(keys <= pos, 0.0, float("-inf")).to(h.dtype)
+    xn = None  # as in decode_step
     for i, w in enumerate(params["layers"]):
-        x = _first_norm(h, w, cfg)
+        x = xn or _first_norm(h, w, cfg)
         fp8 = "wqkv_fp8" in w
         if fused_attention and (fp8 or "wqkv" in w) and cfg.head_dim == 128:
             kc, vc = cache[i]
@@ -356,7 +366,7 @@ def decode_step_static(tokens, pos, params: dict, cos, sin, cache, cfg: DecoderC
                                                  cfg.n_kv_heads, 1.0 / math.sqrt(cfg.head_dim),
                                                  True)
             if fp8:
-                h, _ = _rest_of_layer_fp8(a, h, w, cfg, None)
+                h, xn = _rest_of_layer_fp8(a, h, w, cfg, _norm_after(i, params))
                 continue
             h = h + F.linear(a, w["wo"]).view(B, 1, cfg.hidden)
             x = F.rms_norm(h, (cfg.hidden,), w["mlp_norm"], cfg.eps)
@@ -370,14 +380,14 @@ def decode_step_static(tokens, pos, params: dict, cos, sin, cache, cfg: DecoderC
         kc.index_copy_(2, pos, k.transpose(1, 2))
         vc.index_copy_(3, pos, v.permute(0, 2, 3, 1))
         if fp8:
-            h, _ = _rest_of_layer_fp8(_attention(q, kc, vc.transpose(2, 3), cfg, mask), h, w, cfg,
-                                      None)
+            h, xn = _rest_of_layer_fp8(_attention(q, kc, vc.transpose(2, 3), cfg, mask), h, w, cfg,
+                                       _norm_after(i, params))
             continue
         h = h + F.linear(_attention(q, kc, vc.transpose(2, 3), cfg, mask),
                          w["wo"]).view(B, 1, cfg.hidden)
         x = F.rms_norm(h, (cfg.hidden,), w["mlp_norm"], cfg.eps)
         h = h + _mlp(x, w, cfg)
-    return lm_logits(h[:, 0], params, cfg)
+    return lm_logits(h[:, 0], params, cfg, xn and [t[:, 0] for t in xn])
 
 
 def generate(prompt, params: dict, cfg: DecoderConfig, steps: int, device, layer_fn=None,

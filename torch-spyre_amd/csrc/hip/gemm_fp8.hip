@@ -276,8 +276,13 @@ double tiles_us(int c, int64_t tiles, int64_t k) {
 // 4 blocks a wave is the whole product: 512 workgroups and K of 4096 at most,
 // above 16 rows (W read more than once, from the caches) half of their product.
 //     1 x 6144 x 4096 8.0 (ring 8.8), 16 x 4096 x 4096 6.6 (8.2), 16 x 8192 x 4096
-//     10.3 (10.3), 16 x 12288 x 4096 14.8 (12.1), 1 x 4096 x 12800 12.8 (12.4),
-//     64 x 2048 x 2048 5.8 (6.9), 512 x 256 x 4096 10.2 (8.2)
+//     10.3 (10.3), 16 x 12288 x 4096 14.8 (12.1), 64 x 2048 x 2048 5.8 (6.9), 512 x
+//     256 x 4096 10.2 (8.2)
+//   Up to 8 rows also K to 12800, where 97 to 256 workgroups hold W: no slower in a
+// loop (W from HBM, 4 x 4096 x 8192 10.6 (11.2), 4 x 4096 x 12800 16.1 (14.2 to
+// 15.9), but 16 x 4096 x 8192 12.6 (11.4) and 4 x 1024 x 8192 8.7 (7.9)), and a
+// captured decode step saves the second launch of K slices (8 layers of 4096 x 12800
+// among others, 4 rows: 741 and 759 us a step).
 //   Others the kernel whose fitted time is the least:
 //     16 x 25600 x 4096 ring 21.7 (streamed 30), 333 x 4096 x 12800 ring 34.5 (256-
 //     row tiles 117), 2048 x 6144 x 4096 192-row tiles 47.3 (256-row 50.5, ring
@@ -292,7 +297,8 @@ double tiles_us(int c, int64_t tiles, int64_t k) {
 Fp8Plan fp8_plan(int64_t m, int64_t n, int64_t k, int64_t max_bytes, bool whole = false) {
   Fp8Plan best;
   const int64_t wgs = ceil_div(n, 16) * ceil_div(m, 16);
-  if (k < kGroup || (wgs <= 512 && k <= 32 * kGroup && wgs * k <= (m <= 16 ? 1 << 21 : 1 << 20)))
+  if (k < kGroup || (m <= 8 && wgs > 96 && wgs <= 256 && k <= 100 * kGroup) ||
+      (wgs <= 512 && k <= 32 * kGroup && wgs * k <= (m <= 16 ? 1 << 21 : 1 << 20)))
     return best;
   best = fp8_ring_plan(m, n, k, max_bytes);
   if (k < 2 * kGroup || k % kGroup != 0) return best;

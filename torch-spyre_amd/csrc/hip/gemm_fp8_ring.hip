@@ -227,20 +227,20 @@ int launch_ring8(Fp8Args& p, hipStream_t st) {
 // in flight; us of a round of workgroups beside its blocks of K, of the launch,
 // and per block of K with 1, 2 or 3 workgroups on the CU; us of the reduce's
 // launch and TB/s of its sums; TB/s of the tiles' traffic from the caches and of
-// the operands from memory.  Fitted to 7300 timings of 1 to 2600 rows by 256 to
-// 49155 columns, K 256 to 12800, 1 to 16 slices (rms error 7 to 13 %; the plan
-// that the fitted times choose is 2 % slower than the fastest of a product on
-// average, 16 % at most: 333 x 25600 x 4096), the 128-row tiles' traffic then set to
-// that of products of several rounds (777 x 6144 to 4000 x 6144).
+// the operands from memory.  Fitted to 7300 timings of 1 to 4400 rows by 256 to
+// 49155 columns, K 256 to 25600, 1 to 16 slices, the weights of most of them read
+// from HBM as a model's layers are (rms error 6 to 8 %; the plan that the fitted
+// times choose is 2 % slower than the fastest of a product on average, 25 % at
+// most: 477 x 1895 x 1664).
 struct RingCfg {
   int bm, bn, kb, per_cu, fly;
   double round, launch, blk[3], reduce, sums, traffic, mem;
 };
 constexpr RingCfg kRing[] = {
-    {32, 64, 2, 3, 2, 2.15, 1.0, {0.264, 0.344, 0.439}, 2.44, 5.60, 19.1, 5.24},
-    {64, 128, 1, 2, 2, 0.51, 2.4, {0.428, 0.687, 0}, 2.64, 5.10, 16.7, 5.86},
-    {128, 128, 1, 2, 1, 2.07, 1.42, {0.604, 0.835, 0}, 2.59, 5.12, 11.8, 4.97},
-    {128, 128, 1, 1, 2, 1.54, 2.02, {0.592, 0, 0}, 2.54, 4.96, 11.4, 5.55}};
+    {32, 64, 2, 3, 2, 0.32, 2.2, {0.378, 0.511, 0.53}, 2.9, 4.1, 33.0, 5.14},
+    {64, 128, 1, 2, 2, 0.1, 3.36, {0.439, 0.818, 0}, 2.45, 5.3, 15.4, 5.5},
+    {128, 128, 1, 2, 1, 2.1, 1.8, {0.852, 1.11, 0}, 2.5, 6.1, 15.2, 5.0},
+    {128, 128, 1, 1, 2, 2.2, 2.2, {0.578, 0, 0}, 2.4, 5.6, 10.9, 5.5}};
 constexpr int kRingCfgs = sizeof(kRing) / sizeof(kRing[0]);
 
 template <typename T>
@@ -263,6 +263,8 @@ Fp8Plan fp8_ring_plan(int64_t m, int64_t n, int64_t k, int64_t max_bytes) {
   const double mem_mb = static_cast<double>(m * k + n * k + 2 * m * n) * 1e-6;
   for (int c = 0; c < kRingCfgs; ++c) {
     const RingCfg& f = kRing[c];
+    // (up to 32 rows no 128-row tiles: 4 x 25600 x 4096 27.8 us, 26.9 in 64-row tiles)
+    if (m <= 32 && f.bm > 64) continue;
     const int64_t tiles = ceil_div(m, f.bm) * ceil_div(n, f.bn), slots = kCUs * f.per_cu;
     for (int s = 1; s <= 16; ++s) {
       // at least 2 blocks a slice, no more slices than two rounds hold
@@ -273,14 +275,18 @@ Fp8Plan fp8_ring_plan(int64_t m, int64_t n, int64_t k, int64_t max_bytes) {
       if (bytes > max_bytes) continue;
       const int64_t wgs = tiles * s, full = wgs / slots, rest = wgs % slots;
       const double blocks = static_cast<double>(ceil_div(slice, f.kb) * f.kb);
-      double us = static_cast<double>(full) * (f.round + blocks * f.blk[f.per_cu - 1]);
-      if (rest > 0) us += 0.7 * f.round + blocks * f.blk[(rest - 1) / kCUs];
-      // no faster than what is in flight arrives (1.3 us), the tiles' traffic, or
-      // the operands from memory
+      // a round is no faster than the caches serve its tiles, the whole no faster
+      // than what is in flight arrives (1.3 us) and the operands come from memory
       const double block_bytes = static_cast<double>((f.bm + f.bn) * kGroup);
+      const auto served = [&](int64_t w) {
+        return static_cast<double>(w * slice) * block_bytes / (f.traffic * 1e6);
+      };
+      double us = static_cast<double>(full) *
+                  std::max(f.round + blocks * f.blk[f.per_cu - 1], served(slots));
+      if (rest > 0)
+        us += std::max(0.7 * f.round + blocks * f.blk[(rest - 1) / kCUs], served(rest));
       const double fly = static_cast<double>(std::min(wgs, slots) * f.fly) * block_bytes;
-      us = std::max({us, static_cast<double>((m + n) * k) / fly * 1.3, mem_mb / f.mem,
-                     static_cast<double>(wgs * slice) * block_bytes / (f.traffic * 1e6)});
+      us = std::max({us, static_cast<double>((m + n) * k) / fly * 1.3, mem_mb / f.mem});
       us += f.launch;
       if (s > 1) us += f.reduce + 2.0 * static_cast<double>(bytes) / (f.sums * 1e6);
       if (us < best.us) {

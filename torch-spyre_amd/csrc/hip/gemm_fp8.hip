@@ -36,6 +36,13 @@ namespace {
 //   * A block's scales ride in its stage: waves 0 to 3 fetch X's, 4 and 5 those
 //     of W's first 128 rows (of a 192-row tile: its first block), 6 and 7 the
 //     next.
+//
+// 4096 x 25600 x 4096: 417 to 427 us, 2010 to 2060 TFLOP/s.  Bound by the chip's
+// power and the tiles' way through LDS together: the clock stands at 2.05 GHz
+// (2.35 without the loads), the matrix cores are busy 53 % of it, and of the time
+// 90 us go with the direct loads and 48 with the stores (327 and 369 us without);
+// matrix instructions and scaling alone reach 3600 TFLOP/s.  X's fragments
+// straight from memory to registers, past LDS: 645 us (192-row tiles, 448 as here).
 // ---------------------------------------------------------------------------
 namespace dl8 {
 constexpr int TM = 4, LAG = 2, WN = 2, WM = 4, NW = 8, NT = 512, BM = 256;

@@ -15,6 +15,11 @@
 // barrier, LDS, MFMA, FMA) whatever its size, so the small tiles take two blocks
 // a step (256 x 4096 x 4096 in 32 x 64 tiles 12.1 us, 15.1 with one) and the
 // larger ones 8 waves (777 x 6144 x 4096 in 128 x 128 tiles 32.0 us, 39.8 on 4).
+// Few rows are bound by reading W (24 x 49155 x 4096 43 us, 39.7 at copy rate), the
+// others by what is in flight into LDS (333 x 4096 x 12800 34.5 us: 9.5 TB/s from
+// the caches, the matrix cores busy 21 %).  Asking for W's lines three or six
+// steps ahead made all of them slower (44.8 and 43.5 us in the run whose time
+// without was 38.6), 192 x 128 and 256 x 128 tiles no faster (35.2, 40.7).
 #include <algorithm>
 
 #include "gemm_fp8.h"

@@ -6,6 +6,8 @@ into an asm string.  The loads to LDS take their LDS address from M0 and their
 buffer resource and offset from scalar registers:
 
   * scalar write of M0, then a load to LDS: 1 wait state;
+  * vector write of a scalar register (v_readfirstlane_b32), then a load that
+    reads it: 5 wait states.
 
 Every instruction between the two counts as one wait state, s_nop N as N + 1;
 all ways that lead to a load are followed backwards, across branches.
@@ -91,6 +93,17 @@ def early_m0(body):
             for y in before(body, pred, i, 1) if y.op.startswith("s_") and y.args[:1] == ["m0"]]
 
 
+def early_scalars(body):
+    """Loads to LDS that read a scalar register which a vector instruction has
+    just written."""
+    pred = predecessors(body)
+    return [(y.text, x.text) for i, x in enumerate(body) if is_load(x)
+            for y in before(body, pred, i, 5) if y.op.startswith("v_")
+            # (carry and condition results stand second)
+            and set().union(*map(registers, y.args[:2] if "_co_" in y.op else y.args[:1]))
+            & set().union(*map(registers, x.args))]
+
+
 def listing(*ops):
     return ["0000 <kernel>:"] + [f"\t{op}   // {4 * i:012X}: 00000000" for i, op in enumerate(ops)]
 
@@ -108,6 +121,10 @@ def test_scan_finds_missing_wait_states():
     loop[1] = loop[1] + " <kernel+0x8>"
     loop[5] = loop[5] + " <kernel+0x8>"
     assert not early_m0(*bodies(loop))  # the branch is a wait state
+    late = ("v_readfirstlane_b32 s6, v1", "s_mov_b32 m0, s8")
+    for nop, found in ((0, 1), (2, 1), (3, 0)):
+        assert len(early_scalars(*bodies(listing(*late, f"s_nop {nop}", load)))) == found
+    assert not early_scalars(*bodies(listing("v_readfirstlane_b32 s8, v1", "s_nop 0", load)))
     assert not bodies(listing("buffer_load_dwordx4 v[0:3], v4, s[4:7], 0 offen", "s_endpgm"))
 
 
@@ -131,4 +148,9 @@ def kernels(tmp_path_factory):
 
 def test_m0_is_written_a_wait_state_ahead(kernels):
     bad = [(name, *pair) for name, body in kernels for pair in early_m0(body)]
+    assert not bad, f"{len(bad)} loads, first: {bad[0]}"
+
+
+def test_scalars_are_written_five_wait_states_ahead(kernels):
+    bad = [(name, *pair) for name, body in kernels for pair in early_scalars(body)]
     assert not bad, f"{len(bad)} loads, first: {bad[0]}"

@@ -150,7 +150,8 @@ __device__ inline i32x4 buffer_rsrc(const void* base, uint32_t bytes) {
 // 16 bytes per lane from rsrc[voff + soff] into LDS at lds_addr + 16 * lane
 // (inline asm: the compiler would otherwise wait for it before every LDS
 // read; completion is awaited explicitly).  The s_nop is the wait state that gfx9
-// wants between a scalar write of M0 and a load to LDS.
+// wants between a scalar write of M0 and a load to LDS; resource and offset are
+// written further ahead.
 __device__ inline void dma16(i32x4 rsrc, uint32_t lds_addr, uint32_t voff, uint32_t soff) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                :

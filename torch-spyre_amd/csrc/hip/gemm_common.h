@@ -65,8 +65,11 @@ __device__ inline i32x4 buffer_rsrc(const void* base, uint32_t bytes) {
 }
 
 // 16 bytes per lane from rsrc[voff + soff] into LDS at lds_addr + 16 * lane.
-// gfx9 wants one wait state between a scalar write of M0 and a load to LDS; the
-// compiler puts none into an asm string.
+// gfx9 wants one wait state between a scalar write of M0 and a load to LDS, and five
+// between a vector write of rsrc or soff (readfirstlane) and the load; the compiler
+// puts none into an asm string.  Resources and offsets are set up well ahead here,
+// which the host tests check in the machine code: waiting for five at every load
+// cost 1 to 2 % (8192 x 4096 x 12800 651 and 662 us).
 __device__ inline void dma16(i32x4 rsrc, uint32_t lds_addr, uint32_t voff, uint32_t soff) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                :

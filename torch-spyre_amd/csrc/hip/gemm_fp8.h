@@ -63,10 +63,11 @@ __device__ inline f32x4 mfma_block(i32x8 a, i32x8 b) {
                                                           0, 0, 0);
 }
 
-// 4 bytes per lane from rsrc[voff] into LDS at lds_addr + 4 * lane (waits as in
-// dma16).
+// 4 bytes per lane from rsrc[voff] into LDS at lds_addr + 4 * lane, with the five
+// wait states that a resource just written by a vector instruction takes: its
+// base moves with every block.
 __device__ inline void dma4(i32x4 rsrc, uint32_t lds_addr, uint32_t voff) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dword %1, %2, 0 offen lds"
                :
                : "s"(lds_addr), "v"(voff), "s"(rsrc)
                : "memory", "m0");

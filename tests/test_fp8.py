@@ -583,3 +583,58 @@ def test_fakes_match_the_formulas():
         assert real == fake
     assert math.isclose(2.0 ** -100 / 448, ops.quantize_fp8(torch.zeros(1, 8))[1].item(),
                         rel_tol=2.0 ** -24)  # half an fp32 step
+
+
+# ---- derivatives ---------------------------------------------------------------
+
+def _float_calls(device):
+    """Every operator as a function of one tensor that a derivative could be
+    taken by, and that tensor."""
+    f16 = torch.float16
+    x = rand((4, 256), 30).to(device)
+    q, s = ops.quantize_fp8(x)
+    w, ws = ops.quantize_fp8(rand((130, 256), 31).to(device), 128)
+    return {
+        "quantize": (lambda t: ops.quantize_fp8(t)[1], x),
+        "rms_norm": (lambda t: ops.rms_norm_fp8(t, None, 1e-5)[1], x),
+        "rms_norm weight": (lambda t: ops.rms_norm_fp8(x, t, 1e-5)[1], x[0]),
+        "add_rms_norm": (lambda t: ops.add_rms_norm_fp8(x, t, None, 1e-5)[2], x),
+        "silu": (lambda t: ops.silu_mul_fp8(t)[1], x),
+        "mm x_scale": (lambda t: ops.mm_fp8(q, t, w, ws, f16), s),
+        "mm w_scale": (lambda t: ops.mm_fp8(q, s, w, t, f16), ws),
+        "mm bias": (lambda t: ops.mm_fp8(q, s, w, ws, f16, t), rand((130,), 32, 1.0, f16).to(device)),
+    }
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_derivatives_are_refused(device):
+    """A leaf that requires a gradient and a dual tensor; the same calls without
+    either run, also while a dual level is open."""
+    from torch.autograd import forward_ad
+
+    for name, (call, t) in _float_calls(device).items():
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call(t.detach().clone().requires_grad_())
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(t.detach(), torch.ones_like(t))
+            with pytest.raises(RuntimeError, match="without tangents"):
+                call(dual)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="without tangents"):
+                call(dual)
+            call(t)
+        with torch.no_grad():
+            call(t.detach().clone().requires_grad_())
+
+
+def test_transforms_and_compile_refuse_derivatives():
+    for name, (call, t) in _float_calls("cpu").items():
+        with pytest.raises(RuntimeError, match="no gradient"):
+            torch.func.vjp(call, t)
+        with pytest.raises(RuntimeError, match="no gradient"):
+            torch.func.jvp(call, (t,), (torch.ones_like(t),))
+        leaf = t.detach().clone().requires_grad_()
+        run = torch.compile(lambda v, call=call: call(v) * 2, backend="aot_eager")
+        with pytest.raises(RuntimeError, match="no gradient"):
+            run(leaf)
+        with torch.no_grad():
+            assert torch.equal(run(leaf), call(t) * 2)

@@ -253,15 +253,18 @@ at::Tensor mm_fp8(const at::Tensor& x_in, const at::Tensor& x_scale, const at::T
   return out;
 }
 
-// Rounding to codes has no gradient: a call that would have to record one is
-// refused instead of returning tensors that silently cut the graph.
+// Rounding to codes has no gradient: a call that would have to record one, or to
+// carry a tangent on, is refused instead of returning tensors that silently cut
+// the graph.
 void refuse_gradients(const c10::OperatorHandle& op, c10::DispatchKeySet ks,
                       torch::jit::Stack* stack) {
-  if (at::GradMode::is_enabled()) {
-    const size_t nargs = op.schema().arguments().size();
-    for (const auto& v : torch::jit::last(*stack, nargs))
-      TORCH_CHECK(!v.isTensor() || !v.toTensor().defined() || !v.toTensor().requires_grad(),
-                  op.schema().name(), " has no gradient: call it under torch.no_grad()");
+  const bool grad = at::GradMode::is_enabled();
+  for (const auto& v : torch::jit::last(*stack, op.schema().arguments().size())) {
+    if (!v.isTensor() || !v.toTensor().defined()) continue;
+    TORCH_CHECK(!(grad && v.toTensor().requires_grad()), op.schema().name(),
+                " has no gradient: call it under torch.no_grad()");
+    TORCH_CHECK(!v.toTensor()._fw_grad(/*level=*/0).defined(), op.schema().name(),
+                " has no gradient: call it without tangents");
   }
   at::AutoDispatchBelowADInplaceOrView below;
   op.redispatchBoxed(ks & c10::after_autograd_keyset, stack);

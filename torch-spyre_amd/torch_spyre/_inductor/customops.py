@@ -39,6 +39,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import Unsupported
 from .stickify import (SpyreDCI, StickFormat, elems_per_stick, spyre_reduction_result_shape,
@@ -448,6 +449,32 @@ for _name, _schema in _FP8_SCHEMAS.items():
     torch.library.define(f"spyre::{_name}", _schema)
 
 
+def _fp8_tangent(t) -> bool:
+    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None
+
+
+def _fp8_refuse_gradients(op):
+    """Rounding to codes has no gradient: a call that would have to record one,
+    or to carry a tangent on, is refused, also while a transform or compile
+    traces it.  (The spyre device has a kernel of its own for this, in C++.)"""
+    def kernel(keyset, *args, **kwargs):
+        for t in (*args, *kwargs.values()):
+            if isinstance(t, torch.Tensor):
+                _fp8_check(not (torch.is_grad_enabled() and t.requires_grad),
+                           f"{op.name()} has no gradient: call it under torch.no_grad()")
+                _fp8_check(not _fp8_tangent(t),
+                           f"{op.name()} has no gradient: call it without tangents")
+        with torch._C._AutoDispatchBelowAutograd():
+            return op.redispatch(keyset & torch._C._after_autograd_keyset, *args, **kwargs)
+    return kernel
+
+
+_fp8_lib = torch.library.Library("spyre", "FRAGMENT")
+for _name in _FP8_SCHEMAS:
+    _fp8_lib.impl(_name, _fp8_refuse_gradients(getattr(torch.ops.spyre, _name).default),
+                  "Autograd", with_keyset=True)
+
+
 def _fp8_check(cond: bool, message: str) -> None:
     if not cond:
         raise RuntimeError(message)
@@ -502,12 +529,6 @@ def _fp8_fill(x: torch.Tensor, v: torch.Tensor, shape, row_factor=None):
     return q, s
 
 
-def _fp8_no_grad(name: str, *tensors) -> None:
-    _fp8_check(not (torch.is_grad_enabled() and
-                    any(t is not None and t.requires_grad for t in tensors)),
-               f"spyre::{name} has no gradient: call it under torch.no_grad()")
-
-
 def _quantize_fp8_check(x, block_rows):
     _fp8_check(x.dtype in (torch.float16, torch.bfloat16, torch.float32),
                f"quantize_fp8: x must be fp16, bf16 or fp32, got {x.dtype}")
@@ -527,7 +548,6 @@ def quantize_fp8(x: torch.Tensor, block_rows: int = 1):
     128)] or [ceil(N / 128), ceil(K / 128)]).  A group that holds an infinity
     or a NaN has it as its scale."""
     _quantize_fp8_check(x, block_rows)
-    _fp8_no_grad("quantize_fp8", x)
     if block_rows == 1:
         return _fp8_fill(x, x.reshape(-1, x.shape[-1]).float() if x.numel() else x, x.shape)
     q, s = _fp8_blocks_empty(x)
@@ -568,7 +588,6 @@ def rms_norm_fp8(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float):
     without rounding it to x's type in between.  The codes are those of x *
     weight: the row's 1 / rms is a factor of its scales alone."""
     _rms_norm_fp8_check("rms_norm_fp8", x, None, weight)
-    _fp8_no_grad("rms_norm_fp8", x, weight)
     return _rms_norm_fp8(x, weight, eps)
 
 
@@ -584,7 +603,6 @@ def add_rms_norm_fp8(x: torch.Tensor, residual: torch.Tensor, weight: Optional[t
     """(codes, scales, h) with h = x + residual in x's type, normalised as
     rms_norm_fp8 does."""
     _rms_norm_fp8_check("add_rms_norm_fp8", x, residual, weight)
-    _fp8_no_grad("add_rms_norm_fp8", x, residual, weight)
     h = (x + residual).contiguous()
     return (*_rms_norm_fp8(h, weight, eps), h)
 
@@ -608,7 +626,6 @@ def silu_mul_fp8(gate_up: torch.Tensor):
     """(codes, scales) of silu(gate_up[..., :n]) * gate_up[..., n:] for
     gate_up [..., 2n], formed in fp32."""
     _silu_mul_fp8_check(gate_up)
-    _fp8_no_grad("silu_mul_fp8", gate_up)
     n = gate_up.shape[-1] // 2
     shape = list(gate_up.shape[:-1]) + [n]
     gu = gate_up.reshape(-1, 2 * n).float() if gate_up.numel() else gate_up.float()
@@ -651,7 +668,6 @@ def mm_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: tor
     w [N, K] quantised in blocks of 128 x 128.  The products of two scales have
     to be finite."""
     _mm_fp8_check(x, x_scale, w, w_scale, dtype, bias)
-    _fp8_no_grad("mm_fp8", x_scale, w_scale, bias)
     k = w.shape[1]
     if x.numel() == 0 or w.numel() == 0:
         y = x_scale.new_zeros(list(x.shape[:-1]) + [w.shape[0]])

@@ -304,6 +304,38 @@ def test_mm_whole_numbers(m, n, k):
     assert torch.equal(y, (want + bias.double()).float().half())
 
 
+# Products on 256 rows of X by 256 or 192 of W with several tiles per workgroup, so
+# that the loads of one tile run on behind the stores of the one before: rows of
+# the result on cache lines (streaming stores) and off them, whole and ragged
+# tiles, 192-row tiles that begin in the middle of a block of W.
+TILE_SHAPES = [(3428, 6144, 1024), (3000, 12288, 896), (1501, 15509, 1024), (8192, 6144, 512),
+               (2600, 16384, 512), (2000, 13000, 640)]
+
+
+def test_tile_shapes_cover_both_stores_and_second_tiles():
+    found = set()
+    for m, n, k in TILE_SHAPES:
+        (kernel, tm, tn, _), _, split = plan(m, n, k)
+        assert kernel == "tiles" and not split and -(-m // tm) * -(-n // tn) > 256
+        found.add((tn, n % 64 == 0))
+    assert found == {(256, True), (256, False), (192, True), (192, False)}
+    assert any(-(-m // 256) * -(-n // 192) > 512 for m, n, k in TILE_SHAPES
+               if plan(m, n, k)[0][2] == 192)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", TILE_SHAPES)
+def test_mm_several_tiles_per_workgroup(m, n, k):
+    x, xs, w, ws = whole_operands(m, n, k, m + n + k)
+    want = mm64(x, xs, w, ws)
+    bias = torch.randint(-8, 9, (n,), generator=torch.Generator().manual_seed(6)).to(torch.bfloat16)
+    dev = [t.to("spyre") for t in (x, xs.t().contiguous().t(), w, ws)]
+    for dtype, b in ((torch.bfloat16, bias), (torch.float16, None), (torch.float16, bias.half())):
+        y = ops.mm_fp8(*dev, dtype, None if b is None else b.to("spyre")).cpu()
+        y64 = want if b is None else want + b.double()
+        assert torch.equal(y, y64.float().to(dtype)), (y.double() - y64).abs().max()
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("m,n,k", [(1, 640, 4096), (5, 130, 300), (24, 257, 1000), (130, 384, 640),

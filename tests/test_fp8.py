@@ -670,3 +670,48 @@ def test_transforms_and_compile_refuse_derivatives():
             run(leaf)
         with torch.no_grad():
             assert torch.equal(run(leaf), call(t) * 2)
+
+
+# ---- devices, layouts and fakes ------------------------------------------------
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("shape", [(1, 130), (1, 15), (1, 256), (3, 130), (2, 3, 40)])
+def test_results_stay_on_the_device_in_padded_rows(shape, device):
+    x, w = rand(shape, 33).to(device), rand(shape[-1:], 34).to(device)
+    gu = rand((*shape[:-1], 2 * shape[-1]), 35).to(device)
+    for q, s, *h in (ops.quantize_fp8(x), ops.rms_norm_fp8(x, w, 1e-5),
+                     ops.add_rms_norm_fp8(x, x, w, 1e-5), ops.silu_mul_fp8(gu)):
+        pitch = -(-shape[-1] // 16) * 16
+        rows = math.prod(shape[:-1])
+        strides = (shape[1] * pitch, pitch, 1) if len(shape) == 3 else (pitch, 1)
+        assert all(t.device.type == device for t in (q, s, *h))
+        assert q.stride() == strides
+        # (of one row's scales the row stride says nothing)
+        assert s.stride()[-2:] == (1, rows) or rows == 1 and s.stride(-1) == 1
+        assert q.shape == shape and s.shape == (*shape[:-1], -(-shape[-1] // 128))
+    if len(shape) == 2:
+        q, s = ops.quantize_fp8(x, 128)
+        assert q.device.type == s.device.type == device and q.stride() == (pitch, 1)
+        assert s.is_contiguous() and s.shape == (1, -(-shape[1] // 128))
+
+
+def test_fakes_of_products_and_weights_match():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    def meta(*tensors):
+        return [(t.shape, t.dtype, t.stride(), t.device) for t in tensors]
+
+    for m, n, k in ((5, 130, 384), (1, 7, 100), (0, 16, 64), (4, 3, 0)):
+        x, w = rand((m, k), 36), rand((n, k), 37)
+        lead = (1, m, k)
+        bias = rand((n,), 38, 1.0, torch.float16)
+
+        def results(x, w, bias):
+            q, s = ops.quantize_fp8(x.view(lead))
+            wq, ws = ops.quantize_fp8(w, 128)
+            y = ops.mm_fp8(q, s, wq, ws, torch.float16, bias)
+            return meta(q, s, wq, ws, y, ops.mm_fp8(q[0], s[0], wq, ws, torch.bfloat16))
+
+        real = results(x, w, bias)
+        with FakeTensorMode() as mode:
+            assert results(*(mode.from_tensor(t) for t in (x, w, bias))) == real

@@ -304,6 +304,36 @@ def test_mm_whole_numbers(m, n, k):
     assert torch.equal(y, (want + bias.double()).float().half())
 
 
+# Streamed products of more than one pass of 32 blocks of K, whole and partial last
+# blocks, few rows and few columns.
+STREAMED = [(1, 2048, 5376), (4, 4096, 12800), (8, 4096, 14336), (5, 3001, 9001), (1, 245, 4192),
+            (1, 9152, 1664), (3226, 16, 4210)]
+
+
+def test_streaming_follows_its_fitted_time():
+    for s in STREAMED:
+        assert plan(*s)[0][0] == "stream", s
+    for m in (1, 2, 4, 8):  # a down projection of the decoder, and longer rows
+        for k in (4096, 8192, 12800, 13312, 14336, 16384):
+            assert plan(m, 4096, k)[0][0] == "stream", (m, k)
+        # a 257th workgroup begins a second round
+        assert plan(m, 4097, 12800)[0][0] == "ring", m
+    for m in (16, 24, 32):  # bytes of X beside W's
+        assert plan(m, 4096, 12800)[0][0] == "ring" and plan(m, 4096, 12800)[1] > 1, m
+    assert plan(1, 6144, 4096)[0][0] == plan(1, 4096, 4096)[0][0] == "stream"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", STREAMED)
+def test_mm_streamed_over_long_rows(m, n, k):
+    x, xs, w, ws = whole_operands(m, n, k, m + n + k)
+    bias = torch.randint(-8, 9, (n,), generator=torch.Generator().manual_seed(7)).half()
+    want = mm64(x, xs, w, ws) + bias.double()
+    dev = [t.to("spyre") for t in (x, xs.t().contiguous().t(), w, ws)]
+    y = ops.mm_fp8(*dev, torch.float16, bias.to("spyre")).cpu()
+    assert torch.equal(y, want.float().half()), (y.double() - want).abs().max()
+
+
 # Products on 256 rows of X by 256 or 192 of W with several tiles per workgroup, so
 # that the loads of one tile run on behind the stores of the one before: rows of
 # the result on cache lines (streaming stores) and off them, whole and ragged

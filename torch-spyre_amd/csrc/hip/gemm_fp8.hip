@@ -278,6 +278,18 @@ double tiles_us(int c, int64_t tiles, int64_t k) {
   return us;
 }
 
+// us of a streamed product: the launch, what a workgroup takes beside its bytes,
+// and the bytes of the fullest CU (W's from memory, X's from the caches).  Fitted to
+// 1246 timings of 1 to 70 rows by 64 to 40000 columns, K 128 to 26000, each with W
+// from HBM, in which it comes within 1.6 of the fastest kernel (rms error 8 %).
+double stream_us(int64_t m, int64_t n, int64_t k) {
+  constexpr double kLaunch = 2.33, kWorkgroup = 0.0013, kCuKB = 22.8, kX = 0.47;
+  const int64_t wgs = ceil_div(n, 16) * ceil_div(m, 16);
+  const double rows = 16 + kX * static_cast<double>(std::min<int64_t>(m, 16));
+  return kLaunch + kWorkgroup * static_cast<double>(wgs) +
+         static_cast<double>(ceil_div(wgs, kTileCUs) * k) * rows * 1e-3 / kCuKB;
+}
+
 // The kernel of a product (one MI355X, operands of three products in turn, us).
 //   Streamed rows, where one pass of workgroups over 16 rows each of X and W and
 // 4 blocks a wave is the whole product: 512 workgroups and K of 4096 at most,
@@ -285,11 +297,11 @@ double tiles_us(int c, int64_t tiles, int64_t k) {
 //     1 x 6144 x 4096 8.0 (ring 8.8), 16 x 4096 x 4096 6.6 (8.2), 16 x 8192 x 4096
 //     10.3 (10.3), 16 x 12288 x 4096 14.8 (12.1), 64 x 2048 x 2048 5.8 (6.9), 512 x
 //     256 x 4096 10.2 (8.2)
-//   Up to 8 rows also K to 12800, where 97 to 256 workgroups hold W: no slower in a
-// loop (W from HBM, 4 x 4096 x 8192 10.6 (11.2), 4 x 4096 x 12800 16.1 (14.2 to
-// 15.9), but 16 x 4096 x 8192 12.6 (11.4) and 4 x 1024 x 8192 8.7 (7.9)), and a
-// captured decode step saves the second launch of K slices (8 layers of 4096 x 12800
-// among others, 4 rows: 741 and 759 us a step).
+//   Elsewhere too where its fitted time is 5 % below the ring's: of 1494 products of
+// up to 70 rows 67 stream by this, 0.83 to 1.07 (on average 0.89) of the time of
+// the kernel they had by the limits above and K to 12800 for up to 8 rows.  W from
+// HBM: 4 x 4096 x 12800 13.5 (ring 16.0), 4 x 4096 x 14336 14.9 (17.6), 1 x 9152 x
+// 1664 6.1 (8.3), but 16 x 4096 x 12800 17.5 (16.7) and 4 x 5120 x 12800 22.6 (18.2).
 //   Others the kernel whose fitted time is the least:
 //     16 x 25600 x 4096 ring 21.7 (streamed 30), 333 x 4096 x 12800 ring 34.5 (256-
 //     row tiles 117), 2048 x 6144 x 4096 192-row tiles 47.3 (256-row 50.5, ring
@@ -298,16 +310,22 @@ double tiles_us(int c, int64_t tiles, int64_t k) {
 // rounds alone and leave the other rows (or columns) to a second product, where
 // the fitted times gain 13 %: 2600 x 6144 x 4096 71, whole 82 (192-row tiles) and
 // 78 (ring); 22 such products of random sizes took 0.84 to 1.09 (on average 0.96)
-// of the fastest single kernel.  With less to gain it pays little or nothing: 4096 x
+// of the fastest single kernel.  A rest of few rows or columns that is streamed is
+// counted as nothing: short K, where this happens, takes a single kernel longer than
+// fitted (its stores), by more than the rest.  Six such splits took 0.90 to 1.04 (on
+// average 0.96) of the fastest single kernel, 4100 x 4096 x 256 15.9 and 16.8, 8200 x
+// 4096 x 384 27.7 and 26.6; with the rest's time counted, the plan left them to slower
+// kernels (19.2, 38.0).  With less to gain splitting pays little or nothing: 4096 x
 // 25600 x 4096 417 and 427, 1500 x 25600 x 4096 169 and 171, 4000 x 6200 x 2048 77
 // and 63.
 Fp8Plan fp8_plan(int64_t m, int64_t n, int64_t k, int64_t max_bytes, bool whole = false) {
-  Fp8Plan best;
   const int64_t wgs = ceil_div(n, 16) * ceil_div(m, 16);
-  if (k < kGroup || (m <= 8 && wgs > 96 && wgs <= 256 && k <= 100 * kGroup) ||
+  const Fp8Plan stream{Fp8Plan::kStream, 0, 1, 0, 0, stream_us(m, n, k)};
+  if (k < kGroup ||
       (wgs <= 512 && k <= 32 * kGroup && wgs * k <= (m <= 16 ? 1 << 21 : 1 << 20)))
-    return best;
-  best = fp8_ring_plan(m, n, k, max_bytes);
+    return stream;
+  Fp8Plan best = fp8_ring_plan(m, n, k, max_bytes);
+  if (stream.us < 0.95 * best.us) best = stream;
   if (k < 2 * kGroup || k % kGroup != 0) return best;
   for (int c = 0; c < 2; ++c) {
     const int64_t bn = c == 0 ? 256 : 192, tm = ceil_div(m, dl8::BM), tn = ceil_div(n, bn);
@@ -322,7 +340,9 @@ Fp8Plan fp8_plan(int64_t m, int64_t n, int64_t k, int64_t max_bytes, bool whole 
       if (done == 0 || done >= (cols ? n : m)) continue;
       const Fp8Plan rest = cols ? fp8_plan(m, n - done, k, max_bytes, true)
                                 : fp8_plan(m - done, n, k, max_bytes, true);
-      const double both = tiles_us(c, cols ? tm * (done / bn) : done / dl8::BM * tn, k) + rest.us;
+      // (a streamed rest counts nothing, see above)
+      const double both = tiles_us(c, cols ? tm * (done / bn) : done / dl8::BM * tn, k) +
+                          (rest.kernel == Fp8Plan::kStream ? 0 : rest.us);
       if (both < 0.87 * best.us) {
         best = Fp8Plan{Fp8Plan::kTiles, c, 1, 0, rest.bytes, both};
         (cols ? best.n1 : best.m1) = done;

@@ -233,6 +233,19 @@ def test_silu_mul_extremes(device):
     assert q[8] == 0
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_silu_mul_deep_in_the_negative_tail(device):
+    """Gates at which exp(-g) is near the end of fp32's range, with up values that
+    bring the product back into it."""
+    g = torch.tensor([-80.0, -85.0, -86.5, -87.0, -87.5, -88.0, -88.5])
+    gu = torch.cat([g[:, None].expand(7, 128), torch.full((7, 128), 2.0 ** 110)], 1).bfloat16()
+    q, s = ops.silu_mul_fp8(gu.to(device))
+    g, u = gu.double().chunk(2, 1)
+    y = g / (1 + torch.exp(-g)) * u
+    check_codes(q, y)
+    check_scales(s, group_amax(y) / 448, 2.0 ** -20)
+
+
 # ---- mm_fp8 ------------------------------------------------------------------
 
 def whole_operands(m, n, k, seed=0):

@@ -104,21 +104,21 @@ struct Values {
   }
 };
 
-// silu(g) = g / (1 + exp(-g)) with exp(-g) = 2^n 2^f, n + f = -g log2(e), n
-// whole: f keeps its relative precision for large |g| (log2(e) in two parts).
-// The division is a reciprocal (1 ulp) and one correction of the quotient by its
-// remainder.  2048 x 12800: 27.7 us (25.6 at copy rate), 26.8 without the
-// correction, whose values near a tie fall to the other code twice as often;
-// with the library's expf and an IEEE division 33.8.
+// silu(g) = g / (1 + t) for g >= 0, g t / (1 + t) below, t = exp(-|g|) = 2^n 2^f, n + f =
+// -|g| log2(e), n whole: f keeps its relative precision for large |g| (log2(e) in two
+// parts), and the divisor stays in [1, 2].  (As g / (1 + exp(-g)) 1.5 % faster, but
+// the reciprocal flushes subnormal results: 0 from g = -87.3 on.)  The division is a
+// reciprocal (1 ulp) and one correction by its remainder; without it values near a
+// tie fall to the other code twice as often, for 3 % of the time of 2048 x 12800;
+// the library's expf and an IEEE division cost 22 %.
 __device__ inline float silu_fast(float g) {
-  // (past 150 exp is 0 or infinite in fp32 either way)
-  const float c = __builtin_amdgcn_fmed3f(g, -150.f, 150.f);
+  const float c = fminf(fabsf(g), 150.f);  // (past 150 t is 0 in fp32)
   const float n = rintf(c * -1.44269502f);
   const float f = fmaf(c, -1.92596299e-8f, fmaf(c, -1.44269502f, -n));
-  const float e = __builtin_amdgcn_ldexpf(__builtin_amdgcn_exp2f(f), static_cast<int>(n));
-  const float d = 1.f + e, r = __builtin_amdgcn_rcpf(d), q = g * r;
-  const float t = fmaf(fmaf(-q, d, g), r, q);
-  return t == t ? t : q;  // (an infinite d or g has no remainder)
+  const float t = __builtin_amdgcn_ldexpf(__builtin_amdgcn_exp2f(f), static_cast<int>(n));
+  const float a = g < 0.f ? g * t : g;
+  const float d = 1.f + t, r = __builtin_amdgcn_rcpf(d);
+  return a * fmaf(fmaf(-d, r, 1.f), r, r);
 }
 
 template <typename T>

@@ -758,3 +758,22 @@ def test_fakes_of_products_and_weights_match():
         real = results(x, w, bias)
         with FakeTensorMode() as mode:
             assert results(*(mode.from_tensor(t) for t in (x, w, bias))) == real
+
+
+@pytest.mark.gpu
+def test_operands_on_another_device_than_the_current_one():
+    """Strided operands are copied first, on their own device too."""
+    if torch.spyre.device_count() < 2:
+        pytest.skip("needs two GPUs")
+    x, w = rand((40, 512), 39), rand((130, 256), 40)
+    q, s = ops.quantize_fp8(x[:, ::2])
+    wq, ws = ops.quantize_fp8(w, 128)
+    assert torch.spyre.current_device() == 0
+    x1, w1 = x.to("spyre:1"), w.to("spyre:1")
+    q1, s1 = ops.quantize_fp8(x1[:, ::2])
+    w1q, w1s = ops.quantize_fp8(w1, 128)
+    assert torch.equal(codes64(q1), codes64(q)) and torch.equal(s1.cpu(), s)
+    y = ops.mm_fp8(q1, s1, w1q, w1s, torch.float16)
+    assert y.device.index == 1 and torch.spyre.current_device() == 0
+    want, mags = mm64(q, s, wq, ws), mm64(q, s, wq, ws, mags=True)
+    assert bool(((y.cpu().double() - want).abs() <= mags * 2.0 ** -12 + want.abs() * 2.0 ** -10).all())

@@ -95,8 +95,8 @@ std::tuple<at::Tensor, at::Tensor> quantize_fp8(const at::Tensor& x, int64_t blo
               "quantize_fp8: block_rows must be 1 or 128, got ", block_rows);
   TORCH_CHECK(block_rows == 1 || x.dim() == 2,
               "quantize_fp8: blocks of 128 rows need a 2-dimensional x");
-  const Rows r = as_rows(x, "quantize_fp8");
   c10::DeviceGuard guard(x.device());
+  const Rows r = as_rows(x, "quantize_fp8");
   at::Tensor q = empty_codes(x.sizes(), x.device()), s;
   int64_t sr = 1, sg = r.rows;
   if (block_rows == 1) {
@@ -119,10 +119,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> norm(const char* op, const at::Te
                                                     const std::optional<at::Tensor>& weight,
                                                     double eps) {
   TORCH_CHECK(half_type(x.scalar_type()), op, ": x must be fp16 or bf16, got ", x.scalar_type());
+  c10::DeviceGuard guard(x.device());
   const Rows r = as_rows(x, op);
   Rows res{};
   at::Tensor h;
-  c10::DeviceGuard guard(x.device());
   if (residual) {
     check_device(*residual, x, op, "residual");
     TORCH_CHECK(residual->sizes() == x.sizes() && residual->scalar_type() == x.scalar_type(), op,
@@ -166,11 +166,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rms_norm_fp8(
 std::tuple<at::Tensor, at::Tensor> silu_mul_fp8(const at::Tensor& gu) {
   TORCH_CHECK(half_type(gu.scalar_type()), "silu_mul_fp8: gate_up must be fp16 or bf16, got ",
               gu.scalar_type());
+  c10::DeviceGuard guard(gu.device());
   const Rows r = as_rows(gu, "silu_mul_fp8");
   TORCH_CHECK(r.cols % 2 == 0, "silu_mul_fp8: the last dimension must be even, got ", r.cols);
   std::vector<int64_t> shape(gu.sizes().begin(), gu.sizes().end());
   shape.back() = r.cols / 2;
-  c10::DeviceGuard guard(gu.device());
   at::Tensor q = empty_codes(shape, gu.device());
   at::Tensor s = empty_scales(shape, r.rows, gu.device());
   SPYRE_SPH_CHECK(sph_silu_mul_fp8(to_sph(gu.scalar_type()), r.t.data_ptr(), r.ld, r.rows,

@@ -321,7 +321,7 @@ int sph_rmsnorm_fp8(sph_dtype dtype, sph_dtype w_dtype, const void* x, int64_t l
                     sph_stream_t stream);
 
 /* Codes of silu(gu[:, :cols]) * gu[:, cols:2*cols] for gu [rows, 2*cols] (row
- * stride ld), formed in fp32.  dtype F16 / BF16. */
+ * stride ld), formed in fp32.  dtype F16 / BF16; at most 268435440 rows. */
 int sph_silu_mul_fp8(sph_dtype dtype, const void* gu, int64_t ld, int64_t rows, int64_t cols,
                      void* q, int64_t ldq, float* scale, int64_t scale_row_stride,
                      int64_t scale_group_stride, sph_stream_t stream);

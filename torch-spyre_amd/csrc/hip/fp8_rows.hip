@@ -96,7 +96,6 @@ struct Out {
 // columns behind gate.
 template <typename T>
 struct Values {
-  static constexpr bool kRowsFirst = false;
   const T* x;
   int64_t ld;
   __device__ inline void load(int64_t row, int64_t c0, int64_t cols, float (&v)[8]) const {
@@ -123,7 +122,6 @@ __device__ inline float silu_fast(float g) {
 
 template <typename T>
 struct SiluMul {
-  static constexpr bool kRowsFirst = true;
   const T* x;
   int64_t ld;
   __device__ inline void load(int64_t row, int64_t c0, int64_t cols, float (&v)[8]) const {
@@ -137,18 +135,16 @@ struct SiluMul {
 
 // Groups of 1 x 128.  A wave takes one group of 4 consecutive rows, a workgroup
 // 16 rows, so the scales that it writes lie side by side where a group's scales
-// of all rows do (sr = 1).  (Two groups a wave with their loads ahead: 2331 x 4096
-// 7.1 us instead of 6.8, silu of 2048 x 12800 29.5 instead of 28.2.)
-//
-// Workgroups go along a row's groups first for plain values (8192 x 4096 17.9 us,
-// 20.4 with the rows first; 4096 x 12800 29.4 and 34.1) and along the rows first
-// for the two streams of gate and up (2048 x 12800 24.6 us, 28.9 with the groups
-// first; 2331 x 4096 10.1 and 12.0; behind only from 8192 x 4096 on, 44.0 and 36.7).
+// of all rows do (sr = 1).  (Two groups a wave with their loads ahead: 5 % slower.)
+// Workgroups go along a row's groups first: with operands from memory 8192 x 4096 to
+// codes 21.4 us, 24.0 with the rows first; silu of 2048 x 12800 27.5 and 29.3, of
+// 8192 x 4096 33.5 and 41.2; from the caches the same up to 2048 x 12800 (23.2 and
+// 23.4), 42.8 and 41.6 at 4096 x 12800.
 template <typename S>
 __global__ void __launch_bounds__(256) fp8_groups_kernel(S src, Out o, int64_t rows, int64_t cols) {
   const int l16 = threadIdx.x % kLanes, r16 = threadIdx.x / kLanes;
-  const int64_t ng = (cols + kGroup - 1) / kGroup, nr = (rows + 15) / 16;
-  auto group = [&](int64_t rb, int64_t g) __attribute__((always_inline)) {
+  const int64_t g = blockIdx.x, nr = (rows + 15) / 16;
+  for (int64_t rb = blockIdx.y; rb < nr; rb += gridDim.y) {
     const int64_t row = rb * 16 + r16, c0 = g * kGroup + l16 * 8;
     if (row >= rows) return;
     float v[8];
@@ -156,11 +152,6 @@ __global__ void __launch_bounds__(256) fp8_groups_kernel(S src, Out o, int64_t r
     const float amax = __uint_as_float(max(group_max(amax8(v)), kLeastBits));
     store_codes(o.q + row * o.ldq, c0, cols, codes8(v, kTop / amax));
     if (l16 == 0) o.scale[row * o.sr + g * o.sg] = amax / kTop;
-  };
-  if constexpr (S::kRowsFirst) {
-    for (int64_t g = blockIdx.y; g < ng; g += gridDim.y) group(blockIdx.x, g);
-  } else {
-    for (int64_t rb = blockIdx.y; rb < nr; rb += gridDim.y) group(rb, blockIdx.x);
   }
 }
 
@@ -334,9 +325,8 @@ template <typename S>
 int launch_groups(const char* what, const S& src, const Out& o, int64_t rows, int64_t cols,
                   hipStream_t stream) {
   const int64_t ng = fp8::groups(cols), nr = ceil_div(rows, 16);
-  const int64_t gx = S::kRowsFirst ? nr : ng, gy = S::kRowsFirst ? ng : nr;
-  if (const int rc = fp8::check_grid(what, gx, 256)) return rc;
-  const dim3 grid(static_cast<uint32_t>(gx), static_cast<uint32_t>(gy < 65535 ? gy : 65535));
+  if (const int rc = fp8::check_grid(what, ng, 256)) return rc;
+  const dim3 grid(static_cast<uint32_t>(ng), static_cast<uint32_t>(nr < 65535 ? nr : 65535));
   fp8_groups_kernel<S><<<grid, 256, 0, stream>>>(src, o, rows, cols);
   return check_launch(what);
 }
@@ -413,6 +403,7 @@ extern "C" int sph_silu_mul_fp8(sph_dtype dtype, const void* gu, int64_t ld, int
   if (const int rc = check_out("sph_silu_mul_fp8", rows, cols, o)) return rc;
   SPH_REQUIRE(rows <= 1 || ld >= 2 * cols, SPH_ERR_INVALID_ARG,
               "sph_silu_mul_fp8: ld is less than the gate and up columns");
+  if (const int rc = fp8::check_grid("sph_silu_mul_fp8", ceil_div(rows, 16), 256)) return rc;
   SPH_REQUIRE(dtype == SPH_F16 || dtype == SPH_BF16, SPH_ERR_UNSUPPORTED,
               "sph_silu_mul_fp8: dtype must be F16 or BF16");
   if (rows == 0 || cols == 0) return SPH_OK;

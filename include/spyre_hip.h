@@ -330,9 +330,10 @@ int sph_silu_mul_fp8(sph_dtype dtype, const void* gu, int64_t ld, int64_t rows, 
  * + bias[j], rounded once to dtype (F16 or BF16): X [m, k] and W [n, k] are
  * codes, xs and ws their scales by element strides, bias (may be NULL) has
  * dtype.  Group sums come from the 8-bit matrix instruction, whose own sum is
- * off by up to some 1e-5 of the terms' magnitudes (so no fp32 result is
- * offered), scales and their accumulation are fp32; products of two scales
- * have to be finite.  Rows of X and W must begin on 16 bytes (else
+ * off by 1e-5 (normal data) to 1.6e-4 (any codes) of the terms' magnitudes (so
+ * no fp32 result is offered); scales and their accumulation are fp32.  Products
+ * of two scales have to be finite; below 2^-126 they lose bits, an error of at
+ * most 2^-125 for each group of K.  Rows of X and W must begin on 16 bytes (else
  * SPH_ERR_UNSUPPORTED) and are read in whole aligned 16-byte chunks; what lies
  * past k in the last one does not count.  m is at most 1048560, k, ldx and ldw
  * at most 4194303, x_scale_row_stride at most 2097152 (m of 1: any), n what the

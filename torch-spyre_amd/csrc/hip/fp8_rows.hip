@@ -11,8 +11,10 @@
 // All of them are bound by memory: 16 lanes hold a group, 8 columns each (one
 // 16-byte load of 16-bit values, one 8-byte store of codes), and the largest
 // magnitude goes over the 16 lanes by DPP, without LDS.  At the rate of a large
-// copy (5.1 TB/s) and here: 4096 x 12800 in blocks 30.6 and 29.9 us, residual,
-// norm and codes of 8192 x 4096 45.8 and 52, 2331 x 4096 to codes 5.6 and 6.5.
+// copy (5.14 TB/s) and here, operands from memory: 4096 x 12800 in blocks 30.6 and
+// 30.7 us (of fp32 51.0 and 45.6), 8192 x 4096 to codes 19.6 and 21.4, to norm and
+// codes 19.6 and 30.7, with residual 45.7 and 49.8, silu of 2048 x 12800 25.5 and
+// 27.5, of 8192 x 4096 32.6 and 33.5.
 #include "fp8_common.h"
 
 namespace sph {
@@ -73,7 +75,7 @@ __device__ inline uint2 codes8(const float (&v)[8], float r) {
 
 __device__ inline void store_codes(uint8_t* __restrict__ row, int64_t c0, int64_t cols, uint2 w) {
   if (c0 + 8 <= cols) {
-    // (streaming: 8192 x 4096 rows to codes 24.2 us without, 20.4 with)
+    // (streaming: 4096 x 12800 in blocks 33.8 us without, 30.7 with)
     __builtin_nontemporal_store(u32x2_any{w.x, w.y}, reinterpret_cast<u32x2_any*>(row + c0));
   } else {
     const uint64_t b = (static_cast<uint64_t>(w.y) << 32) | w.x;
@@ -357,8 +359,8 @@ int launch_rmsnorm(const NormArgs& p, hipStream_t stream) {
 template <typename T, typename W>
 int rmsnorm(const NormArgs& p, hipStream_t stream) {
   // One chunk of 8 columns a thread wherever a workgroup holds the row: 8192 x
-  // 4096 (with residual) 52.1 us on 512 threads, 54.0 on 256 of two chunks, 68.6
-  // on 64 of eight; 1000 x 16384 25.5 by passes, 27.4 on 1024 threads of two.
+  // 4096 (with residual) 49.8 us on 512 threads, 52.3 on 256 of two chunks, 66.7
+  // on 64 of eight; 1000 x 16384 25.1 by passes, 26.7 on 1024 threads of two.
   if (p.cols <= 512) return launch_rmsnorm<T, W, 64, 1>(p, stream);
   if (p.cols <= 1024) return launch_rmsnorm<T, W, 64, 2>(p, stream);
   if (p.cols <= 2048) return launch_rmsnorm<T, W, 256, 1>(p, stream);

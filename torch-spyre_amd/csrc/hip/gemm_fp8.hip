@@ -37,7 +37,7 @@ namespace {
 //     of W's first 128 rows (of a 192-row tile: its first block), 6 and 7 the
 //     next.
 //
-// 4096 x 25600 x 4096: 417 to 427 us, 2010 to 2060 TFLOP/s.  Bound by the chip's
+// 4096 x 25600 x 4096: 417 to 430 us, 2000 to 2060 TFLOP/s.  Bound by the chip's
 // power and the tiles' way through LDS together: the clock stands at 2.05 GHz
 // (2.35 without the loads), the matrix cores are busy 53 % of it, and of the time
 // 90 us go with the direct loads and 48 with the stores (327 and 369 us without);
@@ -290,34 +290,34 @@ double stream_us(int64_t m, int64_t n, int64_t k) {
          static_cast<double>(ceil_div(wgs, kTileCUs) * k) * rows * 1e-3 / kCuKB;
 }
 
-// The kernel of a product (one MI355X, operands of three products in turn, us).
+// The kernel of a product (one MI355X, W from memory, us).
 //   Streamed rows, where one pass of workgroups over 16 rows each of X and W and
 // 4 blocks a wave is the whole product: 512 workgroups and K of 4096 at most,
 // above 16 rows (W read more than once, from the caches) half of their product.
-//     1 x 6144 x 4096 8.0 (ring 8.8), 16 x 4096 x 4096 6.6 (8.2), 16 x 8192 x 4096
-//     10.3 (10.3), 16 x 12288 x 4096 14.8 (12.1), 64 x 2048 x 2048 5.8 (6.9), 512 x
-//     256 x 4096 10.2 (8.2)
+//     1 x 6144 x 4096 8.2 (ring 9.6), 16 x 4096 x 4096 7.0 (9.0), 16 x 8192 x 4096
+//     11.1 (11.4), 16 x 12288 x 4096 15.5 (14.3), 64 x 2048 x 2048 6.3 (7.5), 512 x
+//     256 x 4096 10.0 (9.0)
 //   Elsewhere too where its fitted time is 5 % below the ring's: of 1494 products of
-// up to 70 rows 67 stream by this, 0.83 to 1.07 (on average 0.89) of the time of
-// the kernel they had by the limits above and K to 12800 for up to 8 rows.  W from
-// HBM: 4 x 4096 x 12800 13.5 (ring 16.0), 4 x 4096 x 14336 14.9 (17.6), 1 x 9152 x
-// 1664 6.1 (8.3), but 16 x 4096 x 12800 17.5 (16.7) and 4 x 5120 x 12800 22.6 (18.2).
+// up to 70 rows 67 stream by this, 0.73 to 1.12 (on average 0.89) of the time of
+// the kernel they had by the limits above and K to 12800 for up to 8 rows:
+//     4 x 4096 x 12800 13.5 (ring 16.0), 4 x 4096 x 14336 14.9 (17.6), 1 x 9152 x 1664
+//     6.1 (8.3), but 16 x 4096 x 12800 17.5 (16.7) and 4 x 5120 x 12800 22.6 (18.2)
 //   Others the kernel whose fitted time is the least:
-//     16 x 25600 x 4096 ring 21.7 (streamed 30), 333 x 4096 x 12800 ring 34.5 (256-
-//     row tiles 117), 2048 x 6144 x 4096 192-row tiles 47.3 (256-row 50.5, ring
-//     63), 2048 x 25600 x 4096 256-row tiles 239 (ring 262)
+//     16 x 25600 x 4096 ring 24.3 (streamed 30.8), 333 x 4096 x 12800 ring 38.4 (192-
+//     row tiles 131), 2048 x 6144 x 4096 192-row tiles 52.8 (256-row 60.6, ring 76),
+//     1500 x 25600 x 4096 256-row tiles 175 (ring 192)
 //   Large tiles that would leave most of a last round of workgroups idle take whole
 // rounds alone and leave the other rows (or columns) to a second product, where
-// the fitted times gain 13 %: 2600 x 6144 x 4096 71, whole 82 (192-row tiles) and
-// 78 (ring); 22 such products of random sizes took 0.84 to 1.09 (on average 0.96)
-// of the fastest single kernel.  A rest of few rows or columns that is streamed is
-// counted as nothing: short K, where this happens, takes a single kernel longer than
-// fitted (its stores), by more than the rest.  Six such splits took 0.90 to 1.04 (on
-// average 0.96) of the fastest single kernel, 4100 x 4096 x 256 15.9 and 16.8, 8200 x
-// 4096 x 384 27.7 and 26.6; with the rest's time counted, the plan left them to slower
-// kernels (19.2, 38.0).  With less to gain splitting pays little or nothing: 4096 x
-// 25600 x 4096 417 and 427, 1500 x 25600 x 4096 169 and 171, 4000 x 6200 x 2048 77
-// and 63.
+// the fitted times gain 13 %: 2048 x 25600 x 4096 210, whole 233; 13 such products
+// of random sizes took 0.90 to 1.12 (on average 0.97) of the fastest single kernel.
+// A rest of few rows or columns that is streamed is counted as nothing: short K,
+// where this happens, takes a single kernel longer than fitted (its stores), by more
+// than the rest.  Six such splits took 0.90 to 1.04 (on average 0.96) of the fastest
+// single kernel, 4100 x 4096 x 256 15.9 and 16.8, 8200 x 4096 x 384 27.7 and 26.6;
+// with the rest's time counted, the plan left them to slower kernels (19.2, 38.0).
+// With less to gain splitting pays little or nothing: 4096 x 25600 x 4096 410 and 425,
+// 1500 x 25600 x 4096 170 and 175, 4000 x 6200 x 2048 65.3 and 66.7, though 2600 x
+// 6144 x 4096 74 and 79 (ring).
 Fp8Plan fp8_plan(int64_t m, int64_t n, int64_t k, int64_t max_bytes, bool whole = false) {
   const int64_t wgs = ceil_div(n, 16) * ceil_div(m, 16);
   const Fp8Plan stream{Fp8Plan::kStream, 0, 1, 0, 0, stream_us(m, n, k)};

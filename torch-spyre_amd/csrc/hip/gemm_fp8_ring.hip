@@ -15,9 +15,11 @@
 // barrier, LDS, MFMA, FMA) whatever its size, so the small tiles take two blocks
 // a step (256 x 4096 x 4096 in 32 x 64 tiles 12.1 us, 15.1 with one) and the
 // larger ones 8 waves (777 x 6144 x 4096 in 128 x 128 tiles 32.0 us, 39.8 on 4).
-// Few rows are bound by reading W (24 x 49155 x 4096 43 us, 39.7 at copy rate), the
-// others by what is in flight into LDS (333 x 4096 x 12800 34.5 us: 9.5 TB/s from
-// the caches, the matrix cores busy 21 %).  Asking for W's lines three or six
+// Few rows are bound by reading W (24 x 49155 x 4096 45 us, 39.7 at copy rate), the
+// others by what is in flight into LDS (333 x 4096 x 12800 34.6 us: 9.5 TB/s from
+// the caches, the matrix cores busy 21 %).  (Operands of three products in turn, so
+// in part from the caches; with W from memory 256 x 4096 x 4096 17.4, 777 x 6144 x
+// 4096 35.9, 333 x 4096 x 12800 38.4.)  Asking for W's lines three or six
 // steps ahead made all of them slower (44.8 and 43.5 us in the run whose time
 // without was 38.6), 192 x 128 and 256 x 128 tiles no faster (35.2, 40.7).
 #include <algorithm>
@@ -234,9 +236,12 @@ int launch_ring8(Fp8Args& p, hipStream_t st) {
 // launch and TB/s of its sums; TB/s of the tiles' traffic from the caches and of
 // the operands from memory.  Fitted to 7300 timings of 1 to 4400 rows by 256 to
 // 49155 columns, K 256 to 25600, 1 to 16 slices, the weights of most of them read
-// from HBM as a model's layers are (rms error 6 to 8 %; the plan that the fitted
-// times choose is 2 % slower than the fastest of a product on average, 25 % at
-// most: 477 x 1895 x 1664).
+// from HBM as a model's layers are (rms error 6 to 8 %).  The plan that the fitted
+// times choose is 2 % slower than the fastest kernel and slices of a product on
+// average over 1494 products of up to 70 rows and 490 of few columns (30 % at most:
+// 12 x 4046 x 22672; 16 x 4096 x 12800 14 %, 16.7 us in 5 slices and 14.6 in 8), 3 %
+// over 420 of 200 to 9000 rows and K to 2600 (50 % at most: 5904 x 7360 x 256, whose
+// stores the rounds of small tiles leave out).
 struct RingCfg {
   int bm, bn, kb, per_cu, fly;
   double round, launch, blk[3], reduce, sums, traffic, mem;

@@ -10,7 +10,8 @@
 //   * The waves' sums are added through LDS in a fixed order.
 //
 // 1 x 4096 x 4096 5.3 us (3.3 at copy rate), 1 x 6144 x 4096 8.0 (4.9), 16 x 4096 x
-// 4096 6.5.  From the same sweep: 16 waves of 2 blocks 5.3, 8.0 and 6.9, 32 of W's
+// 4096 6.5 (operands of three products in turn; with W from memory 5.7, 8.2 and
+// 7.0).  From the same sweep: 16 waves of 2 blocks 5.3, 8.0 and 6.9, 32 of W's
 // rows a workgroup 6.1, 8.4 and 7.1, 4 waves of 8 blocks 5.9 and 8.5.
 #include <type_traits>
 

@@ -722,6 +722,87 @@ int sph_rope(sph_dtype dtype, const void* x, void* y,
              int64_t head_dim, float theta, sph_stream_t stream);
 
 /* ------------------------------------------------------------------ */
+/* Serving from a paged KV cache                                        */
+/* The reference has no KV cache; what a user of it writes for a layer  */
+/*   is its composite RMSNorm (codegen/inputs/Metadata.yaml:236-253),   */
+/*   mul / add (base.jinja2:16-241) and spyre__bmm_default              */
+/*   (spyre_torch_ops.cpp:297-377) over copied caches.                  */
+/* ------------------------------------------------------------------ */
+
+/* A step's projection rows qkv [tokens, (n_heads + 2 n_kv_heads) *
+ * head_dim] (query heads, then key heads, then value heads) on their way into
+ * a paged cache.  Query and key heads are normalised where q_norm / k_norm
+ * [head_dim] is given, y = x / sqrt(mean(x^2) + eps) * w, and rotated to
+ * positions[token], y cos + rot(y) sin with rot(y) = (-y2, y1) for the halves
+ * y1, y2 and the rows of cos / sin [n_positions, head_dim]; all in fp32,
+ * rounded once.  The queries go to q [tokens, n_heads, head_dim]; keys
+ * and values to slot slots[token] = page * page_size + position of the caches, whose
+ * element (page, head, position, dim) lies at the given strides (dim stride 1).
+ * A slot below 0 marks a padding row: nothing is appended, its queries are
+ * zeros, its position is not read.  A slot or position out of range stores
+ * 3 to *error_word (may be null) and is treated like padding.  Slots of one call have to
+ * differ; one that is named twice holds elements of either row.
+ * dtype F16 / BF16 (rows and caches), table_dtype and norm_dtype that or F32;
+ * head_dim 64 or 128; rows at any alignment; tokens * ceil((n_heads + 2
+ * n_kv_heads) * head_dim / 2048) below 2^24. */
+int sph_paged_append(sph_dtype dtype, sph_dtype table_dtype, sph_dtype norm_dtype, int64_t tokens,
+                     int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, const void* qkv,
+                     int64_t ld_qkv, const void* cos, int64_t ld_cos, const void* sin,
+                     int64_t ld_sin, int64_t n_positions, const int64_t* positions,
+                     const int64_t* slots, const void* q_norm, const void* k_norm, float eps,
+                     void* k_cache, int64_t k_stride_p, int64_t k_stride_h, int64_t k_stride_s,
+                     void* v_cache, int64_t v_stride_p, int64_t v_stride_h, int64_t v_stride_s,
+                     int64_t n_pages, int64_t page_size, void* q, int32_t* error_word,
+                     sph_stream_t stream);
+
+/* Attention of the new tokens of `batch` sequences over their pages.  Sequence
+ * b has seq_lens[b] keys, key x in page block_table[b * ld_table + x /
+ * page_size] at x % page_size; the last n = q_starts[b + 1] - q_starts[b] of
+ * them are its new tokens, whose queries are rows q_starts[b] .. of q
+ * [tokens, n_heads, head_dim].  New token i sees the keys before the new ones
+ * and, of the new ones, those j with mask[(q_starts[b] + i) * ld_mask + j] != 0
+ * (n at most mask_width) or, with mask NULL, j <= i.  o [tokens, n_heads,
+ * head_dim] (contiguous) = softmax(scale q k^T) v over what is seen; rows that see
+ * nothing and rows of no sequence are 0.  Query head h reads KV head
+ * h / (n_heads / n_kv_heads).  Keys and values that a row does not see have
+ * no effect on it, whatever they hold.
+ * A page, length or start out of range stores 3 to *error_word (may be null);
+ * reads stay inside the caches, and what the sequence's rows hold is then not specified.
+ * dtype F16 / BF16, head_dim 64 or 128, rows at any alignment; at most 4096
+ * sequences, 2^26 query rows, 2^30 keys a sequence.  The workspace
+ * (16-byte aligned, sph_paged_attention_workspace_bytes with max_keys =
+ * table_width * page_size) holds partial results; calls that share one have
+ * to be ordered. */
+int64_t sph_paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t n_heads,
+                                            int64_t n_kv_heads, int64_t head_dim,
+                                            int64_t max_keys);
+int sph_paged_attention(sph_dtype dtype, int64_t tokens, int64_t batch, int64_t n_heads,
+                        int64_t n_kv_heads, int64_t head_dim, const void* q, int64_t q_stride_t,
+                        int64_t q_stride_h, const void* k_cache, int64_t k_stride_p,
+                        int64_t k_stride_h, int64_t k_stride_s, const void* v_cache,
+                        int64_t v_stride_p, int64_t v_stride_h, int64_t v_stride_s,
+                        int64_t n_pages, int64_t page_size, const int64_t* block_table,
+                        int64_t ld_table, int64_t table_width, const int64_t* seq_lens,
+                        const int64_t* q_starts, const uint8_t* mask, int64_t ld_mask,
+                        int64_t mask_width, float scale, void* o, void* workspace,
+                        int64_t workspace_bytes, int32_t* error_word, sph_stream_t stream);
+
+/* tokens[r] drawn from the logits row r [vocab] (F16, BF16 or F32, rows ld
+ * apart) by uniform[r] in [0, 1).  With M the row's maximum and t =
+ * temperature[r] a token weighs exp((l - M) / t); in the order of falling logits,
+ * equal ones by index: top_k[r] > 0 keeps the first so many; top_p[r] < 1 of those
+ * the shortest run from the first that holds this share of their weight (one
+ * at least); min_p[r] those that weigh at least so much (at most 1).  The
+ * token is the first by index at which the weights kept, added by index,
+ * exceed uniform * their sum.  t not above 0: the largest logit, the lowest
+ * index first.  NaN counts as -inf; a row without any logit above -inf gives
+ * -1; beside +inf only +inf counts.  Each of the parameter arrays may be NULL (t =
+ * 1, no filter).  vocab at most 2^20, rows below 2^22. */
+int sph_sample(sph_dtype dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld,
+               const float* uniform, const float* temperature, const int64_t* top_k,
+               const float* top_p, const float* min_p, int64_t* tokens, sph_stream_t stream);
+
+/* ------------------------------------------------------------------ */
 /* Stick (tiled) layout                                                 */
 /* Replaces: the host-side stick conversion of the DMA path            */
 /*   (torch_spyre/csrc/spyre_mem.cpp:62-279, generate_dci /             */

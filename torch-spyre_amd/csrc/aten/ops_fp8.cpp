@@ -253,6 +253,8 @@ at::Tensor mm_fp8(const at::Tensor& x_in, const at::Tensor& x_scale, const at::T
   return out;
 }
 
+}  // namespace
+
 // Rounding to codes has no gradient: a call that would have to record one, or to
 // carry a tangent on, is refused instead of returning tensors that silently cut
 // the graph.
@@ -269,8 +271,6 @@ void refuse_gradients(const c10::OperatorHandle& op, c10::DispatchKeySet ks,
   at::AutoDispatchBelowADInplaceOrView below;
   op.redispatchBoxed(ks & c10::after_autograd_keyset, stack);
 }
-
-}  // namespace
 
 TORCH_LIBRARY_IMPL(spyre, PrivateUse1, m) {
   m.impl("quantize_fp8", TORCH_FN(quantize_fp8));

@@ -5,6 +5,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/TensorIterator.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 
 #include "spyre_runtime.h"
 
@@ -48,5 +49,10 @@ at::Tensor empty_spyre(at::IntArrayRef sizes, at::ScalarType dtype, c10::Device 
 // `nbytes` of workspace for a kernel that also runs without one: undefined for
 // 0 bytes and when the device has no room for them.
 at::Tensor optional_workspace(int64_t nbytes, c10::Device device);
+
+// Autograd kernel of operators without a derivative: raises where a gradient or
+// a tangent is asked for, else carries on below (ops_fp8.cpp).
+void refuse_gradients(const c10::OperatorHandle& op, c10::DispatchKeySet ks,
+                      torch::jit::Stack* stack);
 
 }  // namespace spyre

@@ -160,6 +160,10 @@ void check_device_errors(int device) {
     if (code == 2)
       TORCH_CHECK_INDEX(false, "spyre: decode attention position outside the KV cache on "
                         "spyre:", d, " (code 2); the step wrote nothing");
+    if (code == 3)
+      TORCH_CHECK_INDEX(false, "spyre: page, slot, position, length or start outside the paged KV "
+                        "cache on spyre:", d, " (code 3); rows it concerned were not appended, "
+                        "their results are not specified");
     TORCH_CHECK_INDEX(false, "spyre: index out of range in a gather on spyre:", d,
                       " (index_select / embedding / an indexed load of a compiled kernel; "
                       "code ", code, "); the rows of out-of-range indices were zero-filled");

@@ -116,6 +116,16 @@ _SIGS = {
     "sph_gather_rows": ([vp, c_i64, c_i64, c_int, vp, c_int, c_i64, vp, vp, vp], c_int),
     "sph_tri": ([c_int, c_i64, c_int, vp, vp, c_i64, c_i64, c_i64, vp], c_int),
     "sph_rope": ([c_int, vp, vp, vp, c_i64, c_i64, c_i64, c_f32, vp], c_int),
+    "sph_paged_append": ([c_int] * 3 + [c_i64] * 4 + [vp, c_i64] * 3 + [c_i64, vp, vp, vp, vp, c_f32,
+                                                                     vp, c_i64, c_i64, c_i64, vp,
+                                                                     c_i64, c_i64, c_i64, c_i64,
+                                                                     c_i64, vp, vp, vp], c_int),
+    "sph_paged_attention_workspace_bytes": ([c_i64] * 6, c_i64),
+    "sph_paged_attention": ([c_int] + [c_i64] * 5 + [vp, c_i64, c_i64, vp, c_i64, c_i64, c_i64, vp,
+                                                     c_i64, c_i64, c_i64, c_i64, c_i64, vp, c_i64,
+                                                     c_i64, vp, vp, vp, c_i64, c_i64, c_f32, vp, vp,
+                                                     c_i64, vp, vp], c_int),
+    "sph_sample": ([c_int, c_i64, c_i64, vp, c_i64, vp, vp, vp, vp, vp, vp, vp], c_int),
     "sph_stick_nbytes": ([c_int, ctypes.POINTER(c_i64), ctypes.POINTER(ctypes.c_int32), c_int],
                          c_i64),
     "sph_stick_pack": ([vp, vp, c_int, ctypes.POINTER(c_i64), ctypes.POINTER(c_i64),

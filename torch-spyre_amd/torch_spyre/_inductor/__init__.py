@@ -44,7 +44,7 @@ def _autoload():
 
     from .passes import CustomPostPasses
     from .stickify import install_spyre_tensors
-    from . import customops  # noqa: F401  (registers torch.ops.spyre.*)
+    from . import customops, serving  # noqa: F401  (register torch.ops.spyre.*)
     from . import decompositions, lowering
 
     install_spyre_tensors()

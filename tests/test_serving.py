@@ -312,13 +312,14 @@ def test_attention(step, masked, dtype, device):
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("page", [16, 6])
-def test_attention_ignores_what_is_not_seen(page, dtype, device):
+@pytest.mark.parametrize("heads", [(4, 4), (8, 2), (12, 2)])
+def test_attention_ignores_what_is_not_seen(heads, page, dtype, device):
     """Slots past the sequences' ends, pages of nobody, and new tokens that only some
-    rows see hold NaN and infinities."""
+    rows see hold NaN and infinities.  (13 tokens on average: 13, 54 and 81 rows.)"""
     news, lens = [9, 4, 40, 1], [50, 4, 300, 77]
     mask = torch.rand(sum(news), 40, generator=torch.Generator().manual_seed(3)) < 0.4
     mask[0:3, [2, 5, 8]] = False
-    s = Step(news, lens, 8, 2, 128, page, dtype, mask=mask, k=7, fill=NAN)
+    s = Step(news, lens, *heads, 128, page, dtype, mask=mask, k=7, fill=NAN)
     clean = s.check(device)
     # poisoned new tokens: three of sequence 0, one of sequence 2
     for b, j, bad in ((0, 2, NAN), (0, 5, INF), (0, 8, -INF), (2, 31, NAN)):

@@ -33,9 +33,16 @@
 //     j}.  For V^T each lane loads D / 16 consecutive head dims of its 8 keys
 //     (whole cache rows over 16 lanes) and turns the 8 x D / 16 block with byte
 //     permutes; head dim D / 16 m + t is row m of the product's tile t.
+//   * Sequences with more than 64 rows (128-row tiles, every wave its own rows) would
+//     ask the caches for each key four times: their K and V pass through LDS, 64
+//     keys a stage, two stages, a row's 16-byte chunks swapped by the row's number so that
+//     fragments are read without bank conflicts (V^T by transposing reads).
+//   * A workgroup's next unit is looked up, and its first loads are under way, before
+//     the results of the one before it leave.
 //   * Probabilities round to the element type for the second product; scores,
 //     maxima, sums and O stay fp32; O rounds once.
 #include <algorithm>
+#include <type_traits>
 
 #include "gemm_common.h"
 
@@ -45,6 +52,8 @@ namespace {
 constexpr int PT = 256;                 // threads
 constexpr int kItemKeys = 128;          // keys of one item
 constexpr int kMaxSeqs = 4096;
+constexpr int kMaxGrid = 512;             // two workgroups per CU
+constexpr int kFewParts = 16;             // parts of a unit that one group of lanes merges
 constexpr int32_t kPagedIndex = 3;      // error code: page, length or start out of range
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -68,54 +77,19 @@ struct PagedArgs {
   float scale_log2;
   void* o;        // [tokens, H, D]
   float* part;    // [grid][2] partial tiles
-  int32_t* desc;  // [grid][8]
+  int32_t* desc;  // [grid][8] the unit that begins in a workgroup and ends in another: tasks
+                  // to merge it, workgroups, head, first row, rows, first token
   int32_t* err;
 };
 
-// What a workgroup has to know of one sequence.
-struct Seq {
-  int64_t start;
-  int n, len, rows, rw, tiles;  // rw: groups of rows per workgroup
-};
-
-template <int RT>
-__device__ inline Seq sequence(const PagedArgs& p, int b, bool report) {
-  const int64_t s0 = p.starts[b], s1 = p.starts[b + 1], len = p.lens[b];
-  Seq s{s0, 0, 0, 0, 1, 0};
-  if (s0 < 0 || s1 < s0 || s1 > p.tokens) {
-    if (report && p.err != nullptr) *p.err = kPagedIndex;
-    return s;
-  }
-  s.n = static_cast<int>(s1 - s0);
-  const bool bad = len < s.n || len > p.width * p.page || (p.mask != nullptr && s.n > p.mask_w) ||
-                   (len > 0 && p.n_pages == 0);
-  s.len = bad ? 0 : static_cast<int>(len);
-  if (bad && report && p.err != nullptr) *p.err = kPagedIndex;
-  s.rows = s.n * p.g;
-  constexpr int R = 16 * RT;
-  s.rw = s.rows <= R ? 1 : s.rows <= 2 * R ? 2 : 4;
-  s.tiles = (s.rows + R * s.rw - 1) / (R * s.rw);
-  return s;
-}
-
-// Keys that the rows of a tile can see at most (causal: up to its last token).
-template <int RT>
-__device__ inline int tile_keys(const PagedArgs& p, const Seq& s, int tile) {
-  if (p.mask != nullptr) return s.len;
-  const int last = min((tile + 1) * 16 * RT * s.rw, s.rows) - 1;
-  return s.len == 0 ? 0 : s.len - s.n + last / p.g + 1;
-}
-template <int RT>
-__device__ inline int tile_items(const PagedArgs& p, const Seq& s, int tile) {
-  return max(1, (tile_keys<RT>(p, s, tile) + kItemKeys - 1) / kItemKeys);
-}
-// Items of one KV head of a sequence.
-template <int RT>
-__device__ inline int64_t head_items(const PagedArgs& p, const Seq& s) {
-  int64_t k = 0;
-  if (p.mask != nullptr) return s.tiles * static_cast<int64_t>(s.tiles ? tile_items<RT>(p, s, 0) : 0);
-  for (int t = 0; t < s.tiles; ++t) k += tile_items<RT>(p, s, t);
-  return k;
+// The kernel's arguments, read again wherever they are asked for: held all
+// through the key loop they would not fit the scalar registers, and came from vector
+// registers and scratch memory instead (decoding 64 sequences 124 to 148 us).
+typedef const __attribute__((address_space(4))) PagedArgs* ArgPtr;
+__device__ inline ArgPtr args() {
+  ArgPtr a = (ArgPtr)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(a));
+  return a;
 }
 
 // Values that are the same in every lane, in scalar registers.
@@ -123,6 +97,64 @@ __device__ inline int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ inline int64_t uni(int64_t v) {
   const uint32_t lo = uni(static_cast<int>(v)), hi = uni(static_cast<int>(v >> 32));
   return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// What a workgroup has to know of one sequence.
+struct Seq {
+  int64_t start;
+  int n, len, rows, rw, tiles;  // rw: groups of rows per workgroup
+};
+
+// Forms of the kernel, by the rows that a sequence has on average: a wave takes 16 rows, or
+// 32, or 32 of a 128-row tile whose keys pass through LDS.  Each serves any number.
+enum { DECODE, TREE, WIDE };
+constexpr int rows_of(int form) { return form == DECODE ? 16 : 32; }  // of a wave
+
+template <int FORM>
+__device__ inline Seq sequence(int b, bool report) {
+  const ArgPtr p = args();
+  const int64_t s0 = p->starts[b], s1 = p->starts[b + 1], len = p->lens[b];
+  Seq s{s0, 0, 0, 0, 1, 0};
+  if (s0 < 0 || s1 < s0 || s1 > p->tokens) {
+    if (report && p->err != nullptr) *p->err = kPagedIndex;
+    return s;
+  }
+  s.n = static_cast<int>(s1 - s0);
+  const bool bad = len < s.n || len > p->width * p->page ||
+                   (p->mask != nullptr && s.n > p->mask_w) || (len > 0 && p->n_pages == 0);
+  s.len = bad ? 0 : static_cast<int>(len);
+  if (bad && report && p->err != nullptr) *p->err = kPagedIndex;
+  s.rows = s.n * p->g;
+  constexpr int R = rows_of(FORM);
+  s.rw = FORM == WIDE ? 4 : s.rows <= R ? 1 : s.rows <= 2 * R ? 2 : 4;
+  s.tiles = (s.rows + R * s.rw - 1) / (R * s.rw);
+  return s;
+}
+// (of a sequence that is the same in every lane)
+__device__ inline Seq uni(const Seq& s) {
+  return Seq{uni(s.start), uni(s.n), uni(s.len), uni(s.rows), uni(s.rw), uni(s.tiles)};
+}
+
+// Keys that the rows of a tile can see at most (causal: up to its last token).
+template <int FORM>
+__device__ inline int tile_keys(const Seq& s, int tile) {
+  const ArgPtr p = args();
+  if (p->mask != nullptr || s.len == 0) return s.len;
+  const int last = min((tile + 1) * rows_of(FORM) * s.rw, s.rows) - 1;
+  return s.len - s.n + last / p->g + 1;
+}
+template <int FORM>
+__device__ inline int tile_items(const Seq& s, int tile) {
+  return max(1, (tile_keys<FORM>(s, tile) + kItemKeys - 1) / kItemKeys);
+}
+// Items of one KV head of a sequence.
+template <int FORM>
+__device__ inline int64_t head_items(const Seq& s) {
+  if (s.tiles <= 1 || args()->mask != nullptr)
+    return s.tiles == 0 ? 0 : s.tiles * static_cast<int64_t>(tile_items<FORM>(s, 0));
+  int64_t k = 0;
+  for (int t = 0; t < s.tiles; ++t) k += tile_items<FORM>(s, t);
+  return k;
 }
 
 __device__ inline float xor_max(float v) {
@@ -136,34 +168,43 @@ __device__ inline bool not_finite(uint32_t two) {
   return (two & e) == e || ((two >> 16) & e) == e;
 }
 
-// (uniform) index of a 16-key block's page and the position in it, for 64 blocks at once:
-// lane l holds block first + l.
-struct Blocks {
-  int page, at;
-};
-__device__ inline Blocks blocks(const PagedArgs& p, const int64_t* row, int first, int last) {
-  const int x = min(first + static_cast<int>(threadIdx.x & 63), last) * 16;
-  Blocks b;
-  const int i = x / p.page;
-  const int64_t pg = row[i];
-  const bool ok = pg >= 0 && pg < p.n_pages;
-  if (!ok && p.err != nullptr) *p.err = kPagedIndex;
-  b.page = ok ? static_cast<int>(pg) : 0;
-  b.at = x - i * p.page;
-  return b;
+// Two floats rounded to the element type, lo in the low half.
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+template <typename T>
+__device__ inline uint32_t pack2(float lo, float hi) {
+  const f32x2_t v = {lo, hi};
+  if constexpr (__is_same(T, half_t))
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2_t));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2_t));
 }
 
-// T, head dim, groups of 16 rows per wave, whether pages hold whole blocks of 16 keys.
-template <typename T, int D, int RT, bool P16>
-__global__ void __launch_bounds__(PT) paged_attn_kernel(const PagedArgs p) {
+typedef u32x2 u32x2_any __attribute__((aligned(2)));
+
+// T, head dim, form, whether pages hold whole blocks of 16 keys.
+template <typename T, int D, int FORM, bool P16>
+__global__ void __launch_bounds__(PT) __attribute__((amdgpu_waves_per_eu(2)))
+paged_attn_kernel(const PagedArgs) {
+  constexpr int RT = FORM == DECODE ? 1 : 2;
   constexpr int KK = D / 32, DT = D / 16, R = 16 * RT, PITCH = D + 4;
-  constexpr int VW = DT / 2;  // 32-bit words of a lane's share of a V row
+  constexpr int VW = DT / 2;           // 32-bit words of a lane's share of a V row
+  constexpr int KPB = P16 ? 16 : 1;    // keys per page look-up
+  constexpr bool AHEAD = FORM == DECODE;  // (the others have no registers for it)
+  constexpr int SK = 64, CPR = D / 8;  // keys of a stage, 16-byte chunks of a row
+  constexpr int SR = PT / CPR, SP = SK / SR;  // rows and turns of a stage's loads
+  constexpr int STAGE = SK * D * 2;    // bytes of a stage's K (or V)
+  constexpr int MERGE = 4 * R * PITCH * 4, LDS = FORM == WIDE && 4 * STAGE > MERGE ? 4 * STAGE : MERGE;
+  static_assert(SP <= KK, "a stage fits the registers of a step's keys");
   extern __shared__ int64_t prefix[];  // [batch + 1] items before a sequence
-  __shared__ __attribute__((aligned(16))) float merge[4][R][PITCH];
+  __shared__ __attribute__((aligned(1024))) char lds[LDS];
   __shared__ float mg_m[4][R], mg_l[4][R];
   __shared__ int64_t scan[4];
+  __shared__ uint8_t odd_rows[2][SK];  // keys of a stage with a value that is not finite
+  auto merge = reinterpret_cast<float(*)[R][PITCH]>(lds);
   const int t = threadIdx.x, lane = t & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int wave = uni(t >> 6);
   const int n16 = lane & 15, g4 = lane >> 4;
   // contiguous runs of workgroups to each of the 8 XCDs
   int wg = blockIdx.x;
@@ -171,27 +212,14 @@ __global__ void __launch_bounds__(PT) paged_attn_kernel(const PagedArgs p) {
     const int total = gridDim.x, q = total >> 3, r = total & 7, x = wg & 7;
     wg = x * q + min(x, r) + (wg >> 3);
   }
-
-  // rows that belong to no sequence
-  const int64_t before = min(max(p.starts[0], static_cast<int64_t>(0)), p.tokens);
-  const int64_t behind = min(max(p.starts[p.batch], static_cast<int64_t>(0)), p.tokens);
-  {
-    const int64_t rest = before + p.tokens - behind;
-    const int chunks = p.g * p.nkv * D / 8;
-    for (int64_t x = wg; x < rest; x += gridDim.x) {
-      T* o = static_cast<T*>(p.o) + (x < before ? x : behind + x - before) * p.g * p.nkv * D;
-      const float z[8] = {};
-      for (int c = t; c < chunks; c += PT) store8u<T>(o + c * 8, z);
-    }
-  }
-
+  const int batch = args()->batch;
   // items before every sequence
   int64_t total = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += PT) {
+  for (int b0 = 0; b0 < batch; b0 += PT) {
     int64_t v = 0;
-    if (b0 + t < p.batch) {
-      const Seq s = sequence<RT>(p, b0 + t, wg == 0);
-      v = head_items<RT>(p, s) * p.nkv;
+    if (b0 + t < batch) {
+      const Seq s = sequence<FORM>(b0 + t, wg == 0);
+      v = head_items<FORM>(s) * args()->nkv;
     }
     int64_t x = v;
 #pragma unroll
@@ -206,71 +234,219 @@ __global__ void __launch_bounds__(PT) paged_attn_kernel(const PagedArgs p) {
       if (w < wave) base += scan[w];
       total += scan[w];
     }
-    if (b0 + t < p.batch) prefix[b0 + t] = base + x - v;
+    if (b0 + t < batch) prefix[b0 + t] = base + x - v;
     __syncthreads();
   }
-  if (t == 0) prefix[p.batch] = total;
+  if (t == 0) {
+    prefix[batch] = total;
+    args()->desc[static_cast<int64_t>(wg) * 8] = 0;
+  }
   __syncthreads();
   total = uni(total);
   const int64_t quota = uni(max(static_cast<int64_t>(1), (total + gridDim.x - 1) / gridDim.x));
   int64_t item = wg * quota;
   const int64_t end = min(item + quota, total);
-  int32_t* desc = p.desc + static_cast<int64_t>(wg) * 8;
-  if (t == 0) desc[0] = 0;
-  int b = 0;
-  if (item < end) {  // the sequence that holds the first item
-    int lo = 0, hi = p.batch;  // prefix[lo] <= item < prefix[hi]
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (prefix[mid] <= item) lo = mid;
-      else hi = mid;
-    }
-    b = uni(lo);
-  }
 
-  while (item < end) {
-    while (uni(prefix[b + 1]) <= item) ++b;
-    Seq s = sequence<RT>(p, b, false);
-    s = Seq{uni(s.start), uni(s.n), uni(s.len), uni(s.rows), uni(s.rw), uni(s.tiles)};
-    const int64_t per_head = head_items<RT>(p, s);
-    int64_t rem = item - uni(prefix[b]);
-    const int h = uni(static_cast<int>(rem / per_head));
-    rem -= h * per_head;
-    int tile = 0, count = tile_items<RT>(p, s, 0);
-    if (p.mask != nullptr) {
-      tile = static_cast<int>(rem / count);
-      rem -= static_cast<int64_t>(tile) * count;
+  // The unit that holds an item, from there to its end or this workgroup's.
+  struct Unit {
+    Seq s;
+    int b, h, tile, count;  // sequence, KV head, tile of rows, items of the tile
+    int c0, c1, keys;       // this workgroup's items, keys that the tile's rows see at most
+    int kbeg, kend, ctx;    // keys of the items, keys that every row sees
+  };
+  // (The compiler does not see that all of it is uniform across the loop.)
+  auto scalar = [](const Unit& u) {
+    return Unit{uni(u.s),    uni(u.b),  uni(u.h),    uni(u.tile), uni(u.count), uni(u.c0),
+                uni(u.c1),   uni(u.keys), uni(u.kbeg), uni(u.kend), uni(u.ctx)};
+  };
+  auto locate = [&](int64_t at, int b) {
+    Unit u;
+    if (b < 0) {  // (the first: prefix[lo] <= at < prefix[hi])
+      int lo = 0, hi = batch;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (uni(prefix[mid]) <= at) lo = mid;
+        else hi = mid;
+      }
+      b = lo;
+    }
+    while (uni(prefix[b + 1]) <= at) ++b;
+    u.b = b;
+    u.s = uni(sequence<FORM>(b, false));
+    const int64_t per_head = head_items<FORM>(u.s);
+    int64_t rem = at - uni(prefix[b]);
+    if (rem < per_head) {
+      u.h = 0;
+    } else if ((rem | per_head) >> 31 == 0) {
+      u.h = uni(static_cast<int>(static_cast<uint32_t>(rem) / static_cast<uint32_t>(per_head)));
     } else {
-      while (rem >= count) {
-        rem -= count;
-        count = tile_items<RT>(p, s, ++tile);
+      u.h = uni(static_cast<int>(rem / per_head));
+    }
+    rem -= u.h * per_head;
+    u.tile = 0;
+    u.count = tile_items<FORM>(u.s, 0);
+    if (args()->mask != nullptr) {
+      u.tile = rem < u.count ? 0 : uni(static_cast<int>(rem / u.count));
+      rem -= static_cast<int64_t>(u.tile) * u.count;
+    } else {
+      while (rem >= u.count) {
+        rem -= u.count;
+        u.count = tile_items<FORM>(u.s, ++u.tile);
       }
     }
-    tile = uni(tile);
-    const int c0 = uni(static_cast<int>(rem));
-    const int c1 = static_cast<int>(min(static_cast<int64_t>(count), c0 + (end - item)));
-    const int keys = tile_keys<RT>(p, s, tile);
-    const int kbeg = c0 * kItemKeys, kend = min(keys, c1 * kItemKeys);
-    const int ctx = s.len - s.n;  // keys that every row sees
-    const int rw = s.rw, kw = 4 / rw;
-    const int tile0 = tile * R * rw, row0 = tile0 + (wave % rw) * R;
-    const int step = 32 * kw;
+    u.c0 = static_cast<int>(rem);
+    u.c1 = static_cast<int>(min(static_cast<int64_t>(u.count), u.c0 + (end - at)));
+    u.keys = tile_keys<FORM>(u.s, u.tile);
+    u.kbeg = u.c0 * kItemKeys;
+    u.kend = min(u.keys, u.c1 * kItemKeys);
+    u.ctx = u.s.len - u.s.n;
+    return scalar(u);
+  };
+  auto step_of = [&](const Unit& u) { return FORM == WIDE ? SK : 32 * (4 / u.s.rw); };
+  auto first_key = [&](const Unit& u) { return u.kbeg + 32 * (wave / u.s.rw); };  // of this wave (WIDE: 0)
+  auto last_block = [&](const Unit& u) { return (max(u.keys, 1) - 1) / KPB; };
+  // Page of the look-ups blk .. of a unit, one a lane.
+  auto page_at = [&](const Unit& u, int blk) {
+    const ArgPtr p = args();
+    return p->table[u.b * p->ld_table + min(blk + lane, last_block(u)) * KPB / p->page];
+  };
 
-    // this lane's queries
-    int tok[RT];
-    u32x4 qf[RT][KK];
+  u32x4 qf[RT][KK];
+  int tok[RT];
+  u32x4 kr[2][KK];
+  uint32_t vr[8][VW];
+  // Where a key's rows lie, in bytes from the head's first: lane l holds that of
+  // 16-key block base + l (off P16: of key base + l); `ahead` are the pages after those.
+  const char *Kh, *Vh;
+  int base = 0;
+  int64_t ko = 0, vo = 0, ahead = 0;
+  auto turn_pages = [&](const Unit& u, int blk) {
+    const ArgPtr p = args();
+    base = blk;
+    const int x = min(blk + lane, last_block(u)) * KPB;
+    const bool ok = ahead >= 0 && ahead < p->n_pages;
+    if (!ok && p->err != nullptr) *p->err = kPagedIndex;
+    const int64_t pg = ok ? ahead : 0;
+    const int at = x % p->page;
+    ko = (pg * p->k_sp + at * p->k_ss) * 2;
+    vo = (pg * p->v_sp + at * p->v_ss) * 2;
+    ahead = page_at(u, blk + max(64, step_of(u) / KPB));
+  };
+  auto lane_of = [&](int64_t v, int i) {  // (i uniform)
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(v), i);
+    const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), i);
+    return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+  };
+  const uint32_t k_next = static_cast<uint32_t>(args()->k_ss) * 2;
+  const uint32_t v_next = static_cast<uint32_t>(args()->v_ss) * 2;
+  const uint32_t k_lane = (P16 ? n16 * k_next : 0u) + 16 * g4;
+  const uint32_t v_lane = (P16 ? 4 * g4 * v_next : 0u) + 2 * DT * n16;
+  // A step's 32 keys, as fragments.
+  auto load_k = [&](const Unit& u, int kb) {
+    const int last = last_block(u);
+#pragma unroll
+    for (int th = 0; th < 2; ++th) {
+      const char* src;
+      if constexpr (P16)
+        src = Kh + lane_of(ko, min(kb / 16 + th, last) - base);
+      else
+        src = Kh + __shfl(ko, min(kb + 16 * th + n16, last) - base, 64);
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk)
+        kr[th][kk] = *reinterpret_cast<const u32x4_any*>(src + k_lane + 64 * kk);
+    }
+  };
+  auto load_v = [&](const Unit& u, int kb) {
+    const int last = last_block(u);
+#pragma unroll
+    for (int th = 0; th < 2; ++th) {
+      const char* src = Vh;
+      if constexpr (P16) src += lane_of(vo, min(kb / 16 + th, last) - base);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const char* at = src;
+        if constexpr (P16) at += j * v_next;
+        else at += __shfl(vo, min(kb + 16 * th + 4 * g4 + j, last) - base, 64);
+        at += v_lane;
+        if constexpr (VW == 4) {
+          const u32x4 w = *reinterpret_cast<const u32x4_any*>(at);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) vr[4 * th + j][e] = w[e];
+        } else {
+          const u32x2 w = *reinterpret_cast<const u32x2_any*>(at);
+          vr[4 * th + j][0] = w[0];
+          vr[4 * th + j][1] = w[1];
+        }
+      }
+    }
+  };
+  // A stage's 64 keys: this thread's chunk t % CPR of rows t / CPR + SR i, K in
+  // kr[0], V in kr[1].
+  const int srow = t / CPR, schunk = t % CPR;
+  auto load_stage = [&](const Unit& u, int kb) {
+    const int last = last_block(u);
+#pragma unroll
+    for (int i = 0; i < SP; ++i) {
+      const int row = srow + SR * i;
+      const char *k = Kh + 16 * schunk, *v = Vh + 16 * schunk;
+      if constexpr (P16) {
+        const int blk = min((kb + SR * i + uni(srow)) / 16, last) - base;
+        k += lane_of(ko, blk) + (row & 15) * k_next;
+        v += lane_of(vo, blk) + (row & 15) * v_next;
+      } else {
+        const int x = min(kb + row, last) - base;
+        k += __shfl(ko, x, 64);
+        v += __shfl(vo, x, 64);
+      }
+      kr[0][i] = *reinterpret_cast<const u32x4_any*>(k);
+      kr[1][i] = *reinterpret_cast<const u32x4_any*>(v);
+    }
+  };
+  // Queries of a unit and its first keys (its first pages are in `ahead`).
+  auto begin = [&](const Unit& u) {
+    const int row0 = u.tile * R * u.s.rw + (wave % u.s.rw) * R;
+    const ArgPtr p = args();
+    Kh = reinterpret_cast<const char*>(static_cast<const T*>(p->kc) + u.h * p->k_sh);
+    Vh = reinterpret_cast<const char*>(static_cast<const T*>(p->vc) + u.h * p->v_sh);
+    const int kb = first_key(u);
+    if (kb < u.kend && (FORM == WIDE || row0 < u.s.rows)) {
+      turn_pages(u, kb / KPB);
+      if constexpr (FORM == WIDE) {
+        load_stage(u, kb);
+      } else {
+        load_k(u, kb);
+        load_v(u, kb);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
-      const int r = min(row0 + 16 * i + n16, s.rows - 1);
-      tok[i] = r / p.g;
-      const T* q = static_cast<const T*>(p.q) + (s.start + tok[i]) * p.q_st +
-                   static_cast<int64_t>(h * p.g + r % p.g) * p.q_sh;
+      const int r = min(row0 + 16 * i + n16, u.s.rows - 1);
+      tok[i] = r / p->g;
+      const T* q = static_cast<const T*>(p->q) + (u.s.start + tok[i]) * p->q_st +
+                   static_cast<int64_t>(u.h * p->g + r % p->g) * p->q_sh;
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk)
         qf[i][kk] = *reinterpret_cast<const u32x4_any*>(q + 32 * kk + 8 * g4);
     }
-    const bool rows_here = row0 < s.rows;
+  };
 
+  Unit u{}, next{};
+  if (item < end) {
+    u = locate(item, -1);
+    ahead = page_at(u, first_key(u) / KPB);
+    begin(u);
+  }
+  while (item < end) {
+    u = scalar(u);
+    item = uni(item);
+    const bool more_units = AHEAD && item + (u.c1 - u.c0) < end;
+    int64_t ahead_next = 0;
+    if (more_units) {
+      next = locate(item + (u.c1 - u.c0), u.b);
+      ahead_next = page_at(next, first_key(next) / KPB);
+    }
+    const int tile0 = u.tile * R * u.s.rw, row0 = tile0 + (wave % u.s.rw) * R;
+    const int kend = u.kend, ctx = u.ctx;
     f32x4 o[RT][DT];
     float m[RT], l[RT];
 #pragma unroll
@@ -280,217 +456,258 @@ __global__ void __launch_bounds__(PT) paged_attn_kernel(const PagedArgs p) {
 #pragma unroll
       for (int d = 0; d < DT; ++d) o[i][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
+    const float c = args()->scale_log2;
 
-    const T* Kh = static_cast<const T*>(p.kc) + h * p.k_sh;
-    const T* Vh = static_cast<const T*>(p.vc) + h * p.v_sh;
-    const int64_t* trow = p.table + b * p.ld_table;
-    const int last_block = (max(keys, 1) - 1) / 16;
-    int first_block = -1;
-    Blocks tab{0, 0};
-    u32x4 kr[2][KK];
-    uint32_t vr[8][VW];
-    // The page and position of key block `blk` (16 keys) or, off P16, of this lane's own key.
-    auto load_k = [&](int kb) {
+    // Scores of 32 keys from kb on that a row does not see.
+    auto hide = [&](f32x4 (&sc)[RT][2], int kb) {
+      const ArgPtr p = args();
+      const int k0 = kb + 4 * g4;
 #pragma unroll
-      for (int th = 0; th < 2; ++th) {
-        const T* src;
-        if constexpr (P16) {
-          const int i = min(kb / 16 + th, last_block) - first_block;
-          const int pg = __builtin_amdgcn_readlane(tab.page, i);
-          const int at = __builtin_amdgcn_readlane(tab.at, i);
-          src = Kh + pg * p.k_sp + at * p.k_ss + n16 * p.k_ss;
+      for (int i = 0; i < RT; ++i) {
+        uint8_t named[8];
+        if (p->mask != nullptr) {
+          const uint8_t* mr = p->mask + (u.s.start + tok[i]) * p->ld_mask;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            named[j] = mr[max(0, min(k0 + 16 * (j >> 2) + (j & 3) - ctx, u.s.n - 1))];
         } else {
-          const int i = min(kb + 16 * th + n16, keys - 1) - first_block;
-          src = Kh + __shfl(tab.page, i, 64) * p.k_sp + __shfl(tab.at, i, 64) * p.k_ss;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) named[j] = k0 + 16 * (j >> 2) + (j & 3) - ctx <= tok[i];
         }
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk)
-          kr[th][kk] = *reinterpret_cast<const u32x4_any*>(src + 32 * kk + 8 * g4);
-      }
-    };
-    auto load_v = [&](int kb) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int th = j >> 2, in = 4 * g4 + (j & 3);
-        const T* src;
-        if constexpr (P16) {
-          const int i = min(kb / 16 + th, last_block) - first_block;
-          const int pg = __builtin_amdgcn_readlane(tab.page, i);
-          const int at = __builtin_amdgcn_readlane(tab.at, i);
-          src = Vh + pg * p.v_sp + at * p.v_ss + in * p.v_ss;
-        } else {
-          const int i = min(kb + 16 * th + in, keys - 1) - first_block;
-          src = Vh + __shfl(tab.page, i, 64) * p.v_sp + __shfl(tab.at, i, 64) * p.v_ss;
-        }
-        src += DT * n16;
-        if constexpr (VW == 4) {
-          const u32x4 w = *reinterpret_cast<const u32x4_any*>(src);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) vr[j][e] = w[e];
-        } else {
-          typedef u32x2 u32x2_any __attribute__((aligned(2)));
-          const u32x2 w = *reinterpret_cast<const u32x2_any*>(src);
-          vr[j][0] = w[0];
-          vr[j][1] = w[1];
-        }
-      }
-    };
-    // 64 blocks of 16 keys (off P16: 64 keys) from kb on
-    auto pages_for = [&](int kb) {
-      constexpr int span = P16 ? 1024 : 64;
-      if (first_block >= 0 && kb + 32 <= (P16 ? 16 : 1) * first_block + span) return;
-      if constexpr (P16) {
-        first_block = kb / 16;
-        tab = blocks(p, trow, first_block, last_block);
-      } else {
-        first_block = kb;
-        const int x = min(kb + lane, keys - 1), i = x / p.page;
-        const int64_t pg = trow[i];
-        const bool ok = pg >= 0 && pg < p.n_pages;
-        if (!ok && p.err != nullptr) *p.err = kPagedIndex;
-        tab.page = ok ? static_cast<int>(pg) : 0;
-        tab.at = x - i * p.page;
-      }
-    };
-
-    int kb = kbeg + 32 * (wave / rw);
-    if (rows_here && kb < kend) {
-      pages_for(kb);
-      load_k(kb);
-      load_v(kb);
-    }
-    for (; rows_here && kb < kend; kb += step) {
-      f32x4 sc[RT][2];
-#pragma unroll
-      for (int i = 0; i < RT; ++i)
-#pragma unroll
-        for (int th = 0; th < 2; ++th) {
-          f32x4 a = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int kk = 0; kk < KK; ++kk) a = mfma16<T>(kr[th][kk], qf[i][kk], a);
-          sc[i][th] = a;
-        }
-      const bool more = kb + step < kend;
-      const bool edge = kb + 32 > ctx;  // keys that not every row sees
-      uint32_t odd = 0;  // keys of this lane's group with a value that is not finite
-      if (edge) {
-        const int k0 = kb + 4 * g4;
-#pragma unroll
-        for (int i = 0; i < RT; ++i)
-#pragma unroll
-          for (int th = 0; th < 2; ++th)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int key = k0 + 16 * th + r, j = key - ctx;
-              bool see = key < kend;
-              if (j >= 0)
-                see = see && (p.mask != nullptr
-                                  ? p.mask[(s.start + tok[i]) * p.ld_mask + j] != 0
-                                  : j <= tok[i]);
-              if (!see) sc[i][th][r] = -INFINITY;
-            }
-        // Slots past the end may hold anything, and a new key that some rows do
-        // not see may hold infinities or NaN, which a probability of 0 would not cancel in
-        // the product: they are taken out here and added below to the rows
-        // that see them.
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int key = k0 + 16 * (j >> 2) + (j & 3);
-          bool drop = key >= kend;
-          if (!drop && key >= ctx) {
+          const bool see = key < kend && (key < ctx || named[j] != 0);
+          sc[i][j >> 2][j & 3] = see ? sc[i][j >> 2][j & 3] : -INFINITY;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    // Scores to probabilities, in place and as the fragment of the second product.
+    auto softmax = [&](f32x4 (&sc)[2], int i) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) mx = fmaxf(mx, sc[j >> 2][j & 3]);
+      mx *= c;
+      // the reference follows the maximum only when it is passed by more than
+      // 8: a probability is then at most 2^8
+      if (__ballot(mx > m[i] + 8.f) != 0) {
+        mx = xor_max(mx);
+        const float to = fmaxf(m[i], mx);
+        const float a = m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[i] - to);
+        l[i] *= a;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[i][d] *= a;
+        m[i] = to;
+      }
+      const float ref = m[i] == -INFINITY ? 0.f : -m[i];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float pr = __builtin_amdgcn_exp2f(fmaf(sc[j >> 2][j & 3], c, ref));
+        sc[j >> 2][j & 3] = pr;
+        l[i] += pr;
+      }
+      u32x4 pf;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) pf[e] = pack2<T>(sc[e >> 1][2 * (e & 1)], sc[e >> 1][2 * (e & 1) + 1]);
+      return pf;
+    };
+    // Values that are not finite, of new keys that some rows do not see: a probability of
+    // 0 would not cancel them in the product, so they were taken out of it and are
+    // added here to the rows that see them.  bits: of the 32 keys from kb on; dim(d, r): where
+    // o[.][d][r] lies.
+    auto add_odd = [&](f32x4 (&sc)[RT][2], int kb, uint32_t bits, auto dim) {
+#pragma unroll 1
+      for (int x = 0; x < 32; ++x) {
+        if ((bits >> x & 1u) == 0) continue;
+        const ArgPtr p = args();
+        const int key = kb + x, j = 4 * (x >> 4) + (x & 3);
+        const int64_t pg = p->table[u.b * p->ld_table + key / p->page];
+        const T* v = reinterpret_cast<const T*>(Vh) + (pg >= 0 && pg < p->n_pages ? pg : 0) * p->v_sp +
+                     (key % p->page) * p->v_ss;
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+          float w = 0.f;
+#pragma unroll
+          for (int y = 0; y < 8; ++y) w = y == j ? sc[i][y >> 2][y & 3] : w;
+          w = __shfl(w, n16 + 16 * (x >> 2 & 3), 64);
+          if (w == 0.f) continue;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[i][d][r] = fmaf(w, Num<T>::to_f(v[dim(d, r)]), o[i][d][r]);
+            __builtin_amdgcn_sched_barrier(0);  // (few registers are left)
+          }
+        }
+      }
+    };
+
+    if constexpr (FORM != WIDE) {
+      const int step = step_of(u);
+      int kb = first_key(u);
+      // One step of 32 keys; EDGE: some of them are not seen by every row.
+      auto one = [&](auto edge) {
+        constexpr bool EDGE = decltype(edge)::value;
+        f32x4 sc[RT][2];
+#pragma unroll
+        for (int th = 0; th < 2; ++th)
+#pragma unroll
+          for (int i = 0; i < RT; ++i) {
+            f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) a = mfma16<T>(kr[th][kk], qf[i][kk], a);
+            sc[i][th] = a;
+          }
+        const bool more = kb + step < kend;
+        uint32_t bits = 0;
+        if constexpr (EDGE) {
+          hide(sc, kb);
+          // (slots past the end may hold anything, too)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int key = kb + 4 * g4 + 16 * (j >> 2) + (j & 3);
             bool bad = false;
 #pragma unroll
             for (int e = 0; e < VW; ++e) bad = bad || not_finite<T>(vr[j][e]);
-            // (any lane of this key's 16)
-            bad = (__ballot(bad) >> (16 * g4) & 0xffffu) != 0;
-            if (bad) odd |= 1u << j;
-            drop = bad;
-          }
-          if (drop) {
+            bad = bad && key < kend && key >= ctx;
+            const uint64_t all = __ballot(bad);  // (16 lanes hold a key)
 #pragma unroll
-            for (int e = 0; e < VW; ++e) vr[j][e] = 0;
+            for (int g = 0; g < 4; ++g)
+              bits |= ((all >> 16 * g & 0xffffu) != 0 ? 1u : 0u) << (16 * (j >> 2) + 4 * g + (j & 3));
+            const bool drop = key >= kend || (all >> (16 * g4) & 0xffffu) != 0;
+#pragma unroll
+            for (int e = 0; e < VW; ++e) vr[j][e] = drop ? 0u : vr[j][e];
           }
         }
-      }
-      const bool odd_any = edge && __ballot(odd != 0) != 0;
-      if (more) {
-        pages_for(kb + step);
-        load_k(kb + step);
-      }
-      u32x4 pf[RT];
-#pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        float mx = -INFINITY;
-#pragma unroll
-        for (int th = 0; th < 2; ++th)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            sc[i][th][r] *= p.scale_log2;
-            mx = fmaxf(mx, sc[i][th][r]);
-          }
-        // the reference follows the maximum only when it is passed by more than
-        // 8: a probability is then at most 2^8
-        if (__ballot(mx > m[i] + 8.f) != 0) {
-          mx = xor_max(mx);
-          const float to = fmaxf(m[i], mx);
-          const float a = m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[i] - to);
-          l[i] *= a;
-#pragma unroll
-          for (int d = 0; d < DT; ++d) o[i][d] *= a;
-          m[i] = to;
+        if (more) {
+          if (kb + step + 32 > (base + 64) * KPB) turn_pages(u, (kb + step) / KPB);
+          load_k(u, kb + step);
         }
-        const float ref = m[i] == -INFINITY ? 0.f : m[i];
+        __builtin_amdgcn_sched_barrier(0);
+        u32x4 pf[RT];
 #pragma unroll
-        for (int th = 0; th < 2; ++th)
+        for (int i = 0; i < RT; ++i) pf[i] = softmax(sc[i], i);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            sc[i][th][r] = __builtin_amdgcn_exp2f(sc[i][th][r] - ref);
-            l[i] += sc[i][th][r];
-          }
+        for (int d = 0; d < DT; ++d) {
+          // dims DT n16 + d of this lane's 8 keys
+          u32x4 vf;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const T lo = Num<T>::from_f(sc[i][e >> 1][2 * (e & 1)]);
-          const T hi = Num<T>::from_f(sc[i][e >> 1][2 * (e & 1) + 1]);
-          pf[i][e] = __builtin_bit_cast(uint16_t, lo) |
-                     static_cast<uint32_t>(__builtin_bit_cast(uint16_t, hi)) << 16;
+          for (int e = 0; e < 4; ++e)
+            vf[e] = __builtin_amdgcn_perm(vr[2 * e + 1][d >> 1], vr[2 * e][d >> 1],
+                                          d & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+          for (int i = 0; i < RT; ++i) o[i][d] = mfma16<T>(vf, pf[i], o[i][d]);
         }
+        if constexpr (EDGE) {
+          if (bits != 0) add_odd(sc, kb, bits, [&](int d, int r) { return DT * (4 * g4 + r) + d; });
+        }
+        if (more) load_v(u, kb + step);
+        __builtin_amdgcn_sched_barrier(0);
+        kb += step;
+      };
+      if (row0 < u.s.rows) {
+        while (kb < kend && kb + 32 <= ctx) one(std::false_type{});
+        while (kb < kend) one(std::true_type{});
       }
+    } else {
+      // Stages of 64 keys in LDS: [stage][K, V][key][chunk ^ key].
+      auto put = [&](int kb, int slot) {
+        char* to = lds + slot * 2 * STAGE;
+        const bool edge = kb + SK > ctx;
+#pragma unroll
+        for (int i = 0; i < SP; ++i) {
+          const int row = srow + SR * i, at = (row * CPR + (schunk ^ (row & (CPR - 1)))) * 16;
+          u32x4 v = kr[1][i];
+          if (edge) {
+            bool bad = false;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) bad = bad || not_finite<T>(v[e]);
+            bad = bad && kb + row < kend && kb + row >= ctx;
+            bad = (__ballot(bad) >> (lane & ~(CPR - 1)) & ((1ull << CPR) - 1)) != 0;
+            if (schunk == 0) odd_rows[slot][row] = bad;
+            if (bad || kb + row >= kend) v = u32x4{0u, 0u, 0u, 0u};
+          }
+          *reinterpret_cast<u32x4*>(to + at) = kr[0][i];
+          *reinterpret_cast<u32x4*>(to + STAGE + at) = v;
+        }
+      };
+      auto fetch = [&](int kb) {
+        if (kb >= kend) return;
+        if (kb + SK > (base + 64) * KPB) turn_pages(u, kb / KPB);
+        load_stage(u, kb);
+      };
+      // Fragments' places in a stage: the lane's row and swapped chunk; what is added to
+      // the row (16, 32) does not change the swap.
+      uint32_t k_at[KK], v_at[DT];
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk)
+        k_at[kk] = (n16 * CPR + ((4 * kk + g4) ^ (n16 & (CPR - 1)))) * 16;
+      // V^T of dims 16 d .., keys 4 g4 + (0 .. 3): lane 4 e + q of 16 points at row e,
+      // values 4 q ..
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
-        // dims DT n16 + d of this lane's 8 keys
-        u32x4 vf;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          vf[e] = __builtin_amdgcn_perm(vr[2 * e + 1][d >> 1], vr[2 * e][d >> 1],
-                                        d & 1 ? 0x07060302u : 0x05040100u);
-#pragma unroll
-        for (int i = 0; i < RT; ++i) o[i][d] = mfma16<T>(vf, pf[i], o[i][d]);
+        const int row = 4 * g4 + (n16 >> 2), q = n16 & 3;
+        v_at[d] = (row * CPR + ((2 * d + (q >> 1)) ^ (row & (CPR - 1)))) * 16 + 8 * (q & 1);
       }
-      if (odd_any) {
+      const bool here = row0 < u.s.rows;
+      __syncthreads();  // (the buffer is the merge's, too)
+      if (u.kbeg < kend) put(u.kbeg, 0);
+      fetch(u.kbeg + SK);
+      __syncthreads();
+      for (int kb0 = u.kbeg, slot = 0; kb0 < kend; kb0 += SK, slot ^= 1) {
+        if (here) {
+#pragma unroll 1
+          for (int sub = 0; sub < 2; ++sub) {
+            const int kb = kb0 + 32 * sub;
+            if (kb >= kend) break;
+            const char* sk = lds + slot * 2 * STAGE + 32 * sub * D * 2;
+            const SPH_LDS char* sv = (const SPH_LDS char*)(sk + STAGE);
+            f32x4 sc[RT][2];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          for (int gg = 0; gg < 4; ++gg) {
-            if ((__builtin_amdgcn_readlane(odd, 16 * gg) >> j & 1u) == 0) continue;
-            const int key = kb + 16 * (j >> 2) + 4 * gg + (j & 3);
-            const int64_t pg = trow[key / p.page];
-            const T* v = Vh + (pg >= 0 && pg < p.n_pages ? pg : 0) * p.v_sp +
-                         static_cast<int64_t>(key % p.page) * p.v_ss;
+            for (int th = 0; th < 2; ++th) {
+              u32x4 kf[KK];
 #pragma unroll
-            for (int i = 0; i < RT; ++i) {
-              const float pk = __shfl(sc[i][j >> 2][j & 3], n16 + 16 * gg, 64);
-              if (pk == 0.f) continue;
+              for (int kk = 0; kk < KK; ++kk)
+                kf[kk] = *reinterpret_cast<const u32x4*>(sk + k_at[kk] + 16 * th * D * 2);
 #pragma unroll
-              for (int d = 0; d < DT; ++d)
+              for (int i = 0; i < RT; ++i) {
+                f32x4 a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                  o[i][d][r] = fmaf(pk, Num<T>::to_f(v[DT * (4 * g4 + r) + d]), o[i][d][r]);
+                for (int kk = 0; kk < KK; ++kk) a = mfma16<T>(kf[kk], qf[i][kk], a);
+                sc[i][th] = a;
+              }
+            }
+            const bool edge = kb + 32 > ctx;
+            if (edge) hide(sc, kb);
+            u32x4 pf[RT];
+#pragma unroll
+            for (int i = 0; i < RT; ++i) pf[i] = softmax(sc[i], i);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+              u32x2 half[2];  // keys 4 g4 .. and 16 more
+#pragma unroll
+              for (int th = 0; th < 2; ++th)
+                half[th] = __builtin_bit_cast(
+                    u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                               (SPH_LDS s16x4*)(sv + v_at[d] + 16 * th * D * 2)));
+              const u32x4 vf = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3);
+#pragma unroll
+              for (int i = 0; i < RT; ++i) o[i][d] = mfma16<T>(vf, pf[i], o[i][d]);
+            }
+            if (edge) {
+              const uint32_t bits =
+                  static_cast<uint32_t>(__ballot(odd_rows[slot][32 * sub + (lane & 31)] != 0));
+              if (bits != 0) add_odd(sc, kb, bits, [&](int d, int r) { return 16 * d + 4 * g4 + r; });
             }
           }
+        }
+        if (kb0 + SK < kend) put(kb0 + SK, slot ^ 1);
+        fetch(kb0 + 2 * SK);
+        __syncthreads();
       }
-      if (more) load_v(kb + step);
     }
 
-    // The waves' states meet in LDS: rows of wave group wave % rw, from kw waves.
+    // The waves' states meet in LDS: rows of wave group wave % rw, from 4 / rw waves.
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
       l[i] += __shfl_xor(l[i], 16, 64);
@@ -500,20 +717,32 @@ __global__ void __launch_bounds__(PT) paged_attn_kernel(const PagedArgs p) {
         mg_m[wave][r] = m[i];
         mg_l[wave][r] = l[i];
       }
+      if constexpr (FORM == WIDE) {
 #pragma unroll
-      for (int rr = 0; rr < 4; ++rr)
+        for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(&merge[wave][r][16 * d + 4 * g4]) = o[i][d];
+      } else {
 #pragma unroll
-        for (int d = 0; d < DT; d += 4)
-          *reinterpret_cast<f32x4*>(&merge[wave][r][DT * (4 * g4 + rr) + d]) =
-              f32x4{o[i][d][rr], o[i][d + 1][rr], o[i][d + 2][rr], o[i][d + 3][rr]};
+        for (int rr = 0; rr < 4; ++rr)
+#pragma unroll
+          for (int d = 0; d < DT; d += 4)
+            *reinterpret_cast<f32x4*>(&merge[wave][r][DT * (4 * g4 + rr) + d]) =
+                f32x4{o[i][d][rr], o[i][d + 1][rr], o[i][d + 2][rr], o[i][d + 3][rr]};
+      }
+    }
+    if (more_units) {
+      ahead = ahead_next;
+      begin(next);
     }
     __syncthreads();
-    const bool whole = c0 == 0 && c1 == count;
-    const int live = min(R * rw, s.rows - tile0);
-    float* slot = p.part + (static_cast<int64_t>(wg) * 2 + (c0 > 0 ? 0 : 1)) * (4 * R) * (D + 2);
+    const bool whole = u.c0 == 0 && u.c1 == u.count;
+    const int rw = u.s.rw, kw = 4 / rw;
+    const int live = min(R * rw, u.s.rows - tile0);
+    const ArgPtr p = args();
+    float* slot = p->part + (static_cast<int64_t>(wg) * 2 + (u.c0 > 0 ? 0 : 1)) * (4 * R) * (D + 4);
     constexpr int LR = D / 8, RP = PT / LR;  // lanes per row, rows at a time
+#pragma unroll 1
     for (int r = t / LR; r < live; r += RP) {
-      const int w0 = r / R, rr = r % R, c = (t % LR) * 8;
+      const int w0 = r / R, rr = r % R, cc = (t % LR) * 8;
       float M = -INFINITY, sum = 0.f, acc[8] = {};
       for (int k = 0; k < kw; ++k) M = fmaxf(M, mg_m[w0 + k * rw][rr]);
       for (int k = 0; k < kw; ++k) {
@@ -522,94 +751,204 @@ __global__ void __launch_bounds__(PT) paged_attn_kernel(const PagedArgs p) {
         const float a = __builtin_amdgcn_exp2f(mg_m[w][rr] - (M == -INFINITY ? 0.f : M));
         sum = fmaf(a, mg_l[w][rr], sum);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) acc[e] = fmaf(a, merge[w][rr][c + e], acc[e]);
+        for (int e = 0; e < 8; ++e) acc[e] = fmaf(a, merge[w][rr][cc + e], acc[e]);
       }
       if (whole) {
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
         for (int e = 0; e < 8; ++e) acc[e] *= inv;
         const int row = tile0 + r;
-        store8u<T>(static_cast<T*>(p.o) +
-                       ((s.start + row / p.g) * p.nkv * p.g + h * p.g + row % p.g) * D + c,
+        store8u<T>(static_cast<T*>(p->o) +
+                       ((u.s.start + row / p->g) * p->nkv * p->g + u.h * p->g + row % p->g) * D + cc,
                    acc);
       } else {
-        float* to = slot + r * (D + 2);
-        if (c == 0) {
+        float* to = slot + r * (D + 4);
+        if (cc == 0) {
           to[0] = M;
           to[1] = sum;
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) to[2 + c + e] = acc[e];
+        store8<float>(to + 4 + cc, acc);
       }
     }
-    if (t == 0 && c0 == 0 && c1 < count) {
+    if (t == 0 && u.c0 == 0 && u.c1 < u.count) {
       // this workgroup holds the unit's beginning: the merge kernel finds here what it needs
-      const int64_t unit_end = item + count;
-      desc[0] = static_cast<int32_t>((unit_end - 1) / quota - wg) + 1;  // workgroups of the unit
-      desc[1] = h;
-      desc[2] = tile0;
-      desc[3] = live;
-      desc[4] = static_cast<int32_t>(s.start);
+      int32_t* d = p->desc + static_cast<int64_t>(wg) * 8;
+      const int parts = static_cast<int>((item + u.count - 1) / quota - wg) + 1;
+      d[0] = parts > kFewParts ? live : (live + 7) / 8;  // rows, or groups of 8, to merge
+      d[1] = parts;
+      d[2] = u.h;
+      d[3] = tile0;
+      d[4] = live;
+      d[5] = static_cast<int32_t>(u.s.start);
     }
-    item += c1 - c0;
+    item += u.c1 - u.c0;
+    if constexpr (AHEAD) {
+      u = next;
+    } else if (item < end) {
+      u = locate(item, u.b);
+      ahead = page_at(u, first_key(u) / KPB);
+      begin(u);
+    }
     __syncthreads();
   }
-}
 
-// Units that several workgroups hold: workgroup wg0's beginning and the runs of those
-// behind it, a row per wave's turn, in the order of the keys.
-template <typename T, int D, int RT>
-__global__ void __launch_bounds__(PT) paged_attn_merge(const PagedArgs p) {
-  constexpr int R4 = 4 * 16 * RT, V = D / 64;
-  const int32_t* desc = p.desc + static_cast<int64_t>(blockIdx.x) * 8;
-  const int parts = desc[0];
-  if (parts == 0) return;
-  const int h = desc[1], tile0 = desc[2], live = desc[3];
-  const int64_t start = desc[4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int r = blockIdx.y * (PT / 64) + wave; r < live; r += gridDim.y * (PT / 64)) {
-    auto part = [&](int k) {
-      const int64_t slot = (static_cast<int64_t>(blockIdx.x) + k) * 2 + (k == 0 ? 1 : 0);
-      return p.part + (slot * R4 + r) * (D + 2);
-    };
-    float M = -INFINITY;
-    for (int k = lane; k < parts; k += 64) M = fmaxf(M, part(k)[0]);
-    M = wave_reduce<MaxOp>(M);
-    const float ref = M == -INFINITY ? 0.f : M;
-    float sum = 0.f, acc[V] = {};
-#pragma unroll 8
-    for (int k = 0; k < parts; ++k) {
-      const float* x = part(k);
-      const bool nothing = x[0] == -INFINITY && x[1] == 0.f;
-      const float a = nothing ? 0.f : __builtin_amdgcn_exp2f(x[0] - ref);
-      sum = fmaf(a, x[1], sum);
-#pragma unroll
-      for (int v = 0; v < V; ++v) acc[v] = fmaf(a, nothing ? 0.f : x[2 + V * lane + v], acc[v]);
+  {  // rows that belong to no sequence
+    const ArgPtr p = args();
+    const int64_t none = 0;
+    const int64_t before = min(max(p->starts[0], none), p->tokens);
+    const int64_t behind = min(max(p->starts[batch], none), p->tokens);
+    const int64_t rest = before + p->tokens - behind;
+    const int64_t width = static_cast<int64_t>(p->g) * p->nkv * D;
+    for (int64_t x = wg; x < rest; x += gridDim.x) {
+      T* o = static_cast<T*>(p->o) + (x < before ? x : behind + x - before) * width;
+      const float z[8] = {};
+      for (int64_t c = t * 8; c < width; c += PT * 8) store8u<T>(o + c, z);
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int row = tile0 + r;
-    T* o = static_cast<T*>(p.o) +
-           ((start + row / p.g) * p.nkv * p.g + h * p.g + row % p.g) * D + V * lane;
-#pragma unroll
-    for (int v = 0; v < V; ++v) o[v] = Num<T>::from_f(acc[v] * inv);
   }
 }
 
-// Groups of 16 rows per wave: 1 where a sequence's rows fit 16 on average.
-int row_groups(int64_t tokens, int64_t batch, int64_t g) {
-  return tokens * g <= 16 * batch ? 1 : 2;
+// Units that several workgroups hold: the one in which a unit begins has its first part
+// in its second slot, those behind it have theirs in their first.  8 groups of D / 4
+// lanes: with few parts each takes a row, else all of them one row, a run of the parts
+// each, always in the same order.  Every workgroup looks all of them up and takes
+// its turn.  (Two workgroups per unit and a row per wave took 180 of 330 us for one
+// sequence of 131072 keys with 16 new tokens: 8 units of 64 parts and 64 rows.)
+template <typename T, int D, int FORM>
+__global__ void __launch_bounds__(PT) paged_attn_merge(const PagedArgs p, int grid) {
+  constexpr int R4 = 4 * rows_of(FORM), L = D / 4, NB = 8;
+  constexpr int G8 = 8;  // groups of lanes
+  __shared__ int first[kMaxGrid + 1];  // tasks before a workgroup's
+  __shared__ int info[kMaxGrid][5];
+  __shared__ int scan[4];
+  __shared__ float ms[G8], ls[G8];
+  __shared__ __attribute__((aligned(16))) float os[G8][D];
+  const int t = threadIdx.x, lane = t & 63, wave = uni(t >> 6);
+  int total = 0;
+  for (int g0 = 0; g0 < grid; g0 += PT) {
+    int v = 0;
+    if (g0 + t < grid) {
+      const int32_t* d = p.desc + static_cast<int64_t>(g0 + t) * 8;
+      v = d[0];
+#pragma unroll
+      for (int i = 0; i < 5; ++i) info[g0 + t][i] = d[1 + i];
+    }
+    int x = v;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int y = __shfl_up(x, off, 64);
+      if (lane >= off) x += y;
+    }
+    if (lane == 63) scan[wave] = x;
+    __syncthreads();
+    int base = total;
+    for (int w = 0; w < 4; ++w) {
+      if (w < wave) base += scan[w];
+      total += scan[w];
+    }
+    if (g0 + t < grid) first[g0 + t] = base + x - v;
+    __syncthreads();
+  }
+  total = uni(total);
+  const int g = t / L, c = (t % L) * 4;  // (D = 64: 16 groups, the last 8 idle)
+  for (int task = blockIdx.x; task < total; task += gridDim.x) {
+    int lo = 0, hi = grid;  // the last workgroup with first <= task: it has tasks
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (uni(first[mid]) <= task) lo = mid;
+      else hi = mid;
+    }
+    const int parts = uni(info[lo][0]), h = info[lo][1], tile0 = info[lo][2], live = info[lo][3];
+    const bool few = parts <= kFewParts;
+    const int r = (task - uni(first[lo])) * (few ? 8 : 1) + (few ? g : 0);
+    const int k0 = few ? 0 : g, dk = few ? 1 : G8;
+    float M = -INFINITY, sum = 0.f, acc[4] = {};
+    const bool mine = g < G8 && r < live;
+    if (mine) {
+      for (int k1 = k0; k1 < parts; k1 += dk * NB) {
+        float m[NB], l[NB];
+        f32x4 o[NB];
+#pragma unroll
+        for (int k = 0; k < NB; ++k) {
+          const int at = min(k1 + dk * k, parts - 1);
+          const int64_t slot = (static_cast<int64_t>(lo) + at) * 2 + (at == 0 ? 1 : 0);
+          const float* x = p.part + (slot * R4 + r) * (D + 4);
+          m[k] = x[0];
+          l[k] = x[1];
+          o[k] = *reinterpret_cast<const f32x4*>(x + 4 + c);
+        }
+        float to = M;
+#pragma unroll
+        for (int k = 0; k < NB; ++k) {
+          if (k1 + dk * k >= parts) {
+            m[k] = -INFINITY;
+            l[k] = 0.f;
+          }
+          to = fmaxf(to, m[k]);
+        }
+        const float ref = to == -INFINITY ? 0.f : to;
+        const float a = M == -INFINITY ? (sum == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(M - ref);
+        sum *= a;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] *= a;
+#pragma unroll
+        for (int k = 0; k < NB; ++k) {
+          if (m[k] == -INFINITY && l[k] == 0.f) continue;  // saw nothing
+          const float w = __builtin_amdgcn_exp2f(m[k] - ref);
+          sum = fmaf(w, l[k], sum);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[e] = fmaf(w, o[k][e], acc[e]);
+        }
+        M = to;
+      }
+    }
+    if (!few) {
+      if (g < G8) {
+        if (c == 0) {
+          ms[g] = M;
+          ls[g] = sum;
+        }
+        *reinterpret_cast<f32x4*>(&os[g][c]) = f32x4{acc[0], acc[1], acc[2], acc[3]};
+      }
+      __syncthreads();
+      M = -INFINITY;
+      for (int k = 0; k < G8; ++k) M = fmaxf(M, ms[k]);
+      const float ref = M == -INFINITY ? 0.f : M;
+      sum = 0.f;
+      for (int e = 0; e < 4; ++e) acc[e] = 0.f;
+      for (int k = 0; k < G8; ++k) {
+        if (ms[k] == -INFINITY && ls[k] == 0.f) continue;
+        const float a = __builtin_amdgcn_exp2f(ms[k] - ref);
+        sum = fmaf(a, ls[k], sum);
+        for (int e = 0; e < 4; ++e) acc[e] = fmaf(a, os[k][c + e], acc[e]);
+      }
+      __syncthreads();
+    }
+    if (mine && (few || g == 0)) {
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      const int at = tile0 + r;
+      T* to = static_cast<T*>(p.o) + ((static_cast<int64_t>(info[lo][4]) + at / p.g) * p.nkv * p.g +
+                                      h * p.g + at % p.g) * D + c;
+      u32x2 w;
+      w[0] = pack2<T>(acc[0] * inv, acc[1] * inv);
+      w[1] = pack2<T>(acc[2] * inv, acc[3] * inv);
+      *reinterpret_cast<u32x2_any*>(to) = w;
+    }
+  }
+}
+
+// The form for sequences of this many rows on average.
+int form_of(int64_t tokens, int64_t batch, int64_t g) {
+  return tokens * g <= 16 * batch ? DECODE : tokens * g <= 64 * batch ? TREE : WIDE;
 }
 // Workgroups: what the chip holds at once, or fewer when the shapes cannot hold as many items.
 int64_t paged_grid(int64_t tokens, int64_t batch, int64_t n_kv, int64_t g, int64_t max_keys) {
-  const int rt = row_groups(tokens, batch, g);
-  const int64_t most = rt == 1 ? 768 : 512;
-  const int64_t tiles = std::min(tokens, tokens * g / (16 * rt) + batch);
+  const int64_t tiles = std::min(tokens, tokens * g / rows_of(form_of(tokens, batch, g)) + batch);
   const double items = static_cast<double>(tiles) * n_kv *
                        static_cast<double>(std::max<int64_t>(1, ceil_div(max_keys, kItemKeys)));
-  return items < most ? std::max<int64_t>(1, static_cast<int64_t>(items)) : most;
+  return items < kMaxGrid ? std::max<int64_t>(1, static_cast<int64_t>(items)) : kMaxGrid;
 }
 int64_t paged_part_floats(int64_t tokens, int64_t batch, int64_t g, int64_t head_dim) {
-  return 2 * 64 * row_groups(tokens, batch, g) * (head_dim + 2);
+  return 2 * 4 * rows_of(form_of(tokens, batch, g)) * (head_dim + 4);
 }
 
 }  // namespace
@@ -655,6 +994,8 @@ extern "C" int sph_paged_attention(
   SPH_REQUIRE(page_size < (1LL << 30) && n_pages < (1LL << 31) && table_width < (1LL << 30) &&
                   table_width * page_size < (1LL << 30),
               SPH_ERR_TOO_LARGE, "paged attention: at most 2^30 keys a sequence, 2^31 pages");
+  SPH_REQUIRE(k_stride_s >= 0 && v_stride_s >= 0 && k_stride_s < (1 << 26) && v_stride_s < (1 << 26),
+              SPH_ERR_TOO_LARGE, "paged attention: rows of a page at most 2^26 elements apart");
   SPH_REQUIRE(q != nullptr && o != nullptr && seq_lens != nullptr && q_starts != nullptr &&
                   (block_table != nullptr || table_width == 0) &&
                   ((k_cache != nullptr && v_cache != nullptr) || n_pages == 0),
@@ -668,7 +1009,7 @@ extern "C" int sph_paged_attention(
                   reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
               SPH_ERR_INVALID_ARG, "paged attention: workspace too small or not 16-byte aligned");
   const int64_t g = n_heads / n_kv_heads;
-  const int rt = row_groups(tokens, batch, g);
+  const int form = form_of(tokens, batch, g);
   const int64_t grid = paged_grid(tokens, batch, n_kv_heads, g, max_keys);
   PagedArgs a{};
   a.q = q;
@@ -702,20 +1043,22 @@ extern "C" int sph_paged_attention(
   a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + grid * 32);
   a.err = error_word;
   hipStream_t st = as_stream(stream);
+  const unsigned mgrid = static_cast<unsigned>(std::min<int64_t>(1024, tokens * n_heads));
   const size_t lds = static_cast<size_t>(batch + 1) * 8;
   auto go = [&](auto tt, auto dd, auto rr, auto pp) {
     using T = decltype(tt);
-    constexpr int D = decltype(dd)::value, RT = decltype(rr)::value;
-    paged_attn_kernel<T, D, RT, decltype(pp)::value><<<dim3(grid), PT, lds, st>>>(a);
-    if (grid > 1) paged_attn_merge<T, D, RT><<<dim3(grid, 2), PT, 0, st>>>(a);
+    constexpr int D = decltype(dd)::value, FORM = decltype(rr)::value;
+    paged_attn_kernel<T, D, FORM, decltype(pp)::value><<<dim3(grid), PT, lds, st>>>(a);
+    if (grid > 1) paged_attn_merge<T, D, FORM><<<dim3(mgrid), PT, 0, st>>>(a, static_cast<int>(grid));
   };
   auto by_page = [&](auto tt, auto dd, auto rr) {
     if (page_size % 16 == 0) go(tt, dd, rr, std::true_type{});
     else go(tt, dd, rr, std::false_type{});
   };
   auto by_rows = [&](auto tt, auto dd) {
-    if (rt == 1) by_page(tt, dd, std::integral_constant<int, 1>{});
-    else by_page(tt, dd, std::integral_constant<int, 2>{});
+    if (form == DECODE) by_page(tt, dd, std::integral_constant<int, DECODE>{});
+    else if (form == TREE) by_page(tt, dd, std::integral_constant<int, TREE>{});
+    else by_page(tt, dd, std::integral_constant<int, WIDE>{});
   };
   auto by_dim = [&](auto tt) {
     if (head_dim == 128) by_rows(tt, std::integral_constant<int, 128>{});

@@ -599,6 +599,33 @@ def test_sample_special_values(dtype, device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("vocab", [40, 4097, 20000])
+def test_sample_borders_of_the_filters(vocab, device):
+    """min-p through 0, logits far from 0 beside a small temperature, k around the number of
+    threads, filters that meet at one value."""
+    l = rand((16, vocab), vocab, 1.0, torch.float32)
+    l[:, 3] = 0.0
+    l[:, 5] = -0.0
+    l[0:4, 7] = 3.0
+    l[4:8] = 1e6 + torch.round(l[4:8])
+    l[8:12] = torch.round(l[8:12] * 2) / 2
+    l[12:] = -1e-30 * torch.rand(4, vocab)
+    u = uniforms(16, vocab)
+    exact = torch.full((16,), math.exp(-3.0))  # (float: 0 passes or not by its last bit)
+    for m in (exact, torch.nextafter(exact, torch.tensor(1.0)), torch.full((16,), 0.3)):
+        check_sample(l, device, u, m=m)
+        check_sample(l, device, u, m=m, k=30, p=0.9)
+        check_sample(l, device, u, m=m, p=0.7, t=0.5)
+    for t in (1e-3, 1e-10, 30.0):
+        check_sample(l, device, u, t=t)
+        check_sample(l, device, u, t=t, p=0.6)
+        check_sample(l, device, u, t=t, k=700, p=0.8)
+    for k in (39, 512, 1023, 1024, 1025, 4096):
+        check_sample(l, device, u, k=k)
+        check_sample(l, device, u, k=k, p=0.97, m=0.02)
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_sample_bounds_of_the_random_number(device):
     l = torch.tensor([[0.0, 1.0, -INF, 2.0, -INF]]).expand(5, 5).contiguous()
     u = torch.tensor([0.0, 1.0, 5.0, -3.0, NAN])

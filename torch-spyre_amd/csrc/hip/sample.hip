@@ -15,16 +15,27 @@
 // A row has as many borders between tokens as it has tokens, so a relative error
 // e of the weights turns over one drawn token in 1 / (V e): 32-bit weights would err once
 // in some hundred rows.  Weights are therefore formed in 64 bits and held as
-// whole multiples of 2^-shift, shift = 62 - log2 V: their sums in 64-bit
+// whole multiples of 2^-shift, shift = 62 - log2 V (at most 51): their sums in 64-bit
 // integers are exact and do not depend on the order of additions.
 //
-// One workgroup per row.  A cut (top-k by counts, top-p by weights) is found by
-// histograms: first over 2048 equal steps of the logit between the maximum and the least logit
-// that has weight (each step holds few tokens, so the atomics seldom meet), then
-// within the step that the cut falls into, over ranges of the ordered bit patterns until
-// one pattern is left.  What is cut is described by that pattern and by how
-// many of the tokens with it stay.  The draw needs the sums of all 512-token
-// pieces and then one wave in the piece that holds the token.
+// A weight is formed in ten 64-bit operations (2^y by a table of 32 steps and the series to
+// the fifth power).  That is what bounds the kernel: rows are read at the speed of the
+// cache, and a weight for each of 49155 tokens takes one workgroup 8 us (the
+// library's exp and a conversion to integers: 23).  So as few as possible are formed:
+//
+//   * top-k of at most 1024: k of the 1024 threads' own maxima reach down to some value,
+//     so the k largest do; what reaches it is listed in LDS (hardly more than k),
+//     ranked by counting, and top-p, min-p and the draw run over the k first.
+//   * else a cut (top-k by counts, top-p by weights) is found by histograms: over
+//     2048 equal steps of the logit below the maximum (each holds few tokens, so the
+//     atomics seldom meet), then over the ordered bit patterns of the step that the cut
+//     falls into.  What is cut is described by that pattern and by how many of the
+//     tokens with it stay; what stays is listed if there is room.  The draw needs
+//     the sums of all 512-token pieces and then one wave in the piece that holds the token.
+//
+// One workgroup per row, which reads it again where it is needed, two turns of loads ahead.
+#include <algorithm>
+
 #include "sph_common.h"
 
 namespace sph {
@@ -34,9 +45,10 @@ constexpr int ST = 1024;             // threads
 constexpr int WAVES = ST / 64;
 constexpr int TILE = ST * 8;         // tokens of a turn of the workgroup
 constexpr int BINS = 2048;
-constexpr int LIST = 2048;           // tokens of a step that are kept in LDS
+constexpr int LIST = 4096;           // tokens that are listed in LDS
 constexpr int64_t kMaxVocab = 1 << 20;
-static_assert(kMaxVocab / 512 <= BINS, "a piece per entry of the scan");
+constexpr int MAX_PIECES = kMaxVocab / 512;
+static_assert(MAX_PIECES <= BINS, "a piece per entry of the histogram");
 
 struct SampleArgs {
   const void* logits;
@@ -59,70 +71,115 @@ __device__ inline float value_of(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-struct Row {
-  float top;        // M (0 where it is +inf)
-  bool top_inf;
-  double rate;      // 1 / t
-  double unit;      // 2^shift
-  __device__ float clean(float f) const {  // (+ 0: one zero)
-    if (top_inf) return f == INFINITY ? 0.f : -INFINITY;
-    return f != f ? -INFINITY : f + 0.f;
-  }
-  __device__ double weight(float f) const {
-    return f == -INFINITY ? 0.0 : exp((static_cast<double>(f) - top) * rate);
-  }
-  __device__ uint64_t units(double w) const { return static_cast<uint64_t>(fma(w, unit, 0.5)); }
-};
-
 struct Shared {
   uint64_t hist[BINS];
   uint32_t count[BINS];
   float list[LIST];
+  int list_at[LIST];
+  double exp2[32];  // 2^(j / 32 + shift)
   uint64_t wave64[WAVES];
-  float wmax[WAVES], wmin[WAVES];
+  float wmax[WAVES];
   int widx[WAVES];
   uint32_t listed, kmin, kmax;
   int bin;
   uint64_t before, total;
 };
 
-// Inclusive sums of a 64-bit value over the workgroup's threads; total: of all.
+// A row's weights.  Values are clean: NaN counts as -inf, there is one zero, and
+// beside +inf (mapped to 0) there is only -inf.
+struct Row {
+  float top;     // M
+  double rate;   // 32 log2 e / t
+  const double* table;
+  // 32 log2 of the weight; at least -3300, where it has none (NaN: -inf times 0)
+  __device__ double log_of(float f) const {
+    return fmax((static_cast<double>(f) - top) * rate, -3300.0);
+  }
+  // 2^(y / 32 + shift) to the nearest whole number: y = 32 n + j + r, |r| <= 1/2, by a sum with 1.5 2^52, whose low bits then hold 32 n + j; the series of 2^(r / 32) to
+  // the fifth power (the next term is 2e-15 at most); n joins the exponent, and a sum with
+  // 2^52 leaves the whole number in the low bits (shift <= 51).
+  __device__ uint64_t weight(float f) const {
+    constexpr double L = 0.021660849392498290;  // ln 2 / 32
+    const double y = log_of(f);
+    const double s = y + 0x1.8p52;
+    const int k = static_cast<int>(__builtin_bit_cast(uint64_t, s));
+    const double r = y - (s - 0x1.8p52);
+    double q = L * L * L * L * L / 120;
+    q = fma(q, r, L * L * L * L / 24);
+    q = fma(q, r, L * L * L / 6);
+    q = fma(q, r, L * L / 2);
+    q = fma(q, r, L);
+    const double t = table[k & 31];
+    uint64_t bits = __builtin_bit_cast(uint64_t, fma(t, q * r, t));
+    bits += static_cast<uint64_t>(static_cast<uint32_t>(k >> 5) << 20) << 32;
+    const double x = __builtin_bit_cast(double, bits) + 0x1p52;
+    return __builtin_bit_cast(uint64_t, x) & 0xfffffffffffffull;
+  }
+};
+
+// Inclusive sums over a wave, by lane moves inside rows of 16 and broadcasts of their ends.
+template <int CTRL, int ROWS>
+__device__ inline uint64_t moved(uint64_t v) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), CTRL, ROWS, 0xf, false);
+  return static_cast<uint64_t>(hi) << 32 | lo;
+}
+__device__ inline uint64_t wave_scan(uint64_t v) {
+  v += moved<0x111, 0xf>(v);
+  v += moved<0x112, 0xf>(v);
+  v += moved<0x114, 0xf>(v);
+  v += moved<0x118, 0xf>(v);
+  v += moved<0x142, 0xa>(v);
+  v += moved<0x143, 0xc>(v);
+  return v;
+}
+__device__ inline uint64_t last_lane(uint64_t v) {
+  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(v), 63);
+  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), 63);
+  return static_cast<uint64_t>(hi) << 32 | lo;
+}
+// Over the workgroup's threads; total: of all.
 __device__ inline uint64_t scan64(uint64_t v, Shared& s, uint64_t& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const uint64_t y = __shfl_up(v, off, 64);
-    if (lane >= off) v += y;
-  }
+  v = wave_scan(v);
   __syncthreads();
   if (lane == 63) s.wave64[wave] = v;
   __syncthreads();
-  uint64_t base = 0;
-  total = 0;
-  for (int w = 0; w < WAVES; ++w) {
-    if (w < wave) base += s.wave64[w];
-    total += s.wave64[w];
-  }
-  return base + v;
+  const uint64_t all = wave_scan(lane < WAVES ? s.wave64[lane] : 0);
+  total = last_lane(all);
+  const uint32_t lo = __shfl(static_cast<int>(all), max(wave - 1, 0), 64);
+  const uint32_t hi = __shfl(static_cast<int>(all >> 32), max(wave - 1, 0), 64);
+  return v + (wave == 0 ? 0 : static_cast<uint64_t>(hi) << 32 | lo);
 }
 
-// The first entry of s.hist at which cross(sum up to it) holds: s.bin, with the sum before it
-// in s.before and all in s.total.  Every thread calls it; cross holds for the whole sum.
+// The first entry of s.hist at which cross(sum up to it, sum of all) holds: s.bin, with the
+// sum before it in s.before and all in s.total.  Every thread calls it; without such an entry
+// s.bin stays as it is.
 template <typename F>
 __device__ inline void find(Shared& s, F cross) {
   const int t = threadIdx.x;
   const uint64_t a = s.hist[2 * t], b = s.hist[2 * t + 1];
   uint64_t total;
   const uint64_t incl = scan64(a + b, s, total), e0 = incl - a - b, e1 = e0 + a;
-  if (cross(e1) && (t == 0 || !cross(e0))) {
+  if (cross(e1, total) && (t == 0 || !cross(e0, total))) {
     s.bin = 2 * t;
     s.before = e0;
-  } else if (cross(incl) && !cross(e1)) {
+  } else if (cross(incl, total) && !cross(e1, total)) {
     s.bin = 2 * t + 1;
     s.before = e1;
   }
   if (t == 0) s.total = total;
   __syncthreads();
+}
+
+__device__ inline void add(uint64_t* to, uint64_t v) {
+  atomicAdd(reinterpret_cast<unsigned long long*>(to), static_cast<unsigned long long>(v));
+}
+
+// The number that the sums have to exceed.
+__device__ inline uint64_t target_of(double u, uint64_t total) {
+  const uint64_t x = u > 0.0 ? static_cast<uint64_t>(fmin(u, 1.0) * static_cast<double>(total)) : 0;
+  return min(x, total - 1);
 }
 
 template <typename T>
@@ -132,313 +189,415 @@ __global__ void __launch_bounds__(ST) sample_kernel(const SampleArgs p) {
   const int64_t r = blockIdx.x;
   const T* x = static_cast<const T*>(p.logits) + r * p.ld;
   const int V = p.vocab;
+  const float temp = p.temperature != nullptr ? p.temperature[r] : 1.f;
+  const int64_t k = p.top_k != nullptr ? p.top_k[r] : 0;
+  const float share = p.top_p != nullptr ? p.top_p[r] : 1.f;
+  const float min_p = p.min_p != nullptr ? p.min_p[r] : 0.f;
+  const double u = p.uniform[r];
+  if (t < 32) s.exp2[t] = exp2(t / 32.0 + p.shift);
 
-  // f(tile, values, index of the first) for this thread's 8 tokens of every turn
+  // f(index of the turn's first, values, index of the first) for this thread's 8
+  // tokens of every turn; past the row's end the values are -inf
+  auto load = [&](int i, float (&v)[8]) {
+    if (i + 8 <= V) load8u<T>(x + i, v);
+    else load8_partial<T>(x + i, i < V ? V - i : 0, -INFINITY, v);
+  };
   auto groups = [&](auto f) {
-    for (int i0 = 0; i0 < V; i0 += TILE) {
-      const int i = i0 + t * 8;
-      float v[8];
-      if (i + 8 <= V) load8u<T>(x + i, v);
-      else load8_partial<T>(x + i, i < V ? V - i : 0, -INFINITY, v);
-      f(i0, v, i);
+    float a[8], b[8];
+    load(t * 8, a);
+    load(TILE + t * 8, b);
+    for (int i0 = 0; i0 < V; i0 += 2 * TILE) {
+      f(i0, a, i0 + t * 8);
+      load(i0 + 2 * TILE + t * 8, a);
+      if (i0 + TILE >= V) break;
+      f(i0 + TILE, b, i0 + TILE + t * 8);
+      load(i0 + 3 * TILE + t * 8, b);
     }
   };
 
-  // ---- maximum, its first index, least finite value
-  float mx = -INFINITY, mn = INFINITY;
-  int at = 0x7fffffff;
-  groups([&](int, const float (&v)[8], int i) {
+  // ---- maximum (of this thread first); a row at no temperature: its first index
+  float mine = -INFINITY;
+  if (!(temp > 0.f)) {
+    int at = 0x7fffffff;
+    groups([&](int, const float (&v)[8], int i) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (v[e] > mx) {
-        mx = v[e];
-        at = i + e;
+      for (int e = 0; e < 8; ++e)
+        if (v[e] > mine) {
+          mine = v[e];
+          at = i + e;
+        }
+    });
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+      const float om = __shfl_xor(mine, off, 64);
+      const int oa = __shfl_xor(at, off, 64);
+      if (om > mine || (om == mine && oa < at)) {
+        mine = om;
+        at = oa;
       }
-      if (v[e] > -INFINITY) mn = fminf(mn, v[e]);
     }
-  });
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    const float om = __shfl_xor(mx, off, 64);
-    const int oa = __shfl_xor(at, off, 64);
-    if (om > mx || (om == mx && oa < at)) {
-      mx = om;
-      at = oa;
+    if (lane == 0) {
+      s.wmax[wave] = mine;
+      s.widx[wave] = at;
     }
-    mn = fminf(mn, __shfl_xor(mn, off, 64));
-  }
-  if (lane == 0) {
-    s.wmax[wave] = mx;
-    s.widx[wave] = at;
-    s.wmin[wave] = mn;
-  }
-  __syncthreads();
-  for (int w = 0; w < WAVES; ++w) {
-    if (s.wmax[w] > mx || (s.wmax[w] == mx && s.widx[w] < at)) {
-      mx = s.wmax[w];
-      at = s.widx[w];
-    }
-    mn = fminf(mn, s.wmin[w]);
-  }
-  const float temp = p.temperature != nullptr ? p.temperature[r] : 1.f;
-  if (mx == -INFINITY || !(temp > 0.f)) {
-    if (t == 0) p.tokens[r] = mx == -INFINITY ? -1 : at;
+    __syncthreads();
+    for (int w = 0; w < WAVES; ++w)
+      if (s.wmax[w] > mine || (s.wmax[w] == mine && s.widx[w] < at)) {
+        mine = s.wmax[w];
+        at = s.widx[w];
+      }
+    if (t == 0) p.tokens[r] = mine == -INFINITY ? -1 : at;
     return;
   }
+  groups([&](int, const float (&v)[8], int) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) mine = fmaxf(mine, v[e]);
+  });
+  {
+    const float m = wave_reduce<MaxOp>(mine);
+    if (lane == 0) s.wmax[wave] = m;
+  }
+  for (int i = t; i < BINS; i += ST) {
+    s.hist[i] = 0;
+    s.count[i] = 0;
+  }
+  if (t == 0) s.listed = 0;
+  __syncthreads();
+  float mx = s.wmax[0];
+  for (int w = 1; w < WAVES; ++w) mx = fmaxf(mx, s.wmax[w]);
+  if (mx == -INFINITY) {
+    if (t == 0) p.tokens[r] = -1;
+    return;
+  }
+  const bool top_inf = mx == INFINITY;
+  auto clean = [&](float f) {
+    if (top_inf) return f == INFINITY ? 0.f : -INFINITY;
+    return f != f ? -INFINITY : f + 0.f;
+  };
   Row row;
-  row.top_inf = mx == INFINITY;
-  row.top = row.top_inf ? 0.f : mx;
-  row.rate = 1.0 / static_cast<double>(temp);
-  row.unit = ldexp(1.0, p.shift);
+  row.top = top_inf ? 0.f : mx + 0.f;
+  row.rate = 32 * 1.4426950408889634074 / static_cast<double>(temp);
+  row.table = s.exp2;
   // From 44 t below the maximum on a weight is less than half a unit.
-  const float range = row.top_inf ? 0.f : fminf(mx - mn, 44.f * temp);
+  const float range = 44.f * temp;
   const float steps = range > 0.f && range < INFINITY ? (BINS - 1) / range : 0.f;
   auto step_of = [&](float f) {
     return static_cast<int>(fminf((row.top - f) * steps, static_cast<float>(BINS - 1)));
   };
+  // The least value that min-p lets through (the largest weight is 1), to the last bit.
+  float least = -INFINITY;
+  if (min_p > 0.f) {
+    const double y = 32 * log2(static_cast<double>(fminf(min_p, 1.f)));
+    uint32_t lo = key_of(-3.402823466e38f), hi = key_of(row.top);  // (the largest passes)
+    while (lo < hi) {  // 64 places at a time
+      const uint32_t gap = (hi - lo) / 64 + 1, at = min(lo + lane * gap, hi);
+      const uint64_t pass = __ballot(row.log_of(value_of(at)) >= y);
+      const uint32_t l = pass != 0 ? __builtin_ctzll(pass) : 64;
+      hi = pass != 0 ? min(lo + l * gap, hi) : hi;
+      lo = l == 0 ? lo : lo + (l - 1) * gap + 1;
+    }
+    least = value_of(lo) + 0.f;
+  }
+  // f(value, index) for the tokens from lo on, lo > -inf.  (One comparison for 8 that are
+  // below; values as they are in memory, so NaN and, beside +inf, others may come.)
+  auto tokens_from = [&](float lo, auto f) {
+    groups([&](int, const float (&v)[8], int i) {
+      float m = v[0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) m = fmaxf(m, v[e]);
+      if (!(m >= lo)) return;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (v[e] >= lo) f(v[e], i + e);
+    });
+  };
+  auto put = [&](float f, int i) {
+    const uint32_t n = atomicAdd(&s.listed, 1u);
+    if (n < LIST) {
+      s.list[n] = f;
+      s.list_at[n] = i;
+    }
+  };
+  auto clear = [&] {
+    __syncthreads();
+    for (int i = t; i < BINS; i += ST) s.hist[i] = 0;
+    if (t == 0) s.listed = 0;
+    __syncthreads();
+  };
+
+  // ---- few tokens stay: in order by counting
+  if (k > 0 && k <= ST) {
+    // k of the threads' maxima reach the least of those up to some step
+    if (clean(mine) > -INFINITY) add(&s.hist[step_of(clean(mine))], 1);
+    if (t == 0) s.kmin = 0xffffffffu;
+    __syncthreads();
+    find(s, [&](uint64_t sum, uint64_t all) { return sum >= min(all, static_cast<uint64_t>(k)); });
+    const bool enough = s.total >= static_cast<uint64_t>(k);
+    const float c = clean(mine);
+    if (c > -INFINITY && step_of(c) <= s.bin) atomicMin(&s.kmin, key_of(c));
+    __syncthreads();
+    // (fewer maxima than k: some threads have no tokens, so every token may be among the first)
+    const float from = top_inf ? INFINITY : enough ? value_of(s.kmin) : -3.402823466e38f;
+    if (enough || V <= LIST) tokens_from(from, [&](float f, int i) { put(f + 0.f, i); });
+    __syncthreads();
+    const uint32_t n = s.listed;
+    if ((enough || V <= LIST) && n <= ST) {
+      float f = -INFINITY;
+      int at = 0x7fffffff;
+      uint32_t rank = ST;
+      if (t < static_cast<int>(n)) {
+        f = s.list[t];
+        at = s.list_at[t];
+        rank = 0;
+        for (uint32_t j = 0; j < n; ++j) {
+          const float g = s.list[j];
+          rank += g > f || (g == f && s.list_at[j] < at);
+        }
+      }
+      __syncthreads();
+      if (rank < ST) {
+        s.list[ST + rank] = f;
+        s.list_at[ST + rank] = at;
+      }
+      __syncthreads();
+      const bool in = t < static_cast<int>(n) && t < k;
+      f = in ? s.list[ST + t] : -INFINITY;
+      at = in ? s.list_at[ST + t] : -1;
+      uint64_t w = in ? row.weight(top_inf ? 0.f : f) : 0;
+      uint64_t total;
+      const uint64_t upto = scan64(w, s, total);
+      const double want = fmax(static_cast<double>(share), 0.0) * static_cast<double>(total);
+      if (share < 1.f && t > 0 && !(static_cast<double>(upto - w) < want)) w = 0;
+      if (!top_inf && f < least) w = 0;
+      __syncthreads();
+      s.hist[t] = w;
+      const uint64_t mass = scan64(w, s, total);
+      const uint32_t m = __popcll(__ballot(w != 0));  // (what stays are the first)
+      if (lane == 0) s.widx[wave] = m;
+      __syncthreads();
+      int stay = 0;
+      for (int i = 0; i < WAVES; ++i) stay += s.widx[i];
+      (void)mass;
+      const uint64_t target = target_of(u, total);
+      if (w != 0) {
+        uint64_t upper = 0;  // weight up to this token by index
+        for (int j = 0; j < stay; ++j) upper += s.list_at[ST + j] <= at ? s.hist[j] : 0;
+        if (upper > target && upper - w <= target) p.tokens[r] = at;
+      }
+      return;
+    }
+    clear();
+  }
 
   // What stays: keys above cut, and the first `ties` tokens of those equal to it.
   uint32_t cut = key_of(-INFINITY);
   uint32_t ties = 0;
 
-  // Moves the cut up to where cross(sum of amount over the order) first holds; amount(f) of a
-  // token, `whole` times it for the tokens at the cut.  left(before, amount of one,
-  // how many) gives the number that stays of the tokens where it holds.
-  auto move_cut = [&](auto amount, auto cross, auto left) {
-    // steps of the logit
-    auto clear = [&] {
-      __syncthreads();
-      for (int i = t; i < BINS; i += ST) s.hist[i] = 0;
-      if (t == 0) {
-        s.listed = 0;
-        s.kmin = 0xffffffffu;
-        s.kmax = 0;
-      }
-      __syncthreads();
-    };
+  // Moves the cut to the first place in the order at which the amounts summed up to it
+  // reach want_of(all of them); amount(f) of a token.  Of the tokens with the value at that
+  // place as many stay as it takes.  (s.hist and s.listed are 0.)
+  auto move_cut = [&](auto amount, auto want_of) {
     const float cutv = value_of(cut);
-    const bool have = ties > 0;
-    clear();
+    const uint32_t low = cut, low_ties = ties;
     groups([&](int, const float (&v)[8], int) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float f = row.clean(v[e]);
-        if (f > -INFINITY && key_of(f) > cut) {
-          const uint64_t a = amount(f);
-          if (a != 0) atomicAdd(reinterpret_cast<unsigned long long*>(&s.hist[step_of(f)]), a);
-        }
+        const float f = clean(v[e]);
+        const uint64_t a = f > cutv ? amount(f) : 0;
+        if (a != 0) add(&s.hist[step_of(f)], a);
       }
     });
-    if (have && t == 0)
-      atomicAdd(reinterpret_cast<unsigned long long*>(&s.hist[step_of(cutv)]), amount(cutv) * ties);
+    if (low_ties > 0 && t == 0) add(&s.hist[step_of(cutv)], amount(cutv) * low_ties);
     __syncthreads();
-    find(s, [&](uint64_t sum) { return cross(sum, uint64_t{0}); });
-    if (!cross(s.total, uint64_t{0})) return;  // all of it stays
+    find(s, [&](uint64_t sum, uint64_t all) { return static_cast<double>(sum) >= want_of(all); });
+    const double want = want_of(s.total);
+    if (static_cast<double>(s.total) < want) {  // all of it stays
+      clear();
+      return;
+    }
     const int bin = s.bin;
     uint64_t before = s.before;
-    const uint32_t low = cut;
-    clear();
-    // the keys of that step
-    auto in_step = [&](float f) {
-      return f > -INFINITY && key_of(f) > low && step_of(f) == bin && amount(f) != 0;
-    };
-    groups([&](int, const float (&v)[8], int) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float f = row.clean(v[e]);
-        if (in_step(f)) {
-          const uint32_t n = atomicAdd(&s.listed, 1u);
-          if (n < LIST) s.list[n] = f;
-          atomicMin(&s.kmin, key_of(f));
-          atomicMax(&s.kmax, key_of(f));
-        }
-      }
-    });
-    const bool cut_here = have && step_of(cutv) == bin;
     __syncthreads();
-    uint32_t lo = s.kmin, hi = s.kmax;
-    const uint32_t listed = s.listed;
+    if (t == 0) {
+      s.kmin = 0xffffffffu;
+      s.kmax = 0;
+    }
+    __syncthreads();
+    // the tokens of that step (their values lie between these, with room for rounding)
+    const float slack = 1e-6f * (fabsf(row.top) + (bin + 1) / steps);
+    const float up = steps > 0.f ? row.top - bin / steps + slack : INFINITY;
+    const float down = steps > 0.f && bin < BINS - 1 ? row.top - (bin + 1) / steps - slack : -INFINITY;
+    auto in_step = [&](float f) { return f > cutv && step_of(f) == bin && amount(f) != 0; };
+    uint32_t lo = 0xffffffffu, hi = 0;
+    auto step_tokens = [&](auto f) {
+      groups([&](int, const float (&v)[8], int i) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float c = clean(v[e]);
+          if (c >= down && c <= up && in_step(c)) f(c, i + e);
+        }
+      });
+    };
+    step_tokens([&](float f, int i) {
+      lo = min(lo, key_of(f));
+      hi = max(hi, key_of(f));
+      put(f, i);
+    });
+    if (hi != 0) {
+      atomicMin(&s.kmin, lo);
+      atomicMax(&s.kmax, hi);
+    }
+    __syncthreads();
+    const bool cut_here = low_ties > 0 && step_of(cutv) == bin;
+    const uint32_t n = s.listed;
+    lo = s.kmin;
+    hi = s.kmax;
     if (cut_here) {
       lo = min(lo, low);
       hi = max(hi, low);
     }
-    // f(value) for the tokens of the step
-    auto step_tokens = [&](auto f) {
-      if (listed <= LIST) {
-        for (uint32_t i = t; i < listed; i += ST) f(s.list[i]);
-      } else {
-        groups([&](int, const float (&v)[8], int) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float y = row.clean(v[e]);
-            if (in_step(y)) f(y);
-          }
-        });
-      }
-    };
     for (;;) {
       const uint32_t span = hi - lo;
       const int shift = span < BINS ? 0 : 32 - __clz(span) - 11;
       __syncthreads();
       for (int i = t; i < BINS; i += ST) s.hist[i] = 0;
       __syncthreads();
-      step_tokens([&](float f) {
-        const uint32_t k = key_of(f);
-        if (k >= lo && k <= hi)
-          atomicAdd(reinterpret_cast<unsigned long long*>(&s.hist[(hi - k) >> shift]), amount(f));
-      });
+      auto one = [&](float f, int) {
+        const uint32_t key = key_of(f);
+        if (key >= lo && key <= hi) add(&s.hist[(hi - key) >> shift], amount(f));
+      };
+      if (n <= LIST) {
+        for (uint32_t i = t; i < n; i += ST) one(s.list[i], 0);
+      } else {
+        step_tokens(one);
+      }
       if (t == 0 && cut_here && low >= lo && low <= hi)
-        atomicAdd(reinterpret_cast<unsigned long long*>(&s.hist[(hi - low) >> shift]),
-                  amount(cutv) * ties);
+        add(&s.hist[(hi - low) >> shift], amount(cutv) * low_ties);
       __syncthreads();
-      find(s, [&](uint64_t sum) { return cross(sum, before); });
+      find(s, [&](uint64_t sum, uint64_t) { return static_cast<double>(before + sum) >= want; });
       const uint32_t b = s.bin;
+      before += s.before;
       if (shift == 0) {
-        const uint32_t k = hi - b;
-        const uint64_t one = amount(value_of(k)), all = s.hist[b];
-        ties = left(before + s.before, one, static_cast<uint32_t>(all / one));
-        cut = k;
+        const uint32_t key = hi - b;
+        const uint64_t single = amount(value_of(key)), all = s.hist[b];
+        const double more = ceil((want - static_cast<double>(before)) / static_cast<double>(single));
+        ties = min(static_cast<uint32_t>(all / single), static_cast<uint32_t>(fmax(more, 1.0)));
+        cut = key;
+        clear();
         return;
       }
-      before += s.before;
       const uint32_t top = hi - (b << shift);
       lo = max(lo, top - ((1u << shift) - 1));
       hi = top;
     }
   };
-
-  if (p.top_k != nullptr) {
-    const int64_t k = p.top_k[r];
-    if (k > 0 && k < V) {
-      const uint64_t want = k;
-      move_cut([](float) { return uint64_t{1}; },
-               [&](uint64_t sum, uint64_t before) { return before + sum >= want; },
-               [&](uint64_t before, uint64_t, uint32_t n) {
-                 return min(n, static_cast<uint32_t>(want - before));
-               });
-    }
-  }
-  if (p.top_p != nullptr && p.top_p[r] < 1.f) {
-    const double share = fmax(static_cast<double>(p.top_p[r]), 0.0);
-    // the weight of all that stays so far
-    uint64_t mine = 0, total;
-    groups([&](int, const float (&v)[8], int) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float f = row.clean(v[e]);
-        if (f > -INFINITY && key_of(f) > cut) mine += row.units(row.weight(f));
-      }
-    });
-    if (t == 0 && ties > 0) mine += row.units(row.weight(value_of(cut))) * ties;
-    scan64(mine, s, total);
-    const double want = share * static_cast<double>(total);
-    move_cut([&](float f) { return row.units(row.weight(f)); },
-             [&](uint64_t sum, uint64_t before) { return static_cast<double>(before + sum) >= want; },
-             [&](uint64_t before, uint64_t one, uint32_t n) {
-               const double more = ceil((want - static_cast<double>(before)) / static_cast<double>(one));
-               return min(n, static_cast<uint32_t>(fmax(more, 1.0)));
+  if (k > 0 && k < V)
+    move_cut([](float) { return uint64_t{1}; }, [&](uint64_t) { return static_cast<double>(k); });
+  if (share < 1.f)
+    move_cut([&](float f) { return row.weight(f); },
+             [&](uint64_t all) {
+               return fmax(static_cast<double>(share), 0.0) * static_cast<double>(all);
              });
+  if (least > value_of(cut) && !top_inf) {
+    cut = key_of(least) - (least == 0.f ? 2 : 1);  // (below 0 comes -0, which equals it)
+    ties = 0;
   }
-  double least = 0.0;
-  if (p.min_p != nullptr && p.min_p[r] > 0.f) least = fminf(p.min_p[r], 1.f);
 
   // ---- the draw: weight above the cut and tokens at the cut in each piece of 512
-  __syncthreads();
-  for (int i = t; i < BINS; i += ST) {
-    s.hist[i] = 0;
-    s.count[i] = 0;
+  // (s.hist, s.count and s.listed are 0)
+  const float cutv = value_of(cut);
+  const uint64_t tie_units = ties > 0 ? row.weight(cutv) : 0;
+  bool listed = false;
+  if (cut != key_of(-INFINITY) && !top_inf) {
+    tokens_from(ties > 0 ? cutv : value_of(cut + 1), [&](float f, int i) { put(f + 0.f, i); });
+    __syncthreads();
+    listed = s.listed <= LIST;
   }
-  __syncthreads();
-  const double wc = ties > 0 ? row.weight(value_of(cut)) : 0.0;
-  const uint64_t tie_units = wc >= least ? row.units(wc) : 0;
-  auto units_above = [&](float f) -> uint64_t {
-    if (!(f > -INFINITY) || key_of(f) <= cut) return 0;
-    const double w = row.weight(f);
-    return w >= least ? row.units(w) : 0;
-  };
-  groups([&](int i0, const float (&v)[8], int) {
-    uint64_t sum = 0;
-    uint32_t n = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float f = row.clean(v[e]);
-      sum += units_above(f);
-      n += ties > 0 && f > -INFINITY && key_of(f) == cut;
+  if (listed) {
+    const int n = static_cast<int>(s.listed);
+    for (int i = t; i < n; i += ST) {
+      const float f = s.list[i];
+      if (f > cutv) add(&s.hist[s.list_at[i] / 512], row.weight(f));
+      else atomicAdd(&s.count[s.list_at[i] / 512], 1u);
     }
+  } else {
+    groups([&](int i0, const float (&v)[8], int) {
+      uint64_t sum = 0;
+      uint32_t n = 0;
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-      sum += __shfl_xor(sum, off, 64);
-      n += __shfl_xor(n, off, 64);
-    }
-    if (lane == 0) {
-      s.hist[i0 / 512 + wave] = sum;
-      s.count[i0 / 512 + wave] = n;
-    }
-  });
-  __syncthreads();
-  uint64_t total;
-  {  // tokens at the cut stay by their index
-    const uint32_t a = s.count[2 * t], b = s.count[2 * t + 1];
-    const uint64_t incl = scan64(static_cast<uint64_t>(a) + b, s, total);
-    const uint64_t e0 = incl - a - b, e1 = e0 + a;
-    auto stay = [&](uint64_t first, uint32_t n) {
-      return first >= ties ? 0u : min(n, static_cast<uint32_t>(ties - first));
-    };
-    s.hist[2 * t] += stay(e0, a) * tie_units;
-    s.hist[2 * t + 1] += stay(e1, b) * tie_units;
-    s.count[2 * t] = static_cast<uint32_t>(e0);
-    s.count[2 * t + 1] = static_cast<uint32_t>(e1);
-  }
-  __syncthreads();
-  {
-    uint64_t mine = s.hist[2 * t] + s.hist[2 * t + 1];
-    scan64(mine, s, total);
-  }
-  const double u = p.uniform[r];
-  uint64_t target = u > 0.0 ? static_cast<uint64_t>(fmin(u, 1.0) * static_cast<double>(total)) : 0;
-  target = min(target, total - 1);
-  find(s, [&](uint64_t sum) { return sum > target; });
-  if (wave != 0) return;
-  const int piece = s.bin;
-  const int i = piece * 512 + lane * 8;
-  float v[8];
-  if (i + 8 <= V) load8u<T>(x + i, v);
-  else load8_partial<T>(x + i, i < V ? V - i : 0, -INFINITY, v);
-  uint32_t n = 0;
-  uint64_t sum = 0;
-  for (int e = 0; e < 8; ++e) {
-    v[e] = row.clean(v[e]);
-    n += ties > 0 && v[e] > -INFINITY && key_of(v[e]) == cut;
-  }
-  uint32_t first = n;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const uint32_t y = __shfl_up(first, off, 64);
-    if (lane >= off) first += y;
-  }
-  first += s.count[piece] - n;
-  uint64_t w[8];
-  for (int e = 0; e < 8; ++e) {
-    w[e] = units_above(v[e]);
-    if (ties > 0 && v[e] > -INFINITY && key_of(v[e]) == cut) w[e] = first++ < ties ? tie_units : 0;
-    sum += w[e];
-  }
-  uint64_t run = sum;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const uint64_t y = __shfl_up(run, off, 64);
-    if (lane >= off) run += y;
-  }
-  const uint64_t upto = s.before + run;
-  run = upto - sum;
-  if (upto > target && run <= target) {
-    int token = i;
-    for (int e = 0; e < 8; ++e) {
-      run += w[e];
-      if (run > target) {
-        token = i + e;
-        break;
+      for (int e = 0; e < 8; ++e) {
+        const float f = clean(v[e]);
+        const uint64_t w = row.weight(f);
+        sum += f > cutv ? w : 0;
+        n += ties > 0 && f == cutv;
       }
+      sum = last_lane(wave_scan(sum));
+      if (ties > 0) n = static_cast<uint32_t>(last_lane(wave_scan(n)));
+      if (lane == 0) {
+        s.hist[i0 / 512 + wave] = sum;
+        s.count[i0 / 512 + wave] = n;
+      }
+    });
+  }
+  __syncthreads();
+  if (wave != 0) return;
+  // Each lane a run of the pieces, in order.  (Tokens at the cut stay by their index.)
+  const int pieces = (V + 511) / 512, run = (pieces + 63) / 64;
+  const int p0 = min(lane * run, pieces), p1 = min(p0 + run, pieces);
+  uint64_t first = 0;
+  if (ties > 0) {
+    uint64_t n = 0;
+    for (int i = p0; i < p1; ++i) n += s.count[i];
+    first = wave_scan(n) - n;
+    uint64_t seen = first;
+    for (int i = p0; i < p1; ++i) {
+      const uint32_t c = s.count[i];
+      const uint64_t stay = seen >= ties ? 0 : min(static_cast<uint64_t>(c), ties - seen);
+      s.hist[i] += stay * tie_units;
+      s.count[i] = static_cast<uint32_t>(seen);
+      seen += c;
+    }
+  }
+  uint64_t sum = 0;
+  for (int i = p0; i < p1; ++i) sum += s.hist[i];
+  const uint64_t upto = wave_scan(sum);
+  const uint64_t target = target_of(u, last_lane(upto));
+  {
+    uint64_t before = upto - sum;
+    if (upto > target && before <= target) {  // (one lane)
+      int i = p0;
+      while (before + s.hist[i] <= target) before += s.hist[i++];
+      s.bin = i;
+      s.before = before;
+    }
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  const int piece = s.bin, i = piece * 512 + lane * 8;
+  float v[8];
+  load(i, v);
+  uint64_t n = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    v[e] = clean(v[e]);
+    n += ties > 0 && v[e] == cutv;
+  }
+  uint64_t tie = wave_scan(n) - n + (ties > 0 ? s.count[piece] : 0);
+  uint64_t w[8], all = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    w[e] = v[e] > cutv ? row.weight(v[e]) : 0;
+    if (ties > 0 && v[e] == cutv) w[e] = tie++ < ties ? tie_units : 0;
+    all += w[e];
+  }
+  const uint64_t up = s.before + wave_scan(all);
+  uint64_t at = up - all;
+  if (up > target && at <= target) {
+    int token = i;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (at <= target && at + w[e] > target) token = i + e;
+      at += w[e];
     }
     p.tokens[r] = token;
   }
@@ -463,7 +622,7 @@ extern "C" int sph_sample(sph_dtype dtype, int64_t rows, int64_t vocab, const vo
   SPH_REQUIRE(rows == 1 || ld >= 0, SPH_ERR_INVALID_ARG, "sample: negative leading dimension");
   int bits = 0;
   while ((int64_t{1} << bits) < vocab) ++bits;
-  const SampleArgs a{logits, ld, static_cast<int>(vocab), 62 - bits, uniform, temperature,
+  const SampleArgs a{logits, ld, static_cast<int>(vocab), std::min(62 - bits, 51), uniform, temperature,
                      top_k, top_p, min_p, tokens};
   const dim3 grid(static_cast<unsigned>(rows));
   hipStream_t st = as_stream(stream);

@@ -592,7 +592,8 @@ def test_sample_special_values(dtype, device):
     l[11, :-1] = -INF
     u = uniforms(12, 5)
     for kw in ({}, {"t": 0.0}, {"k": 3}, {"p": 0.8}, {"t": 0.5, "k": 50, "p": 0.9, "m": 0.05},
-               {"m": 1.0}, {"t": 1e20}, {"t": 1e20, "k": 7, "p": 0.5}):
+               {"m": 1.0}, {"t": 1e20}, {"t": 1e20, "k": 7, "p": 0.5}, {"t": 3e37},
+               {"t": 1e38, "p": 0.3}, {"t": 3e38, "k": 2000, "m": 0.9}):
         got = check_sample(l, device, u, **kw)
         assert got[:2] == [-1, -1] and got[4] == 17 and got[10] == 0 and got[11] == v - 1
         assert got[5] in (3, 8000, 8999)

@@ -18,10 +18,9 @@
 // whole multiples of 2^-shift, shift = 62 - log2 V (at most 51): their sums in 64-bit
 // integers are exact and do not depend on the order of additions.
 //
-// A weight is formed in ten 64-bit operations (2^y by a table of 32 steps and the series to
-// the fifth power).  That is what bounds the kernel: rows are read at the speed of the
-// cache, and a weight for each of 49155 tokens takes one workgroup 8 us (the
-// library's exp and a conversion to integers: 23).  So as few as possible are formed:
+// A weight is formed in eleven 64-bit operations (2^y by a table of 256 steps and the series to
+// the third power).  They bound the kernel: a 64-bit operation takes twice a 32-bit one's
+// time, rows are read at the speed of the cache.  So as few weights as possible are formed:
 //
 //   * top-k of at most 1024: k of the 1024 threads' own maxima reach down to some value,
 //     so the k largest do; what reaches it is listed in LDS (hardly more than k),
@@ -33,8 +32,11 @@
 //     tokens with it stay; what stays is listed if there is room.  The draw needs
 //     the sums of all 512-token pieces and then one wave in the piece that holds the token.
 //
-// One workgroup per row, which reads it again where it is needed, two turns of loads ahead.
+// One workgroup per row, which reads it again where it is needed, a turn of loads ahead.  (Four
+// turns ahead, the loops four times as long, doubled every pass's time: most
+// instructions run a few times only, so fetching them counts.)
 #include <algorithm>
+#include <type_traits>
 
 #include "sph_common.h"
 
@@ -45,7 +47,7 @@ constexpr int ST = 1024;             // threads
 constexpr int WAVES = ST / 64;
 constexpr int TILE = ST * 8;         // tokens of a turn of the workgroup
 constexpr int BINS = 2048;
-constexpr int LIST = 4096;           // tokens that are listed in LDS
+constexpr int LIST = 14336;          // tokens that are listed in LDS
 constexpr int64_t kMaxVocab = 1 << 20;
 constexpr int MAX_PIECES = kMaxVocab / 512;
 static_assert(MAX_PIECES <= BINS, "a piece per entry of the histogram");
@@ -76,7 +78,7 @@ struct Shared {
   uint32_t count[BINS];
   float list[LIST];
   int list_at[LIST];
-  double exp2[32];  // 2^(j / 32 + shift)
+  double exp2[256];  // 2^(j / 256 + shift)
   uint64_t wave64[WAVES];
   float wmax[WAVES];
   int widx[WAVES];
@@ -85,33 +87,31 @@ struct Shared {
   uint64_t before, total;
 };
 
-// A row's weights.  Values are clean: NaN counts as -inf, there is one zero, and
-// beside +inf (mapped to 0) there is only -inf.
+// A row's weights.
 struct Row {
   float top;     // M
-  double rate;   // 32 log2 e / t
+  float floor;   // a value that has no weight for sure
+  double rate;   // 256 log2 e / t
   const double* table;
-  // 32 log2 of the weight; at least -3300, where it has none (NaN: -inf times 0)
+  // 256 log2 of the weight; at least -26000, where it has none (NaN: -inf times 0)
   __device__ double log_of(float f) const {
-    return fmax((static_cast<double>(f) - top) * rate, -3300.0);
+    return fmax((static_cast<double>(f) - top) * rate, -26000.0);
   }
-  // 2^(y / 32 + shift) to the nearest whole number: y = 32 n + j + r, |r| <= 1/2, by a sum with 1.5 2^52, whose low bits then hold 32 n + j; the series of 2^(r / 32) to
-  // the fifth power (the next term is 2e-15 at most); n joins the exponent, and a sum with
-  // 2^52 leaves the whole number in the low bits (shift <= 51).
+  // The weight times 2^shift, to the nearest whole number: y = 256 n + j + r, |r| <= 1/2, by
+  // a sum with 1.5 2^52, whose low bits then hold 256 n + j; the series of 2^(r / 256)
+  // to the third power (the next term is 1.4e-13 at most); n joins the exponent, and a sum
+  // with 2^52 leaves the whole number in the low bits (shift <= 51).  NaN and -inf: 0.
   __device__ uint64_t weight(float f) const {
-    constexpr double L = 0.021660849392498290;  // ln 2 / 32
-    const double y = log_of(f);
+    constexpr double L = 0.0027076061740622863;  // ln 2 / 256
+    const double y = (static_cast<double>(fmaxf(f, floor)) - top) * rate;
     const double s = y + 0x1.8p52;
     const int k = static_cast<int>(__builtin_bit_cast(uint64_t, s));
     const double r = y - (s - 0x1.8p52);
-    double q = L * L * L * L * L / 120;
-    q = fma(q, r, L * L * L * L / 24);
-    q = fma(q, r, L * L * L / 6);
-    q = fma(q, r, L * L / 2);
+    double q = fma(L * L * L / 6, r, L * L / 2);
     q = fma(q, r, L);
-    const double t = table[k & 31];
+    const double t = table[k & 255];
     uint64_t bits = __builtin_bit_cast(uint64_t, fma(t, q * r, t));
-    bits += static_cast<uint64_t>(static_cast<uint32_t>(k >> 5) << 20) << 32;
+    bits += static_cast<uint64_t>(static_cast<uint32_t>(k >> 8) << 20) << 32;
     const double x = __builtin_bit_cast(double, bits) + 0x1p52;
     return __builtin_bit_cast(uint64_t, x) & 0xfffffffffffffull;
   }
@@ -131,6 +131,20 @@ __device__ inline uint64_t wave_scan(uint64_t v) {
   v += moved<0x118, 0xf>(v);
   v += moved<0x142, 0xa>(v);
   v += moved<0x143, 0xc>(v);
+  return v;
+}
+__device__ inline uint32_t wave_scan(uint32_t v) {
+  auto moved32 = [&](auto ctrl, auto rows) {
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(
+        0, static_cast<int>(v), decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
+  };
+  using std::integral_constant;
+  v += moved32(integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});
+  v += moved32(integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{});
+  v += moved32(integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{});
+  v += moved32(integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{});
+  v += moved32(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});
+  v += moved32(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});
   return v;
 }
 __device__ inline uint64_t last_lane(uint64_t v) {
@@ -194,24 +208,48 @@ __global__ void __launch_bounds__(ST) sample_kernel(const SampleArgs p) {
   const float share = p.top_p != nullptr ? p.top_p[r] : 1.f;
   const float min_p = p.min_p != nullptr ? p.min_p[r] : 0.f;
   const double u = p.uniform[r];
-  if (t < 32) s.exp2[t] = exp2(t / 32.0 + p.shift);
+  if (t < 256) s.exp2[t] = exp2(t / 256.0 + p.shift);
 
-  // f(index of the turn's first, values, index of the first) for this thread's 8
-  // tokens of every turn; past the row's end the values are -inf
-  auto load = [&](int i, float (&v)[8]) {
-    if (i + 8 <= V) load8u<T>(x + i, v);
-    else load8_partial<T>(x + i, i < V ? V - i : 0, -INFINITY, v);
+  // 8 values from token i on, as they lie in memory; past the row's end -inf
+  constexpr int RAW = sizeof(T) / 2;
+  struct Eight {
+    u32x4 w[RAW];
   };
+  auto fetch = [&](int i) {
+    Eight g;
+    if (i + 8 <= V) {
+#pragma unroll
+      for (int j = 0; j < RAW; ++j) g.w[j] = *reinterpret_cast<const u32x4_any*>(x + i + j * 16 / sizeof(T));
+    } else {
+      T e[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) e[j] = i + j < V ? x[i + j] : Num<T>::from_f(-INFINITY);
+      __builtin_memcpy(&g, e, sizeof(g));
+    }
+    return g;
+  };
+  // (beside +inf, which becomes 0, there is only -inf)
+  bool top_inf = false;
+  auto values = [&](const Eight& g, float (&v)[8]) {
+    T e[8];
+    __builtin_memcpy(e, &g, sizeof(g));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = Num<T>::to_f(e[j]);
+    if (top_inf) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = v[j] == INFINITY ? 0.f : -INFINITY;
+    }
+  };
+  // f(index of the turn's first, values, index of the first) for this thread's 8
+  // tokens of every turn
   auto groups = [&](auto f) {
-    float a[8], b[8];
-    load(t * 8, a);
-    load(TILE + t * 8, b);
-    for (int i0 = 0; i0 < V; i0 += 2 * TILE) {
-      f(i0, a, i0 + t * 8);
-      load(i0 + 2 * TILE + t * 8, a);
-      if (i0 + TILE >= V) break;
-      f(i0 + TILE, b, i0 + TILE + t * 8);
-      load(i0 + 3 * TILE + t * 8, b);
+    Eight now = fetch(t * 8);
+#pragma unroll 1
+    for (int i0 = 0; i0 < V; i0 += TILE) {
+      float v[8];
+      values(now, v);
+      now = fetch(i0 + TILE + t * 8);
+      f(i0, v, i0 + t * 8);
     }
   };
 
@@ -269,54 +307,59 @@ __global__ void __launch_bounds__(ST) sample_kernel(const SampleArgs p) {
     if (t == 0) p.tokens[r] = -1;
     return;
   }
-  const bool top_inf = mx == INFINITY;
-  auto clean = [&](float f) {
-    if (top_inf) return f == INFINITY ? 0.f : -INFINITY;
-    return f != f ? -INFINITY : f + 0.f;
-  };
+  top_inf = mx == INFINITY;
+  if (top_inf) mine = mine == INFINITY ? 0.f : -INFINITY;
   Row row;
-  row.top = top_inf ? 0.f : mx + 0.f;
-  row.rate = 32 * 1.4426950408889634074 / static_cast<double>(temp);
+  row.top = top_inf ? 0.f : mx + 0.f;  // (+ 0: one zero)
+  row.rate = 256 * 1.4426950408889634074 / static_cast<double>(temp);
   row.table = s.exp2;
+  {
+    const float f = fmaxf(row.top - 72.f * temp, -3.402823466e38f);
+    uint32_t key = key_of(f);  // (where t is small beside the last bit of M: one below it)
+    while (key > 0x800000u && row.log_of(value_of(key)) > -25000.0 && key + 2 > key_of(f)) --key;
+    row.floor = row.log_of(value_of(key)) > -25000.0 ? -INFINITY : value_of(key);
+    // (there it is a value or two below M: whatever makes nothing of them will do)
+    if (row.floor > -INFINITY)
+      row.rate = fmin(row.rate, 32000.0 / (static_cast<double>(row.top) - row.floor));
+  }
+  // (a temperature at which -3.4e38 has weight: values are looked at one by one)
+  const bool flat = row.floor == -INFINITY;
+  auto weight = [&](float f) { return flat && !(f > -INFINITY) ? 0 : row.weight(f); };
   // From 44 t below the maximum on a weight is less than half a unit.
   const float range = 44.f * temp;
   const float steps = range > 0.f && range < INFINITY ? (BINS - 1) / range : 0.f;
   auto step_of = [&](float f) {
     return static_cast<int>(fminf((row.top - f) * steps, static_cast<float>(BINS - 1)));
   };
-  // The least value that min-p lets through (the largest weight is 1), to the last bit.
-  float least = -INFINITY;
-  if (min_p > 0.f) {
-    const double y = 32 * log2(static_cast<double>(fminf(min_p, 1.f)));
-    uint32_t lo = key_of(-3.402823466e38f), hi = key_of(row.top);  // (the largest passes)
-    while (lo < hi) {  // 64 places at a time
-      const uint32_t gap = (hi - lo) / 64 + 1, at = min(lo + lane * gap, hi);
-      const uint64_t pass = __ballot(row.log_of(value_of(at)) >= y);
-      const uint32_t l = pass != 0 ? __builtin_ctzll(pass) : 64;
-      hi = pass != 0 ? min(lo + l * gap, hi) : hi;
-      lo = l == 0 ? lo : lo + (l - 1) * gap + 1;
-    }
-    least = value_of(lo) + 0.f;
-  }
-  // f(value, index) for the tokens from lo on, lo > -inf.  (One comparison for 8 that are
-  // below; values as they are in memory, so NaN and, beside +inf, others may come.)
-  auto tokens_from = [&](float lo, auto f) {
+  const double log_min = min_p > 0.f ? 256 * log2(static_cast<double>(fminf(min_p, 1.f))) : -30000.0;
+  // Appends the tokens from lo to hi (lo > -inf) to the list, as far as there is room, and
+  // counts them in s.listed.
+  auto list_tokens = [&](float lo, float hi) {
     groups([&](int, const float (&v)[8], int i) {
-      float m = v[0];
+      float most = v[0];
 #pragma unroll
-      for (int e = 1; e < 8; ++e) m = fmaxf(m, v[e]);
-      if (!(m >= lo)) return;
+      for (int e = 1; e < 8; ++e) most = fmaxf(most, v[e]);
+      if (__ballot(most >= lo) == 0) return;
+      uint32_t m = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m |= (v[e] >= lo && v[e] <= hi ? 1u : 0u) << e;
+      if (__ballot(m != 0) == 0) return;
+      const uint32_t n = __popc(m), upto = wave_scan(n);
+      uint32_t at = 0;
+      if (lane == 63) at = atomicAdd(&s.listed, upto);
+      at = __builtin_amdgcn_readlane(at, 63) + upto - n;
+      if (at >= LIST) return;
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (v[e] >= lo) f(v[e], i + e);
+        if (m >> e & 1u) {
+          if (at < LIST) {
+            s.list[at] = v[e] + 0.f;
+            s.list_at[at] = i + e;
+          }
+          ++at;
+        }
     });
-  };
-  auto put = [&](float f, int i) {
-    const uint32_t n = atomicAdd(&s.listed, 1u);
-    if (n < LIST) {
-      s.list[n] = f;
-      s.list_at[n] = i;
-    }
+    __syncthreads();
   };
   auto clear = [&] {
     __syncthreads();
@@ -328,60 +371,54 @@ __global__ void __launch_bounds__(ST) sample_kernel(const SampleArgs p) {
   // ---- few tokens stay: in order by counting
   if (k > 0 && k <= ST) {
     // k of the threads' maxima reach the least of those up to some step
-    if (clean(mine) > -INFINITY) add(&s.hist[step_of(clean(mine))], 1);
+    if (mine > -INFINITY) add(&s.hist[step_of(mine)], 1);
     if (t == 0) s.kmin = 0xffffffffu;
     __syncthreads();
     find(s, [&](uint64_t sum, uint64_t all) { return sum >= min(all, static_cast<uint64_t>(k)); });
     const bool enough = s.total >= static_cast<uint64_t>(k);
-    const float c = clean(mine);
-    if (c > -INFINITY && step_of(c) <= s.bin) atomicMin(&s.kmin, key_of(c));
+    if (mine > -INFINITY && step_of(mine) <= s.bin) atomicMin(&s.kmin, key_of(mine + 0.f));
     __syncthreads();
     // (fewer maxima than k: some threads have no tokens, so every token may be among the first)
-    const float from = top_inf ? INFINITY : enough ? value_of(s.kmin) : -3.402823466e38f;
-    if (enough || V <= LIST) tokens_from(from, [&](float f, int i) { put(f + 0.f, i); });
-    __syncthreads();
+    const float from = enough ? value_of(s.kmin) : -3.402823466e38f;
+    if (enough || V <= LIST) list_tokens(from, INFINITY);
     const uint32_t n = s.listed;
     if ((enough || V <= LIST) && n <= ST) {
-      float f = -INFINITY;
-      int at = 0x7fffffff;
-      uint32_t rank = ST;
-      if (t < static_cast<int>(n)) {
-        f = s.list[t];
-        at = s.list_at[t];
-        rank = 0;
-        for (uint32_t j = 0; j < n; ++j) {
-          const float g = s.list[j];
-          rank += g > f || (g == f && s.list_at[j] < at);
-        }
-      }
+      // value and index in one number, larger for those that come first
+      uint64_t mine64 = 0;
+      if (t < static_cast<int>(n))
+        mine64 = static_cast<uint64_t>(key_of(s.list[t])) << 32 | ~static_cast<uint32_t>(s.list_at[t]);
+      s.hist[t] = mine64;
       __syncthreads();
-      if (rank < ST) {
-        s.list[ST + rank] = f;
-        s.list_at[ST + rank] = at;
+      if (mine64 != 0) {
+        uint32_t rank = 0;
+#pragma unroll 8
+        for (uint32_t j = 0; j < n; ++j) rank += s.hist[j] > mine64;
+        s.hist[ST + rank] = mine64;
       }
       __syncthreads();
       const bool in = t < static_cast<int>(n) && t < k;
-      f = in ? s.list[ST + t] : -INFINITY;
-      at = in ? s.list_at[ST + t] : -1;
-      uint64_t w = in ? row.weight(top_inf ? 0.f : f) : 0;
+      mine64 = in ? s.hist[ST + t] : 0;
+      const float f = value_of(static_cast<uint32_t>(mine64 >> 32));
+      const int at = static_cast<int>(~static_cast<uint32_t>(mine64));
+      uint64_t w = in ? weight(f) : 0;
       uint64_t total;
       const uint64_t upto = scan64(w, s, total);
       const double want = fmax(static_cast<double>(share), 0.0) * static_cast<double>(total);
       if (share < 1.f && t > 0 && !(static_cast<double>(upto - w) < want)) w = 0;
-      if (!top_inf && f < least) w = 0;
-      __syncthreads();
+      if (in && row.log_of(f) < log_min) w = 0;
       s.hist[t] = w;
-      const uint64_t mass = scan64(w, s, total);
-      const uint32_t m = __popcll(__ballot(w != 0));  // (what stays are the first)
+      s.list_at[t] = at;
+      scan64(w, s, total);
+      const int m = __popcll(__ballot(w != 0));  // (what stays are the first)
       if (lane == 0) s.widx[wave] = m;
       __syncthreads();
       int stay = 0;
       for (int i = 0; i < WAVES; ++i) stay += s.widx[i];
-      (void)mass;
       const uint64_t target = target_of(u, total);
       if (w != 0) {
         uint64_t upper = 0;  // weight up to this token by index
-        for (int j = 0; j < stay; ++j) upper += s.list_at[ST + j] <= at ? s.hist[j] : 0;
+#pragma unroll 8
+        for (int j = 0; j < stay; ++j) upper += s.list_at[j] <= at ? s.hist[j] : 0;
         if (upper > target && upper - w <= target) p.tokens[r] = at;
       }
       return;
@@ -392,64 +429,82 @@ __global__ void __launch_bounds__(ST) sample_kernel(const SampleArgs p) {
   // What stays: keys above cut, and the first `ties` tokens of those equal to it.
   uint32_t cut = key_of(-INFINITY);
   uint32_t ties = 0;
+  bool listed = false;  // the list holds all that stays
 
+  // f(value) for every token of the list or the row
+  auto tokens = [&](bool of_list, auto f) {
+    if (of_list) {
+      const int n = static_cast<int>(s.listed);
+      for (int i = t; i < n; i += ST) f(s.list[i]);
+    } else {
+      groups([&](int, const float (&v)[8], int) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f(v[e]);
+      });
+    }
+  };
   // Moves the cut to the first place in the order at which the amounts summed up to it
   // reach want_of(all of them); amount(f) of a token.  Of the tokens with the value at that
-  // place as many stay as it takes.  (s.hist and s.listed are 0.)
+  // place as many stay as it takes.  (s.hist is 0.)
   auto move_cut = [&](auto amount, auto want_of) {
     const float cutv = value_of(cut);
-    const uint32_t low = cut, low_ties = ties;
-    groups([&](int, const float (&v)[8], int) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float f = clean(v[e]);
-        const uint64_t a = f > cutv ? amount(f) : 0;
-        if (a != 0) add(&s.hist[step_of(f)], a);
-      }
+    const uint32_t low_ties = ties;
+    tokens(listed, [&](float f) {
+      const uint64_t a = amount(f);
+      if (f > cutv && a != 0) add(&s.hist[step_of(f)], a);
     });
     if (low_ties > 0 && t == 0) add(&s.hist[step_of(cutv)], amount(cutv) * low_ties);
     __syncthreads();
     find(s, [&](uint64_t sum, uint64_t all) { return static_cast<double>(sum) >= want_of(all); });
     const double want = want_of(s.total);
-    if (static_cast<double>(s.total) < want) {  // all of it stays
-      clear();
-      return;
-    }
     const int bin = s.bin;
     uint64_t before = s.before;
-    __syncthreads();
+    auto empty = [&] {
+      __syncthreads();
+      for (int i = t; i < BINS; i += ST) s.hist[i] = 0;
+      __syncthreads();
+    };
+    const bool all_stay = static_cast<double>(s.total) < want;
     if (t == 0) {
       s.kmin = 0xffffffffu;
       s.kmax = 0;
+      if (!listed) s.listed = 0;
     }
-    __syncthreads();
-    // the tokens of that step (their values lie between these, with room for rounding)
-    const float slack = 1e-6f * (fabsf(row.top) + (bin + 1) / steps);
-    const float up = steps > 0.f ? row.top - bin / steps + slack : INFINITY;
-    const float down = steps > 0.f && bin < BINS - 1 ? row.top - (bin + 1) / steps - slack : -INFINITY;
+    empty();
+    if (all_stay) return;
+    bool stepped = listed;  // the list holds the tokens of that step
+    if (!listed) {
+      // a list of what lies above the end of that step, or of the step alone (with room
+      // for rounding)
+      const float slack = 1e-6f * (fabsf(row.top) + (bin + 1) / steps);
+      const float down = steps > 0.f && bin < BINS - 1
+                             ? fmaxf(row.top - (bin + 1) / steps - slack, -3.402823466e38f)
+                             : -3.402823466e38f;
+      const float up = steps > 0.f ? row.top - bin / steps + slack : INFINITY;
+      list_tokens(down, INFINITY);
+      listed = stepped = s.listed <= LIST;
+      if (!listed && up < row.top) {
+        __syncthreads();
+        if (t == 0) s.listed = 0;
+        __syncthreads();
+        list_tokens(down, up);
+        stepped = s.listed <= LIST;
+      }
+    }
     auto in_step = [&](float f) { return f > cutv && step_of(f) == bin && amount(f) != 0; };
     uint32_t lo = 0xffffffffu, hi = 0;
-    auto step_tokens = [&](auto f) {
-      groups([&](int, const float (&v)[8], int i) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float c = clean(v[e]);
-          if (c >= down && c <= up && in_step(c)) f(c, i + e);
-        }
-      });
-    };
-    step_tokens([&](float f, int i) {
-      lo = min(lo, key_of(f));
-      hi = max(hi, key_of(f));
-      put(f, i);
+    tokens(stepped, [&](float f) {
+      if (!in_step(f)) return;
+      lo = min(lo, key_of(f + 0.f));
+      hi = max(hi, key_of(f + 0.f));
     });
     if (hi != 0) {
       atomicMin(&s.kmin, lo);
       atomicMax(&s.kmax, hi);
     }
     __syncthreads();
+    const uint32_t low = cut;
     const bool cut_here = low_ties > 0 && step_of(cutv) == bin;
-    const uint32_t n = s.listed;
     lo = s.kmin;
     hi = s.kmax;
     if (cut_here) {
@@ -459,31 +514,24 @@ __global__ void __launch_bounds__(ST) sample_kernel(const SampleArgs p) {
     for (;;) {
       const uint32_t span = hi - lo;
       const int shift = span < BINS ? 0 : 32 - __clz(span) - 11;
-      __syncthreads();
-      for (int i = t; i < BINS; i += ST) s.hist[i] = 0;
-      __syncthreads();
-      auto one = [&](float f, int) {
-        const uint32_t key = key_of(f);
+      tokens(stepped, [&](float f) {
+        if (!in_step(f)) return;
+        const uint32_t key = key_of(f + 0.f);
         if (key >= lo && key <= hi) add(&s.hist[(hi - key) >> shift], amount(f));
-      };
-      if (n <= LIST) {
-        for (uint32_t i = t; i < n; i += ST) one(s.list[i], 0);
-      } else {
-        step_tokens(one);
-      }
+      });
       if (t == 0 && cut_here && low >= lo && low <= hi)
         add(&s.hist[(hi - low) >> shift], amount(cutv) * low_ties);
       __syncthreads();
       find(s, [&](uint64_t sum, uint64_t) { return static_cast<double>(before + sum) >= want; });
       const uint32_t b = s.bin;
+      const uint64_t all = s.hist[b];
       before += s.before;
+      empty();
       if (shift == 0) {
-        const uint32_t key = hi - b;
-        const uint64_t single = amount(value_of(key)), all = s.hist[b];
+        cut = hi - b;
+        const uint64_t single = amount(value_of(cut));
         const double more = ceil((want - static_cast<double>(before)) / static_cast<double>(single));
         ties = min(static_cast<uint32_t>(all / single), static_cast<uint32_t>(fmax(more, 1.0)));
-        cut = key;
-        clear();
         return;
       }
       const uint32_t top = hi - (b << shift);
@@ -494,48 +542,84 @@ __global__ void __launch_bounds__(ST) sample_kernel(const SampleArgs p) {
   if (k > 0 && k < V)
     move_cut([](float) { return uint64_t{1}; }, [&](uint64_t) { return static_cast<double>(k); });
   if (share < 1.f)
-    move_cut([&](float f) { return row.weight(f); },
+    move_cut([&](float f) { return weight(f); },
              [&](uint64_t all) {
                return fmax(static_cast<double>(share), 0.0) * static_cast<double>(all);
              });
-  if (least > value_of(cut) && !top_inf) {
+  // The least value that min-p lets through (the largest weight is 1), to the last bit.
+  float least = -INFINITY;
+  if (min_p > 0.f) {
+    uint32_t lo = key_of(-3.402823466e38f), hi = key_of(row.top);  // (the largest passes)
+    while (lo < hi) {  // 64 places at a time
+      const uint32_t gap = (hi - lo) / 64 + 1, at = min(lo + lane * gap, hi);
+      const uint64_t pass = __ballot(row.log_of(value_of(at)) >= log_min);
+      const uint32_t l = pass != 0 ? __builtin_ctzll(pass) : 64;
+      hi = pass != 0 ? min(lo + l * gap, hi) : hi;
+      lo = l == 0 ? lo : lo + (l - 1) * gap + 1;
+    }
+    least = value_of(lo) + 0.f;
+  }
+  if (least > value_of(cut)) {
     cut = key_of(least) - (least == 0.f ? 2 : 1);  // (below 0 comes -0, which equals it)
     ties = 0;
   }
 
   // ---- the draw: weight above the cut and tokens at the cut in each piece of 512
-  // (s.hist, s.count and s.listed are 0)
+  // (s.hist and s.count are 0)
   const float cutv = value_of(cut);
-  const uint64_t tie_units = ties > 0 ? row.weight(cutv) : 0;
-  bool listed = false;
-  if (cut != key_of(-INFINITY) && !top_inf) {
-    tokens_from(ties > 0 ? cutv : value_of(cut + 1), [&](float f, int i) { put(f + 0.f, i); });
+  const uint64_t tie_units = ties > 0 ? weight(cutv) : 0;
+  if (!listed && cut != key_of(-INFINITY)) {
     __syncthreads();
+    if (t == 0) s.listed = 0;
+    __syncthreads();
+    list_tokens(ties > 0 ? cutv : value_of(cut + 1), INFINITY);
     listed = s.listed <= LIST;
   }
   if (listed) {
-    const int n = static_cast<int>(s.listed);
-    for (int i = t; i < n; i += ST) {
-      const float f = s.list[i];
-      if (f > cutv) add(&s.hist[s.list_at[i] / 512], row.weight(f));
-      else atomicAdd(&s.count[s.list_at[i] / 512], 1u);
-    }
+    // each thread a run of an odd length (neighbours are of one piece, mostly)
+    const int n = static_cast<int>(s.listed), run = n / ST | 1;
+    uint64_t sum = 0;
+    int piece = -1;
+    auto leave = [&] {
+      if (sum != 0) add(&s.hist[piece], sum);
+      sum = 0;
+    };
+    for (int j = 0; j < n; j += run * ST)
+      for (int i = j + t * run; i < min(j + (t + 1) * run, n); ++i) {
+        const float f = s.list[i];
+        const int at = s.list_at[i] / 512;
+        if (f > cutv) {
+          if (at != piece) leave();
+          piece = at;
+          sum += weight(f);
+        } else if (ties > 0 && f == cutv) {
+          atomicAdd(&s.count[at], 1u);
+        }
+      }
+    leave();
+  } else if (cut == key_of(-INFINITY) && !flat) {
+    groups([&](int i0, const float (&v)[8], int) {
+      uint64_t sum = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum += row.weight(v[e]);
+      sum = wave_scan(sum);
+      if (lane == 63) s.hist[i0 / 512 + wave] = sum;
+    });
   } else {
     groups([&](int i0, const float (&v)[8], int) {
       uint64_t sum = 0;
       uint32_t n = 0;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float f = clean(v[e]);
-        const uint64_t w = row.weight(f);
-        sum += f > cutv ? w : 0;
-        n += ties > 0 && f == cutv;
+        const uint64_t w = weight(v[e]);
+        sum += v[e] > cutv ? w : 0;
+        n += ties > 0 && v[e] == cutv;
       }
-      sum = last_lane(wave_scan(sum));
-      if (ties > 0) n = static_cast<uint32_t>(last_lane(wave_scan(n)));
-      if (lane == 0) {
+      sum = wave_scan(sum);
+      const uint64_t m = ties > 0 ? wave_scan(n) : 0;
+      if (lane == 63) {
         s.hist[i0 / 512 + wave] = sum;
-        s.count[i0 / 512 + wave] = n;
+        s.count[i0 / 512 + wave] = static_cast<uint32_t>(m);
       }
     });
   }
@@ -575,18 +659,17 @@ __global__ void __launch_bounds__(ST) sample_kernel(const SampleArgs p) {
   __builtin_amdgcn_wave_barrier();
   const int piece = s.bin, i = piece * 512 + lane * 8;
   float v[8];
-  load(i, v);
+  values(fetch(i), v);
   uint64_t n = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    v[e] = clean(v[e]);
     n += ties > 0 && v[e] == cutv;
   }
   uint64_t tie = wave_scan(n) - n + (ties > 0 ? s.count[piece] : 0);
   uint64_t w[8], all = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    w[e] = v[e] > cutv ? row.weight(v[e]) : 0;
+    w[e] = v[e] > cutv ? weight(v[e]) : 0;
     if (ties > 0 && v[e] == cutv) w[e] = tie++ < ties ? tie_units : 0;
     all += w[e];
   }

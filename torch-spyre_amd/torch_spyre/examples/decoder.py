@@ -25,6 +25,12 @@ add_rms_norm_fp8, quantize_fp8, silu_mul_fp8}) and meet the weights' codes in
 torch.ops.spyre.mm_fp8; the residual stream, RoPE, attention and the cache stay
 in the model's type.  prefill, decode_step, decode_step_static and generate
 take such weights as they are.
+
+Sequences of different lengths share a paged cache (new_paged_cache, PagedPlan)
+in step_paged: any mix of prompt pieces, decoded tokens and trees of drafted
+tokens as rows of one call, with torch.ops.spyre.{paged_append, paged_attention}
+in every layer.  generate_paged samples with torch.ops.spyre.sample;
+generate_speculative verifies drafted trees.
 """
 
 from __future__ import annotations
@@ -37,6 +43,7 @@ import torch
 import torch.nn.functional as F
 
 import torch_spyre._inductor.customops  # noqa: F401  (torch.ops.spyre.decode_attention)
+import torch_spyre._inductor.serving  # noqa: F401  (torch.ops.spyre.paged_append ...)
 
 
 @dataclasses.dataclass(frozen=True)
@@ -126,7 +133,8 @@ def quantize_params(params: dict) -> dict:
 
     layers = [{"attn_norm": w["attn_norm"], "mlp_norm": w["mlp_norm"],
                "wqkv_fp8": q(fused(w, "wqkv", ("wq", "wk", "wv"))), "wo_fp8": q(w["wo"]),
-               "wgu_fp8": q(fused(w, "wgu", ("wg", "wu"))), "wd_fp8": q(w["wd"])}
+               "wgu_fp8": q(fused(w, "wgu", ("wg", "wu"))), "wd_fp8": q(w["wd"]),
+               **{n: w[n] for n in ("q_norm", "k_norm") if n in w}}
               for w in params["layers"]]
     return {"embed": params["embed"], "layers": layers, "final_norm": params["final_norm"],
             "lm_head_fp8": q(params["lm_head"])}
@@ -450,3 +458,209 @@ def _generate_graph(logits, pos, params, cfg, steps, cos, sin, cache, decode_fn,
             feed.copy_(step_arg if teacher is None else teacher[:, t + 1])
     g.reset()
     return torch.stack(out, 1), torch.stack(logits, 0)
+
+
+# ---- a paged cache shared by sequences of different lengths -------------------
+
+def new_paged_cache(cfg: DecoderConfig, pages: int, page_size: int, device, dtype=torch.float16):
+    """Per layer, zeroed K and V pages [pages, n_kv_heads, page_size, head_dim]."""
+    shape = (pages, cfg.n_kv_heads, page_size, cfg.head_dim)
+    return [(torch.zeros(shape, dtype=dtype, device=device),
+             torch.zeros(shape, dtype=dtype, device=device)) for _ in range(cfg.n_layers)]
+
+
+class PagedPlan:
+    """Where sequences of up to `lengths` tokens lie in a cache of pages, on the
+    host: pages in turn, a page of each sequence at a time, as if they had grown
+    side by side."""
+
+    def __init__(self, lengths, page_size: int):
+        self.page_size = page_size
+        need = [-(-n // page_size) for n in lengths]
+        self.pages = sum(need)
+        self.table = torch.zeros(len(need), max(need + [1]), dtype=torch.int64)
+        free = 0
+        for j in range(self.table.shape[1]):
+            for b, n in enumerate(need):
+                if j < n:
+                    self.table[b, j] = free
+                    free += 1
+
+    def slots(self, b: int, first: int, n: int) -> torch.Tensor:
+        """Slots of tokens first .. first + n - 1 of sequence b."""
+        at = torch.arange(first, first + n)
+        return self.table[b, at // self.page_size] * self.page_size + at % self.page_size
+
+
+def step_paged(tokens, positions, slots, block_table, seq_lens, q_starts, params: dict, cos, sin,
+               cache, cfg: DecoderConfig, mask=None, rows=None):
+    """One step of a batch over a paged cache: tokens [T], those of sequence b at
+    q_starts[b] .. q_starts[b + 1] - 1, at `positions` [T]; their keys and values go to
+    `slots` [T] (-1: padding), and seq_lens [B] counts them in.  mask [T, N] (bool): which
+    of its sequence's new tokens each of them sees (None: causal).  Returns the
+    logits of every token, or of `rows` (int64)."""
+    ops = torch.ops.spyre
+    layers = params["layers"]
+    h = F.embedding(tokens, params["embed"])
+    scale = 1.0 / math.sqrt(cfg.head_dim)
+    xn = None  # as in decode_step
+    for i, w in enumerate(layers):
+        x = xn or _first_norm(h, w, cfg)
+        if "wqkv_fp8" in w:
+            qkv = ops.mm_fp8(*x, *w["wqkv_fp8"], h.dtype)
+        elif "wqkv" in w:
+            qkv = F.linear(x, w["wqkv"])
+        else:
+            qkv = torch.cat([F.linear(x, w[n]) for n in ("wq", "wk", "wv")], -1)
+        kc, vc = cache[i]
+        q = ops.paged_append(qkv, cos, sin, positions, slots, kc, vc, cfg.n_heads,
+                             w.get("q_norm"), w.get("k_norm"), cfg.eps)
+        a = ops.paged_attention(q, kc, vc, block_table, seq_lens, q_starts, scale, mask)
+        a = a.view(a.shape[0], -1)
+        if "wo_fp8" in w:
+            h, xn = _rest_of_layer_fp8(a, h, w, cfg, _norm_after(i, params))
+            continue
+        h = h + F.linear(a, w["wo"])
+        h = h + _mlp(F.rms_norm(h, (cfg.hidden,), w["mlp_norm"], cfg.eps), w, cfg)
+    if rows is not None and xn is None:
+        h = h.index_select(0, rows)
+    logits = lm_logits(h, params, cfg, xn)
+    return logits if rows is None or xn is None else logits.index_select(0, rows)
+
+
+def generate_paged(prompts, params: dict, cfg: DecoderConfig, steps: int, device, page_size=16,
+                   uniform=None, temperature=None, top_k=None, top_p=None, min_p=None,
+                   teacher=None, step_fn=None, use_graph=False):
+    """Decodes `steps` tokens behind each of `prompts` (1-D token tensors of any lengths)
+    over one paged cache: one step_paged for all prompts, then one for each token.
+    Tokens are drawn by torch.ops.spyre.sample with `uniform` [steps, B] (fp32 in [0,
+    1)) and the other parameters [B] (see there), without `uniform` the largest
+    logit's.  `teacher` [B, steps]: tokens to feed instead.  `step_fn` (e.g.
+    torch.compile(step_paged)) takes the decode steps; with `use_graph` one of them, its
+    draw included, is captured and replayed.  Returns (tokens [B, steps], logits
+    [steps + 1, B, vocab])."""
+    step_fn = step_fn or step_paged
+    ops, dt, B = torch.ops.spyre, params["embed"].dtype, len(prompts)
+    lens = [int(p.shape[0]) for p in prompts]
+    plan = PagedPlan([n + steps for n in lens], page_size)
+    cos, sin = rope_tables(cfg, max(lens) + steps, device, torch.float32)
+    cache = new_paged_cache(cfg, plan.pages, page_size, device, dt)
+    table = plan.table.to(device)
+    starts = torch.tensor([0] + lens).cumsum(0)
+    if uniform is None:
+        uniform, temperature = torch.zeros(steps + 1, B), torch.zeros(B)
+        top_k = top_p = min_p = None
+    uniform = uniform.to(device)
+    how = [None if x is None else x.to(device) for x in (temperature, top_k, top_p, min_p)]
+    logits = [step_paged(
+        torch.cat([p.to("cpu") for p in prompts]).to(device),
+        torch.cat([torch.arange(n) for n in lens]).to(device),
+        torch.cat([plan.slots(b, 0, n) for b, n in enumerate(lens)]).to(device), table,
+        torch.tensor(lens).to(device), starts.to(device), params, cos, sin, cache, cfg,
+        rows=(starts[1:] - 1).to(device))]
+    if steps == 0:
+        return torch.zeros(B, 0, dtype=torch.int64, device=device), torch.stack(logits, 0)
+    # what a step is given, for all of them
+    at = torch.stack([torch.tensor(lens) + t for t in range(steps)]).to(device)
+    slot = torch.stack([torch.cat([plan.slots(b, n + t, 1) for b, n in enumerate(lens)])
+                        for t in range(steps)]).to(device)
+    length = at + 1
+    q_starts = torch.arange(B + 1).to(device)
+    token = ops.sample(logits[0], uniform[0], *how)
+    out = [token]
+    feed = (token if teacher is None else teacher[:, 0]).clone()
+    now = [x[0].clone() for x in (at, slot, length, uniform)]
+
+    def step():
+        l = step_fn(feed, now[0], now[1], table, now[2], q_starts, params, cos, sin, cache, cfg)
+        return l, ops.sample(l, now[3], *how)
+
+    graph = None
+    if use_graph:
+        import torch_spyre.graphs as graphs
+
+        step()  # loads every kernel; writes what the first replay will write again
+        graph = graphs.SpyreGraph()
+        with graphs.graph(graph):
+            step_logits, step_token = step()
+    for t in range(steps):
+        if t:
+            feed.copy_(out[-1] if teacher is None else teacher[:, t])
+        for x, y in zip(now, (at, slot, length)):
+            x.copy_(y[t])
+        if t + 1 < steps:
+            now[3].copy_(uniform[t + 1])
+        if graph is None:
+            step_logits, step_token = step()
+        else:
+            graph.replay()
+        logits.append(step_logits.clone())
+        if t + 1 < steps:
+            out.append(step_token.clone())
+    if graph is not None:
+        graph.reset()
+    return torch.stack(out, 1), torch.stack(logits, 0)
+
+
+def tree_mask(parents) -> torch.Tensor:
+    """[n, n] (bool): each node of a tree sees itself and its ancestors; parents[i] < i,
+    the root's -1."""
+    m = torch.eye(len(parents), dtype=torch.bool)
+    for i, p in enumerate(parents):
+        if p >= 0:
+            m[i] |= m[p]
+    return m
+
+
+def generate_speculative(prompt, params: dict, cfg: DecoderConfig, steps: int, device, draft,
+                         page_size=16, most=32):
+    """Greedy decoding of one sequence with drafted trees: draft(tokens so far) gives
+    (tokens, parents) of at most most - 1 nodes that may follow, parents[i] < i, -1 for those that
+    follow the last token itself.  Each round runs the last token and the tree as rows
+    of one step_paged, accepts the path that the largest logits follow and moves its
+    keys and values behind each other.  Returns (the `steps` tokens that greedy decoding
+    gives, rounds taken)."""
+    dt, n = params["embed"].dtype, int(prompt.shape[0])
+    plan = PagedPlan([n + steps + most], page_size)
+    cos, sin = rope_tables(cfg, n + steps + most, device, torch.float32)
+    cache = new_paged_cache(cfg, plan.pages, page_size, device, dt)
+    table = plan.table.to(device)
+
+    def run(tokens, positions, first, mask):
+        m = len(tokens)
+        return step_paged(torch.tensor(tokens).to(device), torch.tensor(positions).to(device),
+                          plan.slots(0, first, m).to(device), table,
+                          torch.tensor([first + m]).to(device), torch.tensor([0, m]).to(device),
+                          params, cos, sin, cache, cfg,
+                          None if mask is None else mask.to(device)).argmax(-1).tolist()
+
+    seq = prompt.tolist()
+    seq.append(run(seq, list(range(n)), 0, None)[-1])
+    rounds = 0
+    while len(seq) < n + steps:
+        rounds += 1
+        first = len(seq) - 1  # the last token is not in the cache yet
+        tokens, parents = draft(seq)
+        tokens = [seq[-1]] + list(tokens)[:most - 1]
+        parents = [-1] + [p + 1 for p in list(parents)[:most - 1]]
+        depth = [0] * len(tokens)
+        for i in range(1, len(tokens)):
+            depth[i] = depth[parents[i]] + 1
+        best = run(tokens, [first + d for d in depth], first, tree_mask(parents))
+        path = [0]
+        while True:
+            follow = [i for i in range(path[-1] + 1, len(tokens))
+                      if parents[i] == path[-1] and tokens[i] == best[path[-1]]]
+            if not follow:
+                break
+            path.append(follow[0])
+        if path != list(range(len(path))):  # accepted nodes move behind each other
+            old, new = plan.slots(0, first, len(tokens))[path], plan.slots(0, first, len(path))
+            for kc, vc in cache:
+                for c in (kc, vc):
+                    flat = c.transpose(1, 2).reshape(-1, *c.shape[1:2], c.shape[3])
+                    picked = flat.index_select(0, old.to(device))
+                    for j, s in enumerate(new.tolist()):
+                        c[s // page_size, :, s % page_size].copy_(picked[j])
+        seq += [tokens[i] for i in path[1:]] + [best[path[-1]]]
+    return torch.tensor(seq[n:n + steps]), rounds

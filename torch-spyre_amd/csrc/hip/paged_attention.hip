@@ -56,6 +56,8 @@ constexpr int kMaxGrid = 512;             // two workgroups per CU
 constexpr int kFewParts = 16;             // parts of a unit that one group of lanes merges
 constexpr int32_t kPagedIndex = 3;      // error code: page, length or start out of range
 constexpr float kLog2e = 1.4426950408889634f;
+// s_waitcnt for vmcnt(0) alone (fields of gfx9: vmcnt [3:0] and [15:14], the others at their most)
+constexpr int kWaitVmcnt0 = 0x0F70;
 
 struct PagedArgs {
   const void* q;
@@ -383,29 +385,40 @@ paged_attn_kernel(const PagedArgs) {
   // A stage's 64 keys: this thread's chunk t % CPR of rows t / CPR + SR i, K in
   // kr[0], V in kr[1].
   const int srow = t / CPR, schunk = t % CPR;
+  const uint32_t k_row = (P16 ? (srow & 15) * k_next : 0u) + 16 * schunk;
+  const uint32_t v_row = (P16 ? (srow & 15) * v_next : 0u) + 16 * schunk;
   auto load_stage = [&](const Unit& u, int kb) {
     const int last = last_block(u);
 #pragma unroll
     for (int i = 0; i < SP; ++i) {
-      const int row = srow + SR * i;
-      const char *k = Kh + 16 * schunk, *v = Vh + 16 * schunk;
+      const char *k = Kh, *v = Vh;
       if constexpr (P16) {
         const int blk = min((kb + SR * i + uni(srow)) / 16, last) - base;
-        k += lane_of(ko, blk) + (row & 15) * k_next;
-        v += lane_of(vo, blk) + (row & 15) * v_next;
+        k += lane_of(ko, blk);
+        v += lane_of(vo, blk);
       } else {
-        const int x = min(kb + row, last) - base;
+        const int x = min(kb + srow + SR * i, last) - base;
         k += __shfl(ko, x, 64);
         v += __shfl(vo, x, 64);
       }
-      kr[0][i] = *reinterpret_cast<const u32x4_any*>(k);
-      kr[1][i] = *reinterpret_cast<const u32x4_any*>(v);
+      kr[0][i] = *reinterpret_cast<const u32x4_any*>(k + k_row);
+      kr[1][i] = *reinterpret_cast<const u32x4_any*>(v + v_row);
     }
   };
   // Queries of a unit and its first keys (its first pages are in `ahead`).
   auto begin = [&](const Unit& u) {
     const int row0 = u.tile * R * u.s.rw + (wave % u.s.rw) * R;
     const ArgPtr p = args();
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      const int r = min(row0 + 16 * i + n16, u.s.rows - 1);
+      tok[i] = r / p->g;
+      const T* q = static_cast<const T*>(p->q) + (u.s.start + tok[i]) * p->q_st +
+                   static_cast<int64_t>(u.h * p->g + r % p->g) * p->q_sh;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk)
+        qf[i][kk] = *reinterpret_cast<const u32x4_any*>(q + 32 * kk + 8 * g4);
+    }
     Kh = reinterpret_cast<const char*>(static_cast<const T*>(p->kc) + u.h * p->k_sh);
     Vh = reinterpret_cast<const char*>(static_cast<const T*>(p->vc) + u.h * p->v_sh);
     const int kb = first_key(u);
@@ -417,16 +430,6 @@ paged_attn_kernel(const PagedArgs) {
         load_k(u, kb);
         load_v(u, kb);
       }
-    }
-#pragma unroll
-    for (int i = 0; i < RT; ++i) {
-      const int r = min(row0 + 16 * i + n16, u.s.rows - 1);
-      tok[i] = r / p->g;
-      const T* q = static_cast<const T*>(p->q) + (u.s.start + tok[i]) * p->q_st +
-                   static_cast<int64_t>(u.h * p->g + r % p->g) * p->q_sh;
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk)
-        qf[i][kk] = *reinterpret_cast<const u32x4_any*>(q + 32 * kk + 8 * g4);
     }
   };
 
@@ -447,6 +450,11 @@ paged_attn_kernel(const PagedArgs) {
     }
     const int tile0 = u.tile * R * u.s.rw, row0 = tile0 + (wave % u.s.rw) * R;
     const int kend = u.kend, ctx = u.ctx;
+    // Keys that all rows of this wave (of the tile) see: without a mask also new ones, up to the
+    // first row's token.
+    const bool masked = args()->mask != nullptr;
+    const int seen = masked ? ctx : ctx + row0 / args()->g + 1;
+    const int seen_tile = masked ? ctx : ctx + tile0 / args()->g + 1;
     f32x4 o[RT][DT];
     float m[RT], l[RT];
 #pragma unroll
@@ -542,10 +550,15 @@ paged_attn_kernel(const PagedArgs) {
       }
     };
 
+    // Queries and first keys have landed.  (Else the compiler waits for the queries where the
+    // key loop uses them, in every step, and so for all loads in flight there.)
+    __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
     if constexpr (FORM != WIDE) {
       const int step = step_of(u);
       int kb = first_key(u);
-      // One step of 32 keys; EDGE: some of them are not seen by every row.
+      // One step of 32 keys; EDGE: some of them are not seen by every row.  (The last step as a
+      // third variant, so that the loads ahead are certain and the keys need not be
+      // waited for together with the values, costs more in code than it saves.)
       auto one = [&](auto edge) {
         constexpr bool EDGE = decltype(edge)::value;
         f32x4 sc[RT][2];
@@ -569,7 +582,7 @@ paged_attn_kernel(const PagedArgs) {
             bool bad = false;
 #pragma unroll
             for (int e = 0; e < VW; ++e) bad = bad || not_finite<T>(vr[j][e]);
-            bad = bad && key < kend && key >= ctx;
+            bad = bad && key < kend && key >= seen;
             const uint64_t all = __ballot(bad);  // (16 lanes hold a key)
 #pragma unroll
             for (int g = 0; g < 4; ++g)
@@ -606,23 +619,25 @@ paged_attn_kernel(const PagedArgs) {
         kb += step;
       };
       if (row0 < u.s.rows) {
-        while (kb < kend && kb + 32 <= ctx) one(std::false_type{});
+        while (kb + 32 <= min(kend, seen)) one(std::false_type{});
         while (kb < kend) one(std::true_type{});
       }
     } else {
       // Stages of 64 keys in LDS: [stage][K, V][key][chunk ^ key].
+      static_assert(SR % CPR == 0, "a turn further, the swap is the same");
+      const int put_at = (srow * CPR + (schunk ^ (srow & (CPR - 1)))) * 16;
       auto put = [&](int kb, int slot) {
         char* to = lds + slot * 2 * STAGE;
-        const bool edge = kb + SK > ctx;
+        const bool edge = kb + SK > seen_tile || kb + SK > kend;
 #pragma unroll
         for (int i = 0; i < SP; ++i) {
-          const int row = srow + SR * i, at = (row * CPR + (schunk ^ (row & (CPR - 1)))) * 16;
+          const int row = srow + SR * i, at = put_at + SR * i * CPR * 16;
           u32x4 v = kr[1][i];
           if (edge) {
             bool bad = false;
 #pragma unroll
             for (int e = 0; e < 4; ++e) bad = bad || not_finite<T>(v[e]);
-            bad = bad && kb + row < kend && kb + row >= ctx;
+            bad = bad && kb + row < kend && kb + row >= seen_tile;
             bad = (__ballot(bad) >> (lane & ~(CPR - 1)) & ((1ull << CPR) - 1)) != 0;
             if (schunk == 0) odd_rows[slot][row] = bad;
             if (bad || kb + row >= kend) v = u32x4{0u, 0u, 0u, 0u};
@@ -677,8 +692,7 @@ paged_attn_kernel(const PagedArgs) {
                 sc[i][th] = a;
               }
             }
-            const bool edge = kb + 32 > ctx;
-            if (edge) hide(sc, kb);
+            if (kb + 32 > seen || kb + 32 > kend) hide(sc, kb);
             u32x4 pf[RT];
 #pragma unroll
             for (int i = 0; i < RT; ++i) pf[i] = softmax(sc[i], i);
@@ -694,7 +708,7 @@ paged_attn_kernel(const PagedArgs) {
 #pragma unroll
               for (int i = 0; i < RT; ++i) o[i][d] = mfma16<T>(vf, pf[i], o[i][d]);
             }
-            if (edge) {
+            if (kb + 32 > seen_tile) {
               const uint32_t bits =
                   static_cast<uint32_t>(__ballot(odd_rows[slot][32 * sub + (lane & 31)] != 0));
               if (bits != 0) add_odd(sc, kb, bits, [&](int d, int r) { return 16 * d + 4 * g4 + r; });

@@ -52,6 +52,11 @@ constexpr int64_t kMaxVocab = 1 << 20;
 constexpr int MAX_PIECES = kMaxVocab / 512;
 static_assert(MAX_PIECES <= BINS, "a piece per entry of the histogram");
 
+struct alignas(8) Item {
+  float value;
+  int at;
+};
+
 struct SampleArgs {
   const void* logits;
   int64_t ld;
@@ -74,15 +79,15 @@ __device__ inline float value_of(uint32_t k) {
 }
 
 struct Shared {
-  uint64_t hist[BINS];
+  alignas(16) uint64_t hist[BINS];
   uint32_t count[BINS];
-  float list[LIST];
-  int list_at[LIST];
+  Item list[LIST];
   double exp2[256];  // 2^(j / 256 + shift)
   uint64_t wave64[WAVES];
   float wmax[WAVES];
   int widx[WAVES];
-  uint32_t listed, kmin, kmax;
+  uint32_t few[ST];  // keys of a step's tokens
+  uint32_t listed, in_few, kmin, kmax;
   int bin;
   uint64_t before, total;
 };
@@ -146,6 +151,11 @@ __device__ inline uint32_t wave_scan(uint32_t v) {
   v += moved32(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});
   v += moved32(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});
   return v;
+}
+__device__ inline uint64_t lane_xor(uint64_t v, int off) {
+  const uint32_t lo = __shfl_xor(static_cast<int>(v), off, 64);
+  const uint32_t hi = __shfl_xor(static_cast<int>(v >> 32), off, 64);
+  return static_cast<uint64_t>(hi) << 32 | lo;
 }
 __device__ inline uint64_t last_lane(uint64_t v) {
   const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(v), 63);
@@ -324,7 +334,11 @@ __global__ void __launch_bounds__(ST) sample_kernel(const SampleArgs p) {
   }
   // (a temperature at which -3.4e38 has weight: values are looked at one by one)
   const bool flat = row.floor == -INFINITY;
-  auto weight = [&](float f) { return flat && !(f > -INFINITY) ? 0 : row.weight(f); };
+  // (no branch around a weight: eight in a row run side by side)
+  auto weight = [&](float f) {
+    const uint64_t w = row.weight(f);
+    return f > -INFINITY ? w : 0;
+  };
   // From 44 t below the maximum on a weight is less than half a unit.
   const float range = 44.f * temp;
   const float steps = range > 0.f && range < INFINITY ? (BINS - 1) / range : 0.f;
@@ -352,10 +366,7 @@ __global__ void __launch_bounds__(ST) sample_kernel(const SampleArgs p) {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         if (m >> e & 1u) {
-          if (at < LIST) {
-            s.list[at] = v[e] + 0.f;
-            s.list_at[at] = i + e;
-          }
+          if (at < LIST) s.list[at] = {v[e] + 0.f, i + e};
           ++at;
         }
     });
@@ -386,7 +397,8 @@ __global__ void __launch_bounds__(ST) sample_kernel(const SampleArgs p) {
       // value and index in one number, larger for those that come first
       uint64_t mine64 = 0;
       if (t < static_cast<int>(n))
-        mine64 = static_cast<uint64_t>(key_of(s.list[t])) << 32 | ~static_cast<uint32_t>(s.list_at[t]);
+        mine64 = static_cast<uint64_t>(key_of(s.list[t].value)) << 32 |
+                 ~static_cast<uint32_t>(s.list[t].at);
       s.hist[t] = mine64;
       __syncthreads();
       if (mine64 != 0) {
@@ -406,8 +418,9 @@ __global__ void __launch_bounds__(ST) sample_kernel(const SampleArgs p) {
       const double want = fmax(static_cast<double>(share), 0.0) * static_cast<double>(total);
       if (share < 1.f && t > 0 && !(static_cast<double>(upto - w) < want)) w = 0;
       if (in && row.log_of(f) < log_min) w = 0;
-      s.hist[t] = w;
-      s.list_at[t] = at;
+      __syncthreads();  // (the order above has been read)
+      s.hist[2 * t] = w;
+      s.hist[2 * t + 1] = at;
       scan64(w, s, total);
       const int m = __popcll(__ballot(w != 0));  // (what stays are the first)
       if (lane == 0) s.widx[wave] = m;
@@ -418,7 +431,10 @@ __global__ void __launch_bounds__(ST) sample_kernel(const SampleArgs p) {
       if (w != 0) {
         uint64_t upper = 0;  // weight up to this token by index
 #pragma unroll 8
-        for (int j = 0; j < stay; ++j) upper += s.list_at[j] <= at ? s.hist[j] : 0;
+        for (int j = 0; j < stay; ++j) {
+          const uint64_t other = s.hist[2 * j];
+          upper += static_cast<int>(s.hist[2 * j + 1]) <= at ? other : 0;
+        }
         if (upper > target && upper - w <= target) p.tokens[r] = at;
       }
       return;
@@ -435,7 +451,7 @@ __global__ void __launch_bounds__(ST) sample_kernel(const SampleArgs p) {
   auto tokens = [&](bool of_list, auto f) {
     if (of_list) {
       const int n = static_cast<int>(s.listed);
-      for (int i = t; i < n; i += ST) f(s.list[i]);
+      for (int i = t; i < n; i += ST) f(s.list[i].value);
     } else {
       groups([&](int, const float (&v)[8], int) {
 #pragma unroll
@@ -468,6 +484,7 @@ __global__ void __launch_bounds__(ST) sample_kernel(const SampleArgs p) {
     if (t == 0) {
       s.kmin = 0xffffffffu;
       s.kmax = 0;
+      s.in_few = 0;
       if (!listed) s.listed = 0;
     }
     empty();
@@ -491,6 +508,50 @@ __global__ void __launch_bounds__(ST) sample_kernel(const SampleArgs p) {
         stepped = s.listed <= LIST;
       }
     }
+    const uint32_t low = cut;
+    const bool cut_here = low_ties > 0 && step_of(cutv) == bin;
+    // Few tokens in that step, as a rule: each thread weighs one and adds up what comes before.
+    tokens(stepped, [&](float f) {
+      if (!(f > cutv && step_of(f) == bin)) return;
+      const uint32_t i = atomicAdd(&s.in_few, 1u);
+      if (i < ST) s.few[i] = key_of(f + 0.f);
+    });
+    __syncthreads();
+    const uint32_t n = s.in_few;
+    if (n < 512) {
+      // (2^parts threads a token, each with its part of the others)
+      const int parts = min(__clz(n | 1) - 22, 6), token = t >> parts;
+      const bool own = token < static_cast<int>(n), other = token == static_cast<int>(n) && cut_here;
+      const uint32_t key = own ? s.few[token] : other ? low : 0;
+      const uint64_t single = key != 0 ? amount(value_of(key)) : 0;
+      if (token <= static_cast<int>(n)) {
+        s.hist[2 * token] = own ? single : single * low_ties;
+        s.hist[2 * token + 1] = key;
+      }
+      __syncthreads();
+      uint64_t above = 0;
+#pragma unroll 4
+      for (uint32_t j = t & ((1 << parts) - 1); j <= n; j += 1 << parts) {
+        const uint64_t w = s.hist[2 * j];
+        above += static_cast<uint32_t>(s.hist[2 * j + 1]) > key ? w : 0;
+      }
+      for (int off = 1; off < 1 << parts; off *= 2) above += lane_xor(above, off);
+      // the last key before which the amount is not reached
+      const bool first = (t & ((1 << parts) - 1)) == 0 && single != 0;
+      if (first && (above == 0 || static_cast<double>(before + above) < want)) atomicMin(&s.kmin, key);
+      __syncthreads();
+      cut = s.kmin;
+      if (first && key == cut) {
+        atomicAdd(&s.kmax, own ? 1u : low_ties);
+        s.before = before + above;  // (all write the same)
+        s.total = single;
+      }
+      __syncthreads();
+      const double more = ceil((want - static_cast<double>(s.before)) / static_cast<double>(s.total));
+      ties = min(s.kmax, static_cast<uint32_t>(fmax(more, 1.0)));
+      empty();
+      return;
+    }
     auto in_step = [&](float f) { return f > cutv && step_of(f) == bin && amount(f) != 0; };
     uint32_t lo = 0xffffffffu, hi = 0;
     tokens(stepped, [&](float f) {
@@ -503,8 +564,6 @@ __global__ void __launch_bounds__(ST) sample_kernel(const SampleArgs p) {
       atomicMax(&s.kmax, hi);
     }
     __syncthreads();
-    const uint32_t low = cut;
-    const bool cut_here = low_ties > 0 && step_of(cutv) == bin;
     lo = s.kmin;
     hi = s.kmax;
     if (cut_here) {
@@ -586,8 +645,8 @@ __global__ void __launch_bounds__(ST) sample_kernel(const SampleArgs p) {
     };
     for (int j = 0; j < n; j += run * ST)
       for (int i = j + t * run; i < min(j + (t + 1) * run, n); ++i) {
-        const float f = s.list[i];
-        const int at = s.list_at[i] / 512;
+        const float f = s.list[i].value;
+        const int at = s.list[i].at / 512;
         if (f > cutv) {
           if (at != piece) leave();
           piece = at;
@@ -611,8 +670,7 @@ __global__ void __launch_bounds__(ST) sample_kernel(const SampleArgs p) {
       uint32_t n = 0;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const uint64_t w = weight(v[e]);
-        sum += v[e] > cutv ? w : 0;
+        sum += weight(v[e] > cutv ? v[e] : -INFINITY);
         n += ties > 0 && v[e] == cutv;
       }
       sum = wave_scan(sum);

@@ -664,6 +664,102 @@ def test_sample_large_vocabularies(vocab):
         check_sample(l, "spyre", u, k=5000, p=0.99, m=1e-4)
 
 
+# ---- large buffers, several streams ---------------------------------------------
+
+@pytest.mark.gpu
+def test_caches_past_32_bits():
+    """Pages at both ends of caches of more than 2^32 elements give what pages of small ones
+    give, to the last bit."""
+    page, kv, d, n = 16, 2, 128, 61
+    pages = 2 ** 32 // (kv * page * d) + 8
+    places = torch.tensor([pages - 1, 0, pages // 2 + 1, pages - 7])
+    qkv = rand((n, 8 * d), 60, 1.0).to("spyre")
+    cos, sin = (x.to("spyre") for x in tables(n, d, torch.float32))
+    at = torch.arange(n)
+    got = []
+    for count, where in ((4, torch.arange(4)), (pages, places)):
+        k, v = (torch.empty(count, kv, page, d, dtype=torch.float16, device="spyre")
+                for _ in range(2))
+        q = ops.paged_append(qkv, cos, sin, at.to("spyre"),
+                             (where[at // page] * page + at % page).to("spyre"), k, v, 4)
+        table, lens = where[None].to("spyre"), torch.tensor([n]).to("spyre")
+        for new in (1, 16, n):
+            starts = torch.tensor([0, new]).to("spyre")
+            got.append(ops.paged_attention(q[n - new:], k, v, table, lens, starts, 0.09).cpu())
+        del k, v
+    for small, large in zip(got[:3], got[3:]):
+        assert torch.isfinite(small).all() and torch.equal(small, large)
+
+
+@pytest.mark.gpu
+def test_logits_past_32_bits():
+    rows, vocab = 2052, 1 << 20
+    l = torch.empty(rows, vocab, dtype=torch.float16, device="spyre")
+    last = rand((3, vocab), 61, 2.0)
+    l[rows - 3:].copy_(last)
+    u = uniforms(rows, 61)
+    got = ops.sample(l, u.to("spyre"), None, None, torch.full((rows,), 0.9).to("spyre"))
+    want = check_sample(last, "spyre", u[rows - 3:], p=0.9)
+    assert got[rows - 3:].tolist() == want
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_append_one_slot_twice(device):
+    """Each element is one of the two rows'; nothing else changes."""
+    a = _append_args(device, slots=torch.tensor([5, 20, 5]))
+    before = [a["k_cache"].cpu().clone(), a["v_cache"].cpu().clone()]
+    ops.paged_append(**a)
+    rows = []
+    for keep in ([5, 20, -1], [-1, 20, 5]):
+        b = _append_args(device, slots=torch.tensor(keep))
+        ops.paged_append(**b)
+        rows.append([b["k_cache"].cpu(), b["v_cache"].cpu()])
+    for i, name in enumerate(("k_cache", "v_cache")):
+        got = a[name].cpu()
+        assert ((got == rows[0][i]) | (got == rows[1][i])).all()
+        seen = torch.ones(2, 16, dtype=torch.bool)
+        seen.view(-1)[[5, 20]] = False
+        assert torch.equal(got[:, 0][seen], before[i][:, 0][seen])
+
+
+@pytest.mark.gpu
+def test_c_entries_on_two_streams():
+    """Calls on two streams at once, each with its own workspace and output."""
+    lib, dev = _capi.lib(), "cuda"
+    h, kv, d, page, b, n = 8, 2, 128, 16, 3, 700
+    pages = b * (n // page + 1)
+    k, v = (rand((pages, kv, page, d), 62 + i).to(dev) for i in range(2))
+    q = rand((b, h, d), 64).to(dev)
+    table = torch.randperm(pages, generator=torch.Generator().manual_seed(1)).view(b, -1).to(dev)
+    lens = torch.tensor([n, n - 333, 1], device=dev)
+    starts = torch.arange(b + 1, device=dev)
+    logits, u = rand((b, 49155), 65, 2.0).to(dev), uniforms(b, 65).to(dev)
+    share = torch.full((b,), 0.9, device=dev)
+    bytes_ = lib.sph_paged_attention_workspace_bytes(b, b, h, kv, d, table.shape[1] * page)
+    runs = []
+    for i in range(2):
+        runs.append((torch.cuda.Stream(), torch.empty(bytes_, dtype=torch.uint8, device=dev),
+                     torch.zeros(b, h, d, dtype=torch.float16, device=dev),
+                     torch.zeros(b, dtype=torch.int64, device=dev)))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for stream, ws, out, tokens in runs:
+            s = stream.cuda_stream
+            assert lib.sph_paged_attention(
+                _capi.F16, b, b, h, kv, d, q.data_ptr(), h * d, d, k.data_ptr(), *k.stride()[:3],
+                v.data_ptr(), *v.stride()[:3], pages, page, table.data_ptr(), table.shape[1],
+                table.shape[1], lens.data_ptr(), starts.data_ptr(), None, 0, 0, 0.09,
+                out.data_ptr(), ws.data_ptr(), bytes_, None, s) == 0
+            assert lib.sph_sample(_capi.F16, b, 49155, logits.data_ptr(), 49155, u.data_ptr(), None,
+                                  None, share.data_ptr(), None, tokens.data_ptr(), s) == 0
+    torch.cuda.synchronize()
+    want = ops.paged_attention(*(x.cpu().to("spyre") for x in (q, k, v, table, lens, starts)), 0.09)
+    drawn = ops.sample(logits.cpu().to("spyre"), u.cpu().to("spyre"), None, None,
+                       share.cpu().to("spyre"))
+    for _, _, out, tokens in runs:
+        assert torch.equal(out.cpu(), want.cpu()) and torch.equal(tokens.cpu(), drawn.cpu())
+
+
 # ---- refusals ----------------------------------------------------------------
 
 def _append_args(device, **kw):

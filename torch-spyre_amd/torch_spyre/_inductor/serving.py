@@ -114,7 +114,7 @@ def paged_append(qkv, cos, sin, positions, slots, k_cache, v_cache, n_heads: int
     with rot(y) = (-y2, y1) for the halves y1, y2 and rows of cos / sin [positions,
     head_dim].  slots[token] = page * page_size + offset says where the token's key
     and value go; below 0 the token is padding, its queries are zeros.  fp32 inside,
-    rounded once.  Slots have to differ."""
+    rounded once.  Slots have to differ: of one named twice each element is either row's."""
     _paged_append_check(qkv, cos, sin, positions, slots, k_cache, v_cache, n_heads, q_norm, k_norm)
     pages, kv, page, d = k_cache.shape
     rows = (slots >= 0).nonzero()[:, 0]

@@ -295,6 +295,11 @@ STEPS = [
     ([150], [290], 8, 2, 128, 32, "head"),
     ([130, 1, 200], [130, 512, 411], 3, 1, 128, 16, "token"),
     ([2] * 300, [2 + i % 40 for i in range(300)], 2, 1, 64, 16, "head"),
+    ([37] + [0] * 20 + [1] * 9 + [0] * 30, [340] + [9] * 20 + list(range(60, 150, 10)) + [0] * 30,
+     8, 2, 128, 16, "head"),
+    ([1] * 30 + [70], [200 + 7 * i for i in range(30)] + [500], 4, 2, 128, 16, "token"),
+    ([1, 4], [70, 300], 24, 1, 64, 16, "head"),
+    ([1, 1, 1], [70, 300, 9], 24, 1, 128, 16, "head"),
 ]
 
 

@@ -16,16 +16,16 @@
 // Layout of the work:
 //   * A unit is (sequence, KV head, tile of rows): the G = H / Hkv query heads of
 //     a KV head are rows of one tile (row r = new token r / G, head r % G), so K
-//     and V are read once for all of them.  A wave takes 16 RT rows; the 4 waves of
-//     a workgroup take RW = 1, 2 or 4 groups of rows, by the rows that the
-//     sequence has, and split the keys 4 / RW ways.
+//     and V are read once for all of them.  Where single tokens are decoded, a wave
+//     takes 16 rows; the 4 waves of a workgroup take 1, 2 or 4 groups of rows, by the
+//     rows that the sequence has, and split the keys 4, 2 or 1 ways.
 //   * The lengths are known on the device only, so the launch has a fixed grid and
 //     every workgroup works out its share: units cut into items of 128 keys,
 //     an equal run of items for each workgroup.  A unit that ends up in several
 //     workgroups leaves partial (m, l, O) in the workspace, which a second
 //     kernel merges in a fixed order.  The same launch thus serves any
 //     lengths (a captured graph's too).
-//   * No LDS in the key loop.  S^T = K Q^T on 16x16x32 MFMAs: a lane's K
+//   * No LDS in that key loop.  S^T = K Q^T on 16x16x32 MFMAs: a lane's K
 //     fragment is 16 bytes of a key row, loaded straight from the cache.  A lane then
 //     holds scores of one query (column lane % 16) for keys 4 (lane / 16) + r,
 //     which are the 8 values that O^T += V^T P^T wants from it, in registers:
@@ -33,9 +33,9 @@
 //     j}.  For V^T each lane loads D / 16 consecutive head dims of its 8 keys
 //     (whole cache rows over 16 lanes) and turns the 8 x D / 16 block with byte
 //     permutes; head dim D / 16 m + t is row m of the product's tile t.
-//   * Sequences with more than 64 rows (128-row tiles, every wave its own rows) would
-//     ask the caches for each key four times: their K and V pass through LDS, 64
-//     keys a stage, two stages, a row's 16-byte chunks swapped by the row's number so that
+//   * More tokens (128-row tiles, every wave 32 rows of its own) would ask the
+//     caches for each key four times: their K and V pass through LDS, 64 keys a stage,
+//     two stages, a row's 16-byte chunks swapped by the row's number so that
 //     fragments are read without bank conflicts (V^T by transposing reads).
 //   * A workgroup's next unit is looked up, and its first loads are under way, before
 //     the results of the one before it leave.
@@ -107,9 +107,9 @@ struct Seq {
   int n, len, rows, rw, tiles;  // rw: groups of rows per workgroup
 };
 
-// Forms of the kernel, by the rows that a sequence has on average: a wave takes 16 rows, or
-// 32, or 32 of a 128-row tile whose keys pass through LDS.  Each serves any number.
-enum { DECODE, TREE, WIDE };
+// Forms of the kernel: a wave takes 16 rows, or 32 of a 128-row tile whose keys pass through
+// LDS.  Each serves any number.
+enum { DECODE, WIDE };
 constexpr int rows_of(int form) { return form == DECODE ? 16 : 32; }  // of a wave
 
 template <int FORM>
@@ -950,9 +950,15 @@ __global__ void __launch_bounds__(PT) paged_attn_merge(const PagedArgs p, int gr
   }
 }
 
-// The form for sequences of this many rows on average.
+// The host knows how many tokens come, not whose they are.  One a sequence at most: the form
+// for them (64 ragged sequences of up to 4000 keys 122 us, 141 in the other; as many heads of
+// keys as of queries 99 and 104; 131072 keys 104 and 106).  More are trees or pieces of
+// prompts, perhaps among single tokens: 4 of 131072 keys take 106 and 107 us, 16 of them 183
+// and 116, 63 single tokens beside a piece of 150 take 205 and 127 (2000 keys each).  (A third
+// form, 32 rows a wave without LDS, was ahead of both at 6 tokens a sequence only, 157 us to
+// 169, and took 235 for 63 tokens beside a piece of 512, which now take 152.)
 int form_of(int64_t tokens, int64_t batch, int64_t g) {
-  return tokens * g <= 16 * batch ? DECODE : tokens * g <= 64 * batch ? TREE : WIDE;
+  return tokens <= batch && g <= 16 ? DECODE : WIDE;
 }
 // Workgroups: what the chip holds at once, or fewer when the shapes cannot hold as many items.
 int64_t paged_grid(int64_t tokens, int64_t batch, int64_t n_kv, int64_t g, int64_t max_keys) {
@@ -1071,7 +1077,6 @@ extern "C" int sph_paged_attention(
   };
   auto by_rows = [&](auto tt, auto dd) {
     if (form == DECODE) by_page(tt, dd, std::integral_constant<int, DECODE>{});
-    else if (form == TREE) by_page(tt, dd, std::integral_constant<int, TREE>{});
     else by_page(tt, dd, std::integral_constant<int, WIDE>{});
   };
   auto by_dim = [&](auto tt) {

@@ -769,7 +769,8 @@ int sph_paged_append(sph_dtype dtype, sph_dtype table_dtype, sph_dtype norm_dtyp
  * A page, length or start out of range stores 3 to *error_word (may be null);
  * reads stay inside the caches, and what the sequence's rows hold is then not specified.
  * dtype F16 / BF16, head_dim 64 or 128, rows at any alignment; at most 4096
- * sequences, 2^26 query rows, 2^30 keys a sequence.  The workspace
+ * sequences, 2^24 - 1 tokens, 2^26 query rows, 2^30 keys a sequence, rows of a
+ * page less than 2^26 elements apart.  The workspace
  * (16-byte aligned, sph_paged_attention_workspace_bytes with max_keys =
  * table_width * page_size) holds partial results; calls that share one have
  * to be ordered. */

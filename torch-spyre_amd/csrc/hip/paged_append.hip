@@ -11,9 +11,12 @@
 // queries are zeros and its position is not looked at.  A slot or position
 // outside its range sets the error word and is treated like padding.
 //
-// Bound by memory: every element is read and written once.  D / 8 lanes hold a head in 16-byte chunks;
-// the rotation's partner is half a head away and comes by a lane exchange, the
-// mean by D / 16 of them.  Rows and cache rows may begin at any element (16-byte
+// Bound by memory: every element is read and written once.  With 32 query and 2 x 8 further
+// heads of 128, fp16, 8192 tokens take 42.2 us (206 MB, 4.9 TB/s; a copy of 1 GiB runs at 5.0),
+// 2331 with norms 15.3 (3.9 TB/s), up to 120 the host's call, 5.3 (the kernel 2.6 to 3.7).
+// A workgroup takes 2048 elements of one token, so that one token already has several and
+// none walks: D / 8 lanes hold a head in 16-byte chunks; the rotation's partner is half a head
+// away and comes by a lane exchange, the mean by log2(D / 8) of them.  Rows and cache rows may begin at any element (16-byte
 // accesses off their natural alignment).
 #include "sph_common.h"
 

@@ -39,8 +39,15 @@
 //     fragments are read without bank conflicts (V^T by transposing reads).
 //   * A workgroup's next unit is looked up, and its first loads are under way, before
 //     the results of the one before it leave.
-//   * Probabilities round to the element type for the second product; scores,
-//     maxima, sums and O stay fp32; O rounds once.
+//   * Probabilities round to the element type for the second product (the matrix cores take
+//     both operands in one type; at most half a step of a share of O); scores, maxima,
+//     sums and O stay fp32; O rounds once.
+//
+// What bounds it (32 query heads over 8 of 128): decoding and trees of one long sequence
+// the bytes of K and V, 64 ragged sequences of up to 4000 keys 121 us (530 MB, 4.4
+// TB/s), 131072 keys 104 us for a token and 116 for a tree of 16; four sequences of 1152
+// keys the latency of two kernels, 18 us; pieces of prompts the softmax beside the products, 3 x
+// 777 tokens over 2825 keys 188 us (93 GFLOP, matrix cores busy a fifth of the time).
 #include <algorithm>
 #include <type_traits>
 

@@ -29,12 +29,19 @@
 //     2048 equal steps of the logit below the maximum (each holds few tokens, so the
 //     atomics seldom meet), then over the ordered bit patterns of the step that the cut
 //     falls into.  What is cut is described by that pattern and by how many of the
-//     tokens with it stay; what stays is listed if there is room.  The draw needs
+//     tokens with it stay; what stays is listed if there is room.  (Of a list the step's
+//     tokens are few, and each is weighed by a thread of its own, which adds up those before it:
+//     24 rows of top-p 50 us with the histograms of patterns, 41.5 so.)  The draw needs
 //     the sums of all 512-token pieces and then one wave in the piece that holds the token.
 //
 // One workgroup per row, which reads it again where it is needed, a turn of loads ahead.  (Four
 // turns ahead, the loops four times as long, doubled every pass's time: most
-// instructions run a few times only, so fetching them counts.)
+// instructions run a few times only, so fetching them counts.)  Several workgroups a row, in
+// four launches (maxima, sums, lists, the rest), took 38.7 us for 42.4 at 24 rows of top-p,
+// but 22.6 for 14.2 with top-k.
+//
+// Measured: 1 row of 49155 with every filter 14.3 us, 24 rows of top-p 0.9 41.5 us, 256
+// rows of 131072 fp32 logits without filters 48.9 us (2.7 TB/s; 24 of it the weights).
 #include <algorithm>
 #include <type_traits>
 

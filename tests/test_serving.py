@@ -462,6 +462,25 @@ def test_attention_more_new_tokens_than_the_mask_has_columns(device):
             torch.spyre.synchronize()
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("page", [16, 20])
+@pytest.mark.parametrize("news", [[1], [1, 0, 1], [9], [1, 130, 0, 2]])
+def test_attention_new_tokens_without_pages(news, page, masked, device):
+    """A block table of no columns holds no keys, new ones neither: the call is refused and the
+    table, which has no memory, not read."""
+    n = sum(news)
+    kc = new_cache(2, 2, page, 128, torch.float16).to(device)
+    mask = torch.ones(n, max(news), dtype=torch.bool, device=device) if masked else None
+    for lens in (news, [0] * len(news), [x + 5 for x in news]):
+        with pytest.raises(IndexError):
+            ops.paged_attention(rand((n, 4, 128), 12).to(device), kc, kc,
+                                torch.zeros(len(news), 0, dtype=torch.int64, device=device),
+                                torch.tensor(lens).to(device),
+                                torch.tensor([0] + news).cumsum(0).to(device), 0.1, mask)
+            torch.spyre.synchronize()
+
+
 # ---- sample ------------------------------------------------------------------
 
 def token64(l, u, t=1.0, k=0, p=1.0, m=0.0):

@@ -319,6 +319,11 @@ paged_attn_kernel(const PagedArgs) {
     const ArgPtr p = args();
     return p->table[u.b * p->ld_table + min(blk + lane, last_block(u)) * KPB / p->page];
   };
+  // Those of its first keys.  (New tokens of a sequence that is out of range make a unit without
+  // keys, for which nothing is looked up: the table may have no columns.)
+  auto first_pages = [&](const Unit& u) {
+    return u.keys > 0 ? page_at(u, first_key(u) / KPB) : int64_t{0};
+  };
 
   u32x4 qf[RT][KK];
   int tok[RT];
@@ -443,7 +448,7 @@ paged_attn_kernel(const PagedArgs) {
   Unit u{}, next{};
   if (item < end) {
     u = locate(item, -1);
-    ahead = page_at(u, first_key(u) / KPB);
+    ahead = first_pages(u);
     begin(u);
   }
   while (item < end) {
@@ -453,7 +458,7 @@ paged_attn_kernel(const PagedArgs) {
     int64_t ahead_next = 0;
     if (more_units) {
       next = locate(item + (u.c1 - u.c0), u.b);
-      ahead_next = page_at(next, first_key(next) / KPB);
+      ahead_next = first_pages(next);
     }
     const int tile0 = u.tile * R * u.s.rw, row0 = tile0 + (wave % u.s.rw) * R;
     const int kend = u.kend, ctx = u.ctx;
@@ -807,7 +812,7 @@ paged_attn_kernel(const PagedArgs) {
       u = next;
     } else if (item < end) {
       u = locate(item, u.b);
-      ahead = page_at(u, first_key(u) / KPB);
+      ahead = first_pages(u);
       begin(u);
     }
     __syncthreads();

@@ -894,6 +894,38 @@ def test_no_gradients(device):
     assert not ops.sample(l.detach(), torch.rand(3).to(device)).requires_grad
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("tokens", [3, 0])
+def test_append_raises_the_versions_of_the_caches(tokens, device):
+    """A backward pass that saved a cache raises once the cache has been written."""
+    a = _append_args(device)
+    if tokens == 0:
+        a.update({n: a[n][:0] for n in ("qkv", "positions", "slots")})
+    names = ("k_cache", "v_cache")
+    for name in names:
+        before = [a[n]._version for n in names]
+        # (read through a view: it has its base's version)
+        w = torch.ones(1, 16, 64, dtype=torch.float16).to(device).requires_grad_()
+        y = (w * a[name][1]).sum()
+        with torch.no_grad():
+            ops.paged_append(**a)
+        assert all(a[n]._version > x for n, x in zip(names, before))
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_append_to_inference_tensors(device):
+    want = _append_args(device)
+    q = ops.paged_append(**want)
+    with torch.inference_mode():
+        a = {n: x.clone() if isinstance(x, torch.Tensor) else x
+             for n, x in _append_args(device).items()}
+        assert torch.equal(ops.paged_append(**a).cpu(), q.cpu())
+        for n in ("k_cache", "v_cache"):
+            assert a[n].is_inference() and torch.equal(a[n].cpu(), want[n].cpu())
+
+
 def test_fakes():
     from torch._subclasses.fake_tensor import FakeTensorMode
 

@@ -57,6 +57,13 @@ void check_caches(const at::Tensor& k, const at::Tensor& v, const at::Tensor& li
   check_strided(v, "v_cache");
 }
 
+// The kernel writes `t` past the dispatcher: its version rises here, so that a backward pass
+// which saved it before raises instead of taking the new values.  (Inference tensors have no
+// version and are saved by none.)
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 at::Tensor paged_append(const at::Tensor& qkv_in, const at::Tensor& cos_in,
                         const at::Tensor& sin_in, const at::Tensor& positions_in,
                         const at::Tensor& slots_in, at::Tensor& k_cache, at::Tensor& v_cache,
@@ -106,6 +113,8 @@ at::Tensor paged_append(const at::Tensor& qkv_in, const at::Tensor& cos_in,
   check_strided(cos, "cos");
   check_strided(sin, "sin");
   at::Tensor q = empty_spyre({tokens, n_heads, d}, dt, qkv.device());
+  written(k_cache);
+  written(v_cache);
   if (tokens == 0) return q;
   const int dev = qkv.get_device();
   SPYRE_SPH_CHECK(sph_paged_append(

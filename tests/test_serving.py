@@ -651,6 +651,20 @@ def test_sample_borders_of_the_filters(vocab, device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("vocab", [5, 3000, 20000])
+@pytest.mark.parametrize("t", [1e-45, 1e-40, 1.3e-37, 1.4e-37, 1e-36])
+def test_sample_smallest_temperatures_and_shares(t, vocab, device):
+    """A row has a token however small its temperature and top-p are."""
+    l = rand((6, vocab), vocab, 2.0, torch.float32)
+    l[3:] = torch.round(l[3:])
+    u = uniforms(6, 1)
+    for p in (None, 0.0, -1.0, 1e-30, 0.5):
+        for k in (None, 3, 2000):
+            check_sample(l, device, u, t=t, p=p, k=k)
+            check_sample(l.half(), device, u, t=t, p=p, k=k, m=0.5)
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_sample_bounds_of_the_random_number(device):
     l = torch.tensor([[0.0, 1.0, -INF, 2.0, -INF]]).expand(5, 5).contiguous()
     u = torch.tensor([0.0, 1.0, 5.0, -3.0, NAN])

@@ -610,7 +610,9 @@ __global__ void __launch_bounds__(ST) sample_kernel(const SampleArgs p) {
   if (share < 1.f)
     move_cut([&](float f) { return weight(f); },
              [&](uint64_t all) {
-               return fmax(static_cast<double>(share), 0.0) * static_cast<double>(all);
+               // (one unit at least: of the first steps some may be empty, at a temperature
+               // too small for them even that of the largest logit)
+               return fmax(static_cast<double>(share) * static_cast<double>(all), 1.0);
              });
   // The least value that min-p lets through (the largest weight is 1), to the last bit.
   float least = -INFINITY;

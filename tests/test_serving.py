@@ -391,6 +391,35 @@ def test_attention_large_scores(dtype, device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("gap", [0.0, 9.0, 15.0, 17.0, 17.5, 20.0, 22.0])
+@pytest.mark.parametrize("new", [1, 2])
+def test_attention_one_key_far_above_many(new, gap, dtype, device):
+    """The first key has no value and weighs e^gap times as much as every other: what
+    thousands of small weights add up to is kept.  With n others of value 1 the result is
+    n / (n + e^gap).  It may be off by half a step of every weight and of itself, 2^-12 of
+    it through exp (an exponent of 32 at most, as a product in fp32), and in fp16 by 2^-32 for
+    each weight below 2^-21, whose step is coarser.  (300 sequences share the pages, so that one
+    workgroup has all keys of a row, or most of them.)"""
+    b, m, kv, d, page = 300, 4096, 2, 64, 16
+    k = torch.zeros(m // page, kv, page, d, dtype=dtype)
+    v = torch.ones_like(k)
+    k[0, :, 0, 0] = gap
+    v[0, :, 0] = 0
+    q = torch.zeros(b * new, kv, d, dtype=dtype)
+    q[..., 0] = 1
+    got = ops.paged_attention(*(x.to(device) for x in (
+        q, k, v, torch.arange(m // page).expand(b, -1).contiguous(), torch.full((b,), m),
+        torch.arange(0, b * new + 1, new))), 1.0).cpu().double().view(b, new, kv, d)
+    n = torch.arange(m - new, m).double()[:, None, None]
+    want = n / (n + math.exp(gap))
+    tail = n * 2.0 ** -32 if dtype == torch.float16 else 0.0
+    bound = want * (2 * half(dtype) * (1 + 2.0 ** -4) + 2.0 ** -12) + tail
+    off = (got - want).abs()
+    assert bool((off <= bound).all()), (off / bound).max()
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_attention_strided_queries_tables_and_masks(device):
     news, lens = [5, 2], [60, 33]
     mask = tree(news, 6, 4)

@@ -40,8 +40,12 @@
 //   * A workgroup's next unit is looked up, and its first loads are under way, before
 //     the results of the one before it leave.
 //   * Probabilities round to the element type for the second product (the matrix cores take
-//     both operands in one type; at most half a step of a share of O); scores, maxima,
-//     sums and O stay fp32; O rounds once.
+//     both operands in one type): half a step of each key's share of O.  fp16 has that
+//     step from 2^-14 on only and nothing below 2^-25, so there they are held 2^7 times as
+//     large (at most 2^15, with 2^8 for a maximum that the reference does not follow; the
+//     division by the sum, which holds the factor too, takes it out): half a step from 2^-21 of the
+//     largest on, below it 2^-32 of the largest.  Scores, maxima, sums and O stay fp32; O rounds
+//     once.
 //
 // What bounds it (32 query heads over 8 of 128): decoding and trees of one long sequence
 // the bytes of K and V, 64 ragged sequences of up to 4000 keys 121 us (530 MB, 4.4
@@ -206,6 +210,7 @@ paged_attn_kernel(const PagedArgs) {
   constexpr int STAGE = SK * D * 2;    // bytes of a stage's K (or V)
   constexpr int MERGE = 4 * R * PITCH * 4, LDS = FORM == WIDE && 4 * STAGE > MERGE ? 4 * STAGE : MERGE;
   static_assert(SP <= KK, "a stage fits the registers of a step's keys");
+  constexpr float kLift = __is_same(T, half_t) ? 7.f : 0.f;  // log2 of the probabilities' factor
   extern __shared__ int64_t prefix[];  // [batch + 1] items before a sequence
   __shared__ __attribute__((aligned(1024))) char lds[LDS];
   __shared__ float mg_m[4][R], mg_l[4][R];
@@ -520,7 +525,7 @@ paged_attn_kernel(const PagedArgs) {
         for (int d = 0; d < DT; ++d) o[i][d] *= a;
         m[i] = to;
       }
-      const float ref = m[i] == -INFINITY ? 0.f : -m[i];
+      const float ref = m[i] == -INFINITY ? 0.f : kLift - m[i];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float pr = __builtin_amdgcn_exp2f(fmaf(sc[j >> 2][j & 3], c, ref));

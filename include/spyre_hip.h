@@ -766,8 +766,9 @@ int sph_paged_append(sph_dtype dtype, sph_dtype table_dtype, sph_dtype norm_dtyp
  * nothing and rows of no sequence are 0.  Query head h reads KV head
  * h / (n_heads / n_kv_heads).  Keys and values that a row does not see have
  * no effect on it, whatever they hold.
- * A page, length or start out of range stores 3 to *error_word (may be null);
- * reads stay inside the caches, and what the sequence's rows hold is then not specified.
+ * A length (0 to table_width * page_size, also without new tokens), start or page of a sequence
+ * with new tokens out of range stores 3 to *error_word (may be null); reads stay inside the
+ * caches, and what the sequence's rows hold is then not specified.
  * dtype F16 / BF16, head_dim 64 or 128, rows at any alignment; at most 4096
  * sequences, 2^24 - 1 tokens, 2^26 query rows, 2^30 keys a sequence, rows of a
  * page less than 2^26 elements apart.  The workspace

@@ -510,6 +510,33 @@ def test_attention_new_tokens_without_pages(news, page, masked, device):
             torch.spyre.synchronize()
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("page", [16, 20])
+def test_attention_sequences_without_new_tokens(page, device):
+    """Their lengths have to be in range as the others', their pages are not looked at."""
+    kc = new_cache(2, 2, page, 128, torch.float16).to(device)
+    q = rand((3, 4, 128), 13).to(device)
+
+    def call(lens, starts, table, caches=kc):
+        out = ops.paged_attention(q, caches, caches, torch.tensor(table).to(device),
+                                  torch.tensor(lens).to(device), torch.tensor(starts).to(device), 0.1)
+        torch.spyre.synchronize()
+        return out.cpu()
+
+    want = call([9], [0, 3], [[1]])
+    for other in (0, 1, page):
+        for entry in (-1, 0, 2 ** 40):
+            assert torch.equal(call([9, other], [0, 3, 3], [[1], [entry]]), want)
+            assert torch.equal(call([other, 9], [0, 0, 3], [[entry], [1]]), want)
+    for other in (-1, page + 1, 2 ** 40, -2 ** 40):
+        with pytest.raises(IndexError):
+            call([9, other], [0, 3, 3], [[1], [0]])
+    # no pages at all: nothing is appended, nothing asked
+    assert not call([page, 0], [3, 3, 3], [[0], [0]], kc[:0]).any()
+    with pytest.raises(IndexError):
+        call([9], [0, 3], [[0]], kc[:0])
+
+
 # ---- sample ------------------------------------------------------------------
 
 def token64(l, u, t=1.0, k=0, p=1.0, m=0.0):

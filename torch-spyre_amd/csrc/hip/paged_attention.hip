@@ -134,7 +134,7 @@ __device__ inline Seq sequence(int b, bool report) {
   }
   s.n = static_cast<int>(s1 - s0);
   const bool bad = len < s.n || len > p->width * p->page ||
-                   (p->mask != nullptr && s.n > p->mask_w) || (len > 0 && p->n_pages == 0);
+                   (p->mask != nullptr && s.n > p->mask_w) || (s.n > 0 && p->n_pages == 0);
   s.len = bad ? 0 : static_cast<int>(len);
   if (bad && report && p->err != nullptr) *p->err = kPagedIndex;
   s.rows = s.n * p->g;

@@ -188,7 +188,9 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, q_starts, scale:
     sees every key before the new ones and, of the new ones, those j with
     mask[q_starts[b] + i, j] (a tree's ancestors and itself, say), or without a
     mask j <= i.  Returns softmax(scale q k^T) v over what is seen, like q; rows that see
-    nothing, and rows before the first and behind the last sequence's, are zeros."""
+    nothing, and rows before the first and behind the last sequence's, are zeros.  Of a
+    sequence without new tokens only the length is looked at: it has to be one that the block
+    table holds (0, say), its pages may be anything."""
     _paged_attention_check(q, k_cache, v_cache, block_table, seq_lens, q_starts, scale, mask)
     op, page = "paged_attention", k_cache.shape[2]
     out = q.new_zeros(q.shape)
@@ -197,10 +199,10 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, q_starts, scale:
         first, n = starts[b], starts[b + 1] - starts[b]
         if first < 0 or n < 0 or starts[b + 1] > q.shape[0]:
             raise IndexError(f"{op}: q_starts out of range")
-        if n == 0:
-            continue
         if m < n or m > block_table.shape[1] * page or (mask is not None and n > mask.shape[1]):
             raise IndexError(f"{op}: length out of range")
+        if n == 0:
+            continue
         pages = block_table[b, :-(-m // page)]
         _index((pages < 0) | (pages >= k_cache.shape[0]), op, "page")
         k, v = (c[pages].transpose(1, 2).reshape(-1, c.shape[1], c.shape[3])[:m]

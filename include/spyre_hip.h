@@ -741,7 +741,8 @@ int sph_rope(sph_dtype dtype, const void* x, void* y,
  * A slot below 0 marks a padding row: nothing is appended, its queries are
  * zeros, its position is not read.  A slot or position out of range stores
  * 3 to *error_word (may be null) and is treated like padding.  Slots of one call have to
- * differ; one that is named twice holds elements of either row.
+ * differ; one that is named twice holds elements of either row.  Nothing else may lie in
+ * the caches' memory.
  * dtype F16 / BF16 (rows and caches), table_dtype and norm_dtype that or F32;
  * head_dim 64 or 128; rows at any alignment; tokens * ceil((n_heads + 2
  * n_kv_heads) * head_dim / 2048) below 2^24. */

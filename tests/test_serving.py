@@ -949,6 +949,21 @@ def test_refusals_of_the_device():
                                    q_starts=torch.zeros(5001, dtype=torch.int64).to("spyre")))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["qkv", "cos", "sin", "q_norm", "k_norm", "positions", "slots"])
+@pytest.mark.parametrize("cache", ["k_cache", "v_cache"])
+def test_append_refuses_inputs_in_the_caches(cache, name):
+    """Rows, tables, weights and indices that lie in a cache would be read while it is written."""
+    a = _append_args("spyre", q_norm=rand((64,), 6), k_norm=rand((64,), 7))
+    before = a[cache].cpu()
+    flat = a[cache].view(-1)
+    if a[name].dtype == torch.int64:
+        flat = flat.view(torch.int64)
+    with pytest.raises(RuntimeError, match="overlap|memory location"):
+        ops.paged_append(**dict(a, **{name: flat[:a[name].numel()].view(a[name].shape)}))
+    assert torch.equal(a[cache].cpu(), before)
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_no_gradients(device):
     for call, args, name in ((ops.paged_append, _append_args(device), "qkv"),

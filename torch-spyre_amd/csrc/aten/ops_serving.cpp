@@ -76,6 +76,11 @@ at::Tensor paged_append(const at::Tensor& qkv_in, const at::Tensor& cos_in,
   at::assert_no_internal_overlap(k_cache);
   at::assert_no_internal_overlap(v_cache);
   at::assert_no_overlap(k_cache, v_cache);
+  // (a workgroup would read what another has written)
+  for (const at::Tensor* in : {&qkv_in, &cos_in, &sin_in, &positions_in, &slots_in}) {
+    at::assert_no_overlap(k_cache, *in);
+    at::assert_no_overlap(v_cache, *in);
+  }
   const int64_t kv = k_cache.size(1), page = k_cache.size(2), d = k_cache.size(3);
   TORCH_CHECK(n_heads > 0 && qkv_in.dim() == 2 && qkv_in.size(1) == (n_heads + 2 * kv) * d,
               "paged_append: qkv must be [tokens, (n_heads + 2 n_kv_heads) * head_dim] = [tokens, ",
@@ -100,6 +105,8 @@ at::Tensor paged_append(const at::Tensor& qkv_in, const at::Tensor& cos_in,
                 "paged_append: norm weights must have qkv's type or fp32, got ", nt);
     TORCH_CHECK(i == 0 || !norms[0].defined() || norms[0].scalar_type() == nt,
                 "paged_append: q_norm and k_norm must have one type");
+    at::assert_no_overlap(k_cache, *in);
+    at::assert_no_overlap(v_cache, *in);
     norms[i] = vec(*in, d, nt, qkv_in, op, i == 0 ? "q_norm" : "k_norm");
   }
   const at::Tensor qkv =

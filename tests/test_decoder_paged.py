@@ -245,3 +245,14 @@ def test_two_graphs_of_one_cache():
         del junk
     for x in graphs:
         x.reset()
+
+
+def test_plan_gives_no_slots_of_other_sequences():
+    plan = D.PagedPlan([40, 5, 0], 16)
+    assert plan.pages == 4 and plan.room == [48, 16, 0]
+    mine = [plan.slots(b, 0, n).tolist() for b, n in enumerate(plan.room)]
+    assert sorted(sum(mine, [])) == list(range(64))
+    assert plan.slots(1, 16, 0).numel() == 0
+    for b, first, n in ((0, 0, 49), (0, 48, 1), (1, 16, 1), (1, 7, 10), (2, 0, 1), (0, -1, 2)):
+        with pytest.raises(IndexError):
+            plan.slots(b, first, n)

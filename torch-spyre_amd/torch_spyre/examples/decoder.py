@@ -477,6 +477,7 @@ class PagedPlan:
     def __init__(self, lengths, page_size: int):
         self.page_size = page_size
         need = [-(-n // page_size) for n in lengths]
+        self.room = [n * page_size for n in need]
         self.pages = sum(need)
         self.table = torch.zeros(len(need), max(need + [1]), dtype=torch.int64)
         free = 0
@@ -488,6 +489,9 @@ class PagedPlan:
 
     def slots(self, b: int, first: int, n: int) -> torch.Tensor:
         """Slots of tokens first .. first + n - 1 of sequence b."""
+        if first < 0 or n < 0 or first + n > self.room[b]:
+            raise IndexError(f"tokens {first} to {first + n} of sequence {b}, whose pages hold "
+                             f"{self.room[b]}")
         at = torch.arange(first, first + n)
         return self.table[b, at // self.page_size] * self.page_size + at % self.page_size
 

@@ -256,3 +256,13 @@ def test_plan_gives_no_slots_of_other_sequences():
     for b, first, n in ((0, 0, 49), (0, 48, 1), (1, 16, 1), (1, 7, 10), (2, 0, 1), (0, -1, 2)):
         with pytest.raises(IndexError):
             plan.slots(b, first, n)
+
+
+def test_prompts_have_a_token():
+    """An empty prompt has no last row to go on from (the one before it is another's)."""
+    p, none = _params(), torch.zeros(0, dtype=torch.int64)
+    for prompts in ([none], [PROMPTS[0], none], [none, PROMPTS[0]]):
+        with pytest.raises(ValueError, match="at least one token"):
+            D.generate_paged(prompts, p, CFG, 2, "cpu")
+    with pytest.raises(ValueError, match="at least one token"):
+        D.generate_speculative(none, p, CFG, 2, "cpu", lambda s: ([], []))

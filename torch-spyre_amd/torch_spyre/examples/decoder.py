@@ -546,6 +546,8 @@ def generate_paged(prompts, params: dict, cfg: DecoderConfig, steps: int, device
     step_fn = step_fn or step_paged
     ops, dt, B = torch.ops.spyre, params["embed"].dtype, len(prompts)
     lens = [int(p.shape[0]) for p in prompts]
+    if min(lens) < 1:
+        raise ValueError("a prompt has at least one token")
     plan = PagedPlan([n + steps for n in lens], page_size)
     cos, sin = rope_tables(cfg, max(lens) + steps, device, torch.float32)
     cache = new_paged_cache(cfg, plan.pages, page_size, device, dt)
@@ -625,6 +627,8 @@ def generate_speculative(prompt, params: dict, cfg: DecoderConfig, steps: int, d
     keys and values behind each other.  Returns (the `steps` tokens that greedy decoding
     gives, rounds taken)."""
     dt, n = params["embed"].dtype, int(prompt.shape[0])
+    if n < 1:
+        raise ValueError("a prompt has at least one token")
     plan = PagedPlan([n + steps + most], page_size)
     cos, sin = rope_tables(cfg, n + steps + most, device, torch.float32)
     cache = new_paged_cache(cfg, plan.pages, page_size, device, dt)

@@ -266,3 +266,20 @@ def test_prompts_have_a_token():
             D.generate_paged(prompts, p, CFG, 2, "cpu")
     with pytest.raises(ValueError, match="at least one token"):
         D.generate_speculative(none, p, CFG, 2, "cpu", lambda s: ([], []))
+
+
+@pytest.mark.parametrize("name", ["q_norm", "k_norm"])
+@pytest.mark.parametrize("eight_bit", [False, True])
+def test_norms_of_heads_are_refused_over_the_contiguous_cache(name, eight_bit):
+    """Left out there, they would give another model's logits."""
+    p = _params()
+    p["layers"][1][name] = torch.full((128,), 2.0, dtype=torch.float16)
+    if eight_bit:
+        p = D.quantize_params(p)
+    with pytest.raises(ValueError, match="step_paged"):
+        D.generate(_tokens(2, 5), p, CFG, 2, "cpu")
+    cos, sin = D.rope_tables(CFG, 8, "cpu")
+    for step in (D.decode_step, D.decode_step_static):
+        at = 3 if step is D.decode_step else torch.tensor([3])
+        with pytest.raises(ValueError, match="step_paged"):
+            step(_tokens(2), at, p, cos, sin, D.new_cache(CFG, 2, 8, "cpu"), CFG)

@@ -211,9 +211,16 @@ def _norm_after(i: int, params: dict):
     return layers[i + 1]["attn_norm"] if i + 1 < len(layers) else params["final_norm"]
 
 
+def _no_head_norms(w: dict):
+    if "q_norm" in w or "k_norm" in w:
+        raise ValueError("norms of query and key heads (q_norm, k_norm) are taken by step_paged "
+                         "and what is built on it, not over a contiguous cache")
+
+
 def _qkv(x, w: dict, cfg: DecoderConfig):
     """Q, K, V projections of x [..., hidden] (of its (codes, scales) for
     8-bit weights): one GEMM over the fused weight when the layer has one."""
+    _no_head_norms(w)
     nq, nkv = cfg.n_heads * cfg.head_dim, cfg.n_kv_heads * cfg.head_dim
     if "wqkv_fp8" in w:
         qkv = torch.ops.spyre.mm_fp8(*x, *w["wqkv_fp8"], w["attn_norm"].dtype)
@@ -363,6 +370,7 @@ def decode_step_static(tokens, pos, params: dict, cos, sin, cache, cfg: DecoderC
     xn = None  # as in decode_step
     for i, w in enumerate(params["layers"]):
         x = xn or _first_norm(h, w, cfg)
+        _no_head_norms(w)
         fp8 = "wqkv_fp8" in w
         if fused_attention and (fp8 or "wqkv" in w) and cfg.head_dim == 128:
             kc, vc = cache[i]
@@ -502,7 +510,8 @@ def step_paged(tokens, positions, slots, block_table, seq_lens, q_starts, params
     q_starts[b] .. q_starts[b + 1] - 1, at `positions` [T]; their keys and values go to
     `slots` [T] (-1: padding), and seq_lens [B] counts them in.  mask [T, N] (bool): which
     of its sequence's new tokens each of them sees (None: causal).  Returns the
-    logits of every token, or of `rows` (int64)."""
+    logits of every token, or of `rows` (int64).  A layer's q_norm and k_norm [head_dim], if it
+    has them, normalise the query and key heads."""
     ops = torch.ops.spyre
     layers = params["layers"]
     h = F.embedding(tokens, params["embed"])

@@ -283,3 +283,61 @@ def test_norms_of_heads_are_refused_over_the_contiguous_cache(name, eight_bit):
         at = 3 if step is D.decode_step else torch.tensor([3])
         with pytest.raises(ValueError, match="step_paged"):
             step(_tokens(2), at, p, cos, sin, D.new_cache(CFG, 2, 8, "cpu"), CFG)
+
+
+def _second_children(want, n, vocab):
+    """A draft that names up to three of the tokens `want`, which follow the prompt's n, each
+    behind a wrong one: the accepted nodes are never the first ones of their tree."""
+    def draft(seq):
+        tokens, parents, last = [], [], -1
+        for t in want[len(seq) - n:len(seq) - n + 3]:
+            tokens += [(t + 1) % vocab, t]
+            parents += [last, last]
+            last = len(tokens) - 1
+        return tokens, parents
+    return draft
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("page_size", [16, 5])
+def test_speculation_moves_accepted_nodes(page_size, device, monkeypatch):
+    """Tokens, and keys and values in the cache, are those of decoding one by one.  (This
+    prompt's two largest logits are 0.14 apart at every step, six times 2 % of the logits' root
+    mean square.)"""
+    caches, make = [], D.new_paged_cache
+    monkeypatch.setattr(D, "new_paged_cache",
+                        lambda *a, **kw: caches.append(make(*a, **kw)) or caches[-1])
+    p, prompt, steps = _to(_params(), device), _tokens(20, seed=111), 10
+    n = len(prompt)
+    want = D.generate_paged([prompt], p, CFG, steps, device, page_size)[0][0].tolist()
+    got, rounds = D.generate_speculative(prompt, p, CFG, steps, device,
+                                         _second_children(want, n, CFG.vocab), page_size)
+    assert got.tolist() == want and rounds == 3  # (one token, then four a round)
+    for one, tree in zip(*caches):
+        for a, b in zip(one, tree):
+            a, b = (x.cpu().transpose(1, 2).reshape(-1, 2, 128)[:n + steps - 1].double()
+                    for x in (a, b))
+            assert bool(((a - b).norm(dim=(1, 2)) < BOUND * a.norm(dim=(1, 2))).all())
+
+
+def test_speculation_copies_no_cache():
+    """Moving a few rows takes no tensor of a whole cache's size."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    large = []
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            out = func(*args, **(kwargs or {}))
+            new = all(r.alias_info is None for r in func._schema.returns)
+            if new and isinstance(out, torch.Tensor) and out.numel() >= 2000 * 256:
+                large.append(str(func))
+            return out
+
+    p, prompt, steps = _params(), _tokens(20, seed=111), 10
+    want = D.generate_paged([prompt], p, CFG, steps, "cpu")[0][0].tolist()
+    with Watch():
+        got, _ = D.generate_speculative(prompt, p, CFG, steps, "cpu",
+                                        _second_children(want, 20, CFG.vocab), most=2000)
+    assert got.tolist() == want
+    assert large == ["aten.zeros.default"] * (2 * CFG.n_layers), large

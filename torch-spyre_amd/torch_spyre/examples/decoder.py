@@ -671,13 +671,12 @@ def generate_speculative(prompt, params: dict, cfg: DecoderConfig, steps: int, d
             if not follow:
                 break
             path.append(follow[0])
-        if path != list(range(len(path))):  # accepted nodes move behind each other
-            old, new = plan.slots(0, first, len(tokens))[path], plan.slots(0, first, len(path))
-            for kc, vc in cache:
-                for c in (kc, vc):
-                    flat = c.transpose(1, 2).reshape(-1, *c.shape[1:2], c.shape[3])
-                    picked = flat.index_select(0, old.to(device))
-                    for j, s in enumerate(new.tolist()):
-                        c[s // page_size, :, s % page_size].copy_(picked[j])
+        # Accepted nodes move behind each other.  (None to a place that one of the next has to
+        # leave still: path[j] >= j.)
+        slots = plan.slots(0, first, len(tokens)).tolist()
+        for to, at in zip(slots, [slots[i] for i in path]):
+            if to != at:
+                for c in (c for kv in cache for c in kv):
+                    c[to // page_size, :, to % page_size].copy_(c[at // page_size, :, at % page_size])
         seq += [tokens[i] for i in path[1:]] + [best[path[-1]]]
     return torch.tensor(seq[n:n + steps]), rounds

@@ -341,3 +341,37 @@ def test_speculation_copies_no_cache():
                                         _second_children(want, 20, CFG.vocab), most=2000)
     assert got.tolist() == want
     assert large == ["aten.zeros.default"] * (2 * CFG.n_layers), large
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("compiled", [False, pytest.param(True, marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("eight_bit", [False, True])
+def test_logits_of_some_rows(eight_bit, compiled, device, monkeypatch):
+    """step_paged's `rows` gives the logits that all rows' would hold there, from an LM head
+    of those rows alone."""
+    if compiled and device == "cpu":
+        pytest.skip("compiled for spyre")
+    p = D.quantize_params(_params()) if eight_bit else _params()
+    p, heads, head = _to(p, device), [], D.lm_logits
+    if not compiled:
+        monkeypatch.setattr(D, "lm_logits", lambda h, p, c, x=None: heads.append(
+            (h if x is None else x[0]).shape[0]) or head(h, p, c, x))
+    torch._dynamo.reset()
+    step = torch.compile(D.step_paged) if compiled else D.step_paged
+    plan, n = D.PagedPlan([30], 16), 30
+    cos, sin = D.rope_tables(CFG, n, device, torch.float32)
+    at = torch.arange(n)
+
+    def call(rows):
+        cache = D.new_paged_cache(CFG, plan.pages, 16, device)
+        with torch.no_grad():
+            return step(PROMPTS[2].to(device), at.to(device), plan.slots(0, 0, n).to(device),
+                        plan.table.to(device), torch.tensor([n]).to(device),
+                        torch.tensor([0, n]).to(device), p, cos, sin, cache, CFG, None,
+                        None if rows is None else rows.to(device)).cpu()
+
+    rows = torch.tensor([29, 3, 3, 0])
+    some, every = call(rows), call(None)
+    assert some.shape == (4, CFG.vocab) and every.shape == (n, CFG.vocab)
+    assert _rel(some, every[rows]) < BOUND
+    assert compiled or heads == [4, n]

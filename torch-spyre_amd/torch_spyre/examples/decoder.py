@@ -531,14 +531,15 @@ def step_paged(tokens, positions, slots, block_table, seq_lens, q_starts, params
         a = ops.paged_attention(q, kc, vc, block_table, seq_lens, q_starts, scale, mask)
         a = a.view(a.shape[0], -1)
         if "wo_fp8" in w:
-            h, xn = _rest_of_layer_fp8(a, h, w, cfg, _norm_after(i, params))
+            # (where only some rows get logits, the last norm is of those)
+            some = rows is not None and i + 1 == len(layers)
+            h, xn = _rest_of_layer_fp8(a, h, w, cfg, None if some else _norm_after(i, params))
             continue
         h = h + F.linear(a, w["wo"])
         h = h + _mlp(F.rms_norm(h, (cfg.hidden,), w["mlp_norm"], cfg.eps), w, cfg)
-    if rows is not None and xn is None:
+    if rows is not None:
         h = h.index_select(0, rows)
-    logits = lm_logits(h, params, cfg, xn)
-    return logits if rows is None or xn is None else logits.index_select(0, rows)
+    return lm_logits(h, params, cfg, xn)
 
 
 def generate_paged(prompts, params: dict, cfg: DecoderConfig, steps: int, device, page_size=16,

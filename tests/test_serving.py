@@ -314,6 +314,56 @@ def test_attention(step, masked, dtype, device):
     Step(news, lens, h, kv, d, page, dtype, layout, mask, pad, lead, k=step).check(device)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("news,lens,h,kv,page,masked", [
+    ([1], [4100], 8, 2, 16, False), ([1, 1], [2177, 9000], 3, 1, 5, False),
+    ([16], [4100], 8, 2, 16, True), ([3, 1], [7000, 40], 6, 2, 20, False),
+    ([40], [4300], 6, 1, 16, False), ([40], [4300], 6, 1, 16, True), ([33, 5], [300, 5000], 4, 4, 32, True)])
+def test_attention_of_many_parts(news, lens, h, kv, page, masked, d, dtype):
+    """Keys of one tile of rows over more than 16 workgroups (each has 128 of them), whose parts
+    are merged by all groups of lanes together; tiles with few and with all rows.  Results
+    do not change from call to call."""
+    assert max(lens) > 16 * 128
+    s = Step(news, lens, h, kv, d, page, dtype, mask=tree(news, max(news), 5) if masked else None, k=31)
+    got = s.check("spyre")
+    for _ in range(3):
+        junk = torch.full((64, 1000), NAN, device="spyre")
+        assert torch.equal(s.run("spyre").cpu().double(), got)
+        del junk
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,m,h,kv,d", [(4097, 4097, 4, 2, 128), (2500, 6001, 3, 1, 64)])
+def test_attention_of_long_pieces(n, m, h, kv, d, dtype):
+    """Whole prompts and pieces of many tiles, beside a single token."""
+    s = Step([1, n], [77, m], h, kv, d, 16, dtype, k=33)
+    got = s.run("spyre").cpu().double()[1:]
+    k, v = (x.double() for x in s.keys(1))
+    half_step = half(dtype)
+    for j in range(h):
+        kj, vj = k[:, j * kv // h], v[:, j * kv // h]
+        p = torch.softmax((s.q[1:, j].double() @ kj.t() * s.scale)
+                          .masked_fill(~s.seen(1), -INF), -1)
+        want, a = p @ vj, p @ vj.abs()
+        bound = (half_step * (a + want.abs()) * (1 + 2.0 ** -4) + 2.0 ** -12 * a
+                 + m * 2.0 ** -32 * vj.abs().max())
+        off = (got[:, j] - want).abs()
+        assert bool((off <= bound).all()), (off / bound).max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("last", [1, 2])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_of_as_many_sequences_as_it_takes(d, last):
+    """4096 of them: one token each, and one more (the form of 128-row tiles)."""
+    n = 4096
+    Step([1] * (n - 1) + [last], [2 + i % 40 for i in range(n)], 2, 1, d, 16, torch.float16,
+         k=32).check("spyre")
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("page", [16, 6])

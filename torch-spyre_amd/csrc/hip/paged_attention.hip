@@ -48,10 +48,14 @@
 //     once.
 //
 // What bounds it (32 query heads over 8 of 128): decoding and trees of one long sequence
-// the bytes of K and V, 64 ragged sequences of up to 4000 keys 121 us (530 MB, 4.4
-// TB/s), 131072 keys 104 us for a token and 116 for a tree of 16; four sequences of 1152
-// keys the latency of two kernels, 18 us; pieces of prompts the softmax beside the products, 3 x
-// 777 tokens over 2825 keys 188 us (93 GFLOP, matrix cores busy a fifth of the time).
+// the bytes of K and V, 64 ragged sequences of up to 4000 keys 122 us (530 MB, 4.3
+// TB/s), 131072 keys 105 us for a token and 115 for a tree of 16; four sequences of 1152
+// keys the latency of two kernels, 18 us.  Pieces of prompts, 3 x 777 tokens over 2825 keys, 189 us
+// (93 GFLOP, 24 us of it the merge), are bound by latency: scores, softmax and second product
+// of a wave follow each other, two waves a SIMD, which issue vector instructions 40 % of the
+// time and keep the matrix cores busy 25 %.  Whole prompts are bound by the planning: for each
+// unit head_items and locate walk all tiles of a KV head, some 0.9 us a tile, 1.7 of the
+// 2.06 ms of 8192 tokens and 0.27 of the 0.51 of four times 2048.
 #include <algorithm>
 #include <type_traits>
 
@@ -968,12 +972,12 @@ __global__ void __launch_bounds__(PT) paged_attn_merge(const PagedArgs p, int gr
 }
 
 // The host knows how many tokens come, not whose they are.  One a sequence at most: the form
-// for them (64 ragged sequences of up to 4000 keys 122 us, 141 in the other; as many heads of
-// keys as of queries 99 and 104; 131072 keys 104 and 106).  More are trees or pieces of
-// prompts, perhaps among single tokens: 4 of 131072 keys take 106 and 107 us, 16 of them 183
-// and 116, 63 single tokens beside a piece of 150 take 205 and 127 (2000 keys each).  (A third
-// form, 32 rows a wave without LDS, was ahead of both at 6 tokens a sequence only, 157 us to
-// 169, and took 235 for 63 tokens beside a piece of 512, which now take 152.)
+// for them (64 ragged sequences of up to 4000 keys 123 us, 142 in the other; as many heads of
+// keys as of queries 100 and 104; 131072 keys 105 and 110).  More are trees or pieces of
+// prompts, perhaps among single tokens: 16 tokens of 131072 keys take 183 and 115, 63 single tokens
+// beside a piece of 40 / 150 / 512 / 900 (2000 keys each) 145 / 206 / 261 / 333 and 113 / 125 /
+// 153 / 180.  Where every sequence brings 2 to 4 tokens the form for single ones would be
+// ahead: 64 ragged ones of 2 127 and 150, of 4 132 and 165, of 6 160 and 170.
 int form_of(int64_t tokens, int64_t batch, int64_t g) {
   return tokens <= batch && g <= 16 ? DECODE : WIDE;
 }
